@@ -435,6 +435,85 @@ int mote_cuda_gqa_attention_prefill_f16(const void* q, const void* k_cache, cons
                                         uint64_t row0, uint64_t cache_rows, float scale,
                                         void* stream);
 
+/* ---- KV cache held in 8 bits ----------------------------------------------
+ * No reference counterpart (KV-cache operations are planned primitives,
+ * docs/roadmap.md:60).  Paged, with one f32 scale for each block of tokens and
+ * head:
+ *   k_cache, v_cache   int8 [num_blocks, kv_heads, block_tokens, head_dim]
+ *   k_scales, v_scales f32  [num_blocks, kv_heads]; a value is q * scale
+ *   block_tables       int32 [batch, max_blocks]: position p of sequence b is
+ *                      row p % block_tokens of block block_tables[b][p / block_tokens]
+ * head_dim 64 or 128; block_tokens a multiple of 16 from 16 to 256; caches and
+ * f16 tensors 16-byte aligned, the others 4-byte; batch <= 2^20; null pointers
+ * and other shapes -> 1.  A sequence whose offsets or lengths are out of range is skipped,
+ * and so is a block whose number is; either sets *error_flag (uint32) to 1
+ * or, without one, bit 1 of the device status.  Caches need no
+ * initialisation.  A block that is appended to belongs to one sequence; full
+ * blocks may be shared.
+ *
+ * Append: the rows seq_starts[b] .. seq_starts[b + 1] - 1 of k_new / v_new
+ * ([tokens, kv_heads, head_dim] f16; seq_starts int32 [batch + 1], ascending)
+ * become the last positions of sequence b, whose length with them is
+ * seq_lens[b] (int32 [batch]).  A block's scale is the largest |x| / 127 that
+ * it received since its first row was written; q = rint(x / scale).  When it
+ * grows, the block's earlier rows are rounded again on the new scale (the
+ * rows behind the new ones keep their bytes).  An infinity or a NaN makes the
+ * block read as NaN for its head until its first row is written again.
+ * tokens == 0 returns 0. */
+int mote_cuda_kv_cache_append_q8(const void* k_new, const void* v_new, void* k_cache,
+                                 void* v_cache, void* k_scales, void* v_scales,
+                                 const void* block_tables, const void* seq_starts,
+                                 const void* seq_lens, uint64_t tokens, uint64_t batch,
+                                 uint64_t kv_heads, uint64_t head_dim, uint64_t num_blocks,
+                                 uint64_t block_tokens, uint64_t max_blocks, void* error_flag,
+                                 void* stream);
+/* Reads back in f16: the first starts[b + 1] - starts[b] positions of sequence
+ * b to the rows starts[b] .. of k_out / v_out ([tokens, kv_heads, head_dim]
+ * f16), what mote_cuda_gqa_attention_packed_f16 takes for a prompt continued
+ * over cached positions.  Rows of no sequence keep their values. */
+int mote_cuda_kv_cache_read_q8(const void* k_cache, const void* v_cache, const void* k_scales,
+                               const void* v_scales, const void* block_tables, const void* starts,
+                               void* k_out, void* v_out, uint64_t tokens, uint64_t batch,
+                               uint64_t kv_heads, uint64_t head_dim, uint64_t num_blocks,
+                               uint64_t block_tokens, uint64_t max_blocks, void* error_flag,
+                               void* stream);
+/* Decode attention over that cache, one query token per sequence:
+ *   out[b, h] = softmax(scale * q[b, h] . K_b[:len_b, h / (q_heads / kv_heads)]) . V_b
+ * q / out [batch, q_heads, head_dim] f16; seq_lens int32 [batch], len_b at
+ * most max_blocks * block_tokens; a sequence of length 0 gets zeros.  Positions
+ * of a block outside [0, num_blocks) count as not there and set bit 1 of the
+ * device status.  q_heads % kv_heads == 0, q_heads and batch <= 65535, scale
+ * finite.  Workspace: mote_cuda_gqa_attention_decode_q8_workspace_bytes bytes
+ * (0: none). */
+int mote_cuda_gqa_attention_decode_q8_workspace_bytes(uint64_t batch, uint64_t q_heads,
+                                                      uint64_t kv_heads, uint64_t head_dim,
+                                                      uint64_t* bytes);
+int mote_cuda_gqa_attention_decode_q8(const void* q, const void* k_cache, const void* v_cache,
+                                      const void* k_scales, const void* v_scales,
+                                      const void* block_tables, const void* seq_lens, void* out,
+                                      uint64_t batch, uint64_t q_heads, uint64_t kv_heads,
+                                      uint64_t head_dim, uint64_t num_blocks,
+                                      uint64_t block_tokens, uint64_t max_blocks, float scale,
+                                      void* workspace, uint64_t workspace_bytes, void* stream);
+/* Causal attention over packed prompts of different lengths: sequence b has
+ * the queries q_starts[b] .. q_starts[b + 1] - 1 of q / out [tokens, q_heads,
+ * head_dim] f16 and the positions kv_starts[b] .. kv_starts[b + 1] - 1 of k /
+ * v [kv_tokens, kv_heads, head_dim] f16; with n_q and n_k of them, query i
+ * stands at position n_k - n_q + i:
+ *   out[i, h] = softmax_{p <= n_k - n_q + i}(scale * q[i, h] . k[p, h / g]) . v[p, h / g]
+ * A query before the first position gets zeros; rows of no sequence keep
+ * their values; what k and v hold past a query's position does not reach it.
+ * Offsets int32 [batch + 1] on the device, ascending; a sequence whose
+ * offsets are out of range is skipped and sets bit 1 of the device status.
+ * head_dim 64 or 128, q_heads a multiple of kv_heads and at most 128 times
+ * it, q_heads <= 65535, batch <= 2^20, scale > 0, 16-byte aligned tensors;
+ * tokens == 0 returns 0; null pointers and other shapes -> 1. */
+int mote_cuda_gqa_attention_packed_f16(const void* q, const void* k, const void* v,
+                                       const void* q_starts, const void* kv_starts, void* out,
+                                       uint64_t tokens, uint64_t kv_tokens, uint64_t batch,
+                                       uint64_t q_heads, uint64_t kv_heads, uint64_t head_dim,
+                                       float scale, void* stream);
+
 /* ---- multi-GPU exchange for column-sharded linears ----------------------
  * The reference is single-device (crates/mote-backend-hip/src/context.rs:13-80
  * holds one device and one stream); these entry points are new.  Each rank

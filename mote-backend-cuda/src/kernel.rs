@@ -48,6 +48,10 @@ const KERNELS: &[(&str, DType, &str, usize, Call)] = &[
     ("kv_cache_append", DType::F16, "mote_cuda_kv_cache_append_f16", 11, call_kv_cache_append_f16),
     ("gqa_attention_decode", DType::F16, "mote_cuda_gqa_attention_decode_f16", 15, call_gqa_attention_decode_f16),
     ("gqa_attention_prefill", DType::F16, "mote_cuda_gqa_attention_prefill_f16", 13, call_gqa_attention_prefill_f16),
+    ("kv_cache_append_q8", DType::F16, "mote_cuda_kv_cache_append_q8", 18, call_kv_cache_append_q8),
+    ("kv_cache_read_q8", DType::F16, "mote_cuda_kv_cache_read_q8", 17, call_kv_cache_read_q8),
+    ("gqa_attention_decode_q8", DType::F16, "mote_cuda_gqa_attention_decode_q8", 19, call_gqa_attention_decode_q8),
+    ("gqa_attention_packed", DType::F16, "mote_cuda_gqa_attention_packed_f16", 14, call_gqa_attention_packed_f16),
     ("decoder_stack_q4_0", DType::F16, "mote_cuda_q4_0_decoder_stack_f16", 12, call_q4_0_decoder_stack_f16),
 ];
 
@@ -211,6 +215,22 @@ fn call_gqa_attention_decode_f16(w: &[usize]) -> i32 {
 fn call_gqa_attention_prefill_f16(w: &[usize]) -> i32 {
     // SAFETY: the caller's words follow the entry point's argument list.
     unsafe { ffi::mote_cuda_gqa_attention_prefill_f16(w[0] as *const c_void, w[1] as *const c_void, w[2] as *const c_void, w[3] as *mut c_void, w[4] as u64, w[5] as u64, w[6] as u64, w[7] as u64, w[8] as u64, w[9] as u64, w[10] as u64, f32::from_bits(w[11] as u32), w[12] as *mut c_void) }
+}
+fn call_kv_cache_append_q8(w: &[usize]) -> i32 {
+    // SAFETY: the caller's words follow the entry point's argument list.
+    unsafe { ffi::mote_cuda_kv_cache_append_q8(w[0] as *const c_void, w[1] as *const c_void, w[2] as *mut c_void, w[3] as *mut c_void, w[4] as *mut c_void, w[5] as *mut c_void, w[6] as *const c_void, w[7] as *const c_void, w[8] as *const c_void, w[9] as u64, w[10] as u64, w[11] as u64, w[12] as u64, w[13] as u64, w[14] as u64, w[15] as u64, w[16] as *mut c_void, w[17] as *mut c_void) }
+}
+fn call_kv_cache_read_q8(w: &[usize]) -> i32 {
+    // SAFETY: the caller's words follow the entry point's argument list.
+    unsafe { ffi::mote_cuda_kv_cache_read_q8(w[0] as *const c_void, w[1] as *const c_void, w[2] as *const c_void, w[3] as *const c_void, w[4] as *const c_void, w[5] as *const c_void, w[6] as *mut c_void, w[7] as *mut c_void, w[8] as u64, w[9] as u64, w[10] as u64, w[11] as u64, w[12] as u64, w[13] as u64, w[14] as u64, w[15] as *mut c_void, w[16] as *mut c_void) }
+}
+fn call_gqa_attention_decode_q8(w: &[usize]) -> i32 {
+    // SAFETY: the caller's words follow the entry point's argument list.
+    unsafe { ffi::mote_cuda_gqa_attention_decode_q8(w[0] as *const c_void, w[1] as *const c_void, w[2] as *const c_void, w[3] as *const c_void, w[4] as *const c_void, w[5] as *const c_void, w[6] as *const c_void, w[7] as *mut c_void, w[8] as u64, w[9] as u64, w[10] as u64, w[11] as u64, w[12] as u64, w[13] as u64, w[14] as u64, f32::from_bits(w[15] as u32), w[16] as *mut c_void, w[17] as u64, w[18] as *mut c_void) }
+}
+fn call_gqa_attention_packed_f16(w: &[usize]) -> i32 {
+    // SAFETY: the caller's words follow the entry point's argument list.
+    unsafe { ffi::mote_cuda_gqa_attention_packed_f16(w[0] as *const c_void, w[1] as *const c_void, w[2] as *const c_void, w[3] as *const c_void, w[4] as *const c_void, w[5] as *mut c_void, w[6] as u64, w[7] as u64, w[8] as u64, w[9] as u64, w[10] as u64, w[11] as u64, f32::from_bits(w[12] as u32), w[13] as *mut c_void) }
 }
 fn call_q4_0_decoder_stack_f16(w: &[usize]) -> i32 {
     // SAFETY: the caller's words follow the entry point's argument list.

@@ -87,6 +87,16 @@ SIGNATURES: dict[str, tuple] = {
                                                            ctypes.POINTER(U64)]),
     "mote_cuda_gqa_attention_decode_f16": (I, [P, P, P, P, P, U64, U64, U64, U64, U64, U64,
                                                ctypes.c_float, P, U64, P]),
+    "mote_cuda_kv_cache_append_q8":
+        (I, [P, P, P, P, P, P, P, P, P, U64, U64, U64, U64, U64, U64, U64, P, P]),
+    "mote_cuda_kv_cache_read_q8":
+        (I, [P, P, P, P, P, P, P, P, U64, U64, U64, U64, U64, U64, U64, P, P]),
+    "mote_cuda_gqa_attention_decode_q8_workspace_bytes":
+        (I, [U64, U64, U64, U64, ctypes.POINTER(U64)]),
+    "mote_cuda_gqa_attention_decode_q8":
+        (I, [P, P, P, P, P, P, P, P, U64, U64, U64, U64, U64, U64, U64, F, P, U64, P]),
+    "mote_cuda_gqa_attention_packed_f16":
+        (I, [P, P, P, P, P, P, U64, U64, U64, U64, U64, U64, F, P]),
     "mote_cuda_gqa_attention_prefill_f16": (I, [P, P, P, P, U64, U64, U64, U64, U64, U64, U64,
                                                 ctypes.c_float, P]),
     "mote_cuda_q4_0_decoder_stack_workspace_bytes": (I, [U64, ctypes.POINTER(U64)]),

@@ -285,6 +285,33 @@ class CudaContext:
             self._attn_workspace = ws
         return ws.pointer, ws.size_bytes
 
+    def decode_q8_workspace_bytes(self, batch: int, q_heads: int, kv_heads: int,
+                                  head_dim: int) -> int:
+        """mote_cuda_gqa_attention_decode_q8_workspace_bytes, memoised (it
+        depends only on the shape and this context's device)."""
+        cache = self.__dict__.setdefault("_q8_need", {})
+        key = (batch, q_heads, kv_heads, head_dim)
+        need = cache.get(key)
+        if need is None:
+            out = ctypes.c_uint64(0)
+            self.inner.select()
+            errors.check(lib().mote_cuda_gqa_attention_decode_q8_workspace_bytes(
+                *key, ctypes.byref(out)), "query 8-bit attention workspace")
+            need = cache[key] = out.value
+        return need
+
+    def decode_q8_workspace(self, nbytes: int) -> tuple[int, int]:
+        """A zeroed device workspace of at least ``nbytes`` for the 8-bit
+        decode attention, grown on demand with a stream synchronisation (so
+        the first call of a larger shape comes before any graph capture).
+        Outgrown workspaces stay allocated: a captured graph may use them."""
+        held = self.__dict__.setdefault("_q8_workspaces", [])
+        if not held or held[-1].size_bytes < nbytes:
+            self.sync()
+            size = max(int(nbytes), 1 << 20)
+            held.append(CudaStorage(self.inner, size, np.zeros(size, np.uint8)))
+        return held[-1].pointer, held[-1].size_bytes
+
     def read_bytes(self, tensor: Tensor) -> bytes:
         storage = self.storage(tensor)
         return storage.read_bytes()[: tensor.desc.required_span_bytes]

@@ -13,3 +13,6 @@
 #include "dense_matmul.cu"
 #include "attention.cu"
 #include "attention_prefill.cu"
+#include "kv_cache_q8.cu"
+#include "attention_q8.cu"
+#include "attention_packed.cu"

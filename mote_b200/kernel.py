@@ -125,6 +125,10 @@ _ARG_KINDS = {
     "mote_cuda_kv_cache_append_f16": "pppppuuuupp",
     "mote_cuda_gqa_attention_decode_f16": "pppppuuuuuufpup",
     "mote_cuda_gqa_attention_prefill_f16": "ppppuuuuuuufp",
+    "mote_cuda_kv_cache_append_q8": "pppppppppuuuuuuupp",
+    "mote_cuda_kv_cache_read_q8": "ppppppppuuuuuuupp",
+    "mote_cuda_gqa_attention_decode_q8": "ppppppppuuuuuuufpup",
+    "mote_cuda_gqa_attention_packed_f16": "ppppppuuuuuufp",
     "mote_cuda_q4_0_decoder_stack_f16": "pwpuuuuufpup",
 }
 
@@ -157,6 +161,10 @@ CUDA_KERNELS = {
     ("kv_cache_append", DType.F16): "mote_cuda_kv_cache_append_f16",
     ("gqa_attention_decode", DType.F16): "mote_cuda_gqa_attention_decode_f16",
     ("gqa_attention_prefill", DType.F16): "mote_cuda_gqa_attention_prefill_f16",
+    ("kv_cache_append_q8", DType.F16): "mote_cuda_kv_cache_append_q8",
+    ("kv_cache_read_q8", DType.F16): "mote_cuda_kv_cache_read_q8",
+    ("gqa_attention_decode_q8", DType.F16): "mote_cuda_gqa_attention_decode_q8",
+    ("gqa_attention_packed", DType.F16): "mote_cuda_gqa_attention_packed_f16",
     ("decoder_stack_q4_0", DType.F16): "mote_cuda_q4_0_decoder_stack_f16",
 }
 

@@ -768,3 +768,201 @@ def gqa_attention_prefill_f16(context: CudaContext, q: Tensor, k_cache: Tensor, 
     errors.check(lib().mote_cuda_gqa_attention_prefill_f16(
         *ptrs, tokens, start, qh, kvh, hd, row0, rows, ctypes.c_float(scale), context.stream),
         "launch GQA prefill attention kernel")
+
+
+# ------------------------------------------------ KV cache held in 8 bits --
+def _q8_cache(k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: Tensor,
+              block_tables: Tensor) -> tuple[int, ...]:
+    """(num_blocks, kv_heads, block_tokens, head_dim, batch, max_blocks)."""
+    _plain(k_cache, "k_cache", DType.I8)
+    _rank(k_cache, "k_cache", 4)
+    _plain(v_cache, "v_cache", DType.I8)
+    _shape(v_cache, "v_cache", k_cache.shape)
+    blocks, kvh, bt, hd = k_cache.shape
+    _plain(k_scales, "k_scales", DType.F32)
+    _shape(k_scales, "k_scales", (blocks, kvh))
+    _plain(v_scales, "v_scales", DType.F32)
+    _shape(v_scales, "v_scales", (blocks, kvh))
+    _plain(block_tables, "block_tables", DType.I32)
+    _rank(block_tables, "block_tables", 2)
+    return (blocks, kvh, bt, hd, *block_tables.shape)
+
+
+def _i32_vector(tensor: Tensor, name: str, length: int) -> None:
+    _plain(tensor, name, DType.I32)
+    _shape(tensor, name, (length,))
+
+
+def _error_flag(context: CudaContext, name: str) -> int:
+    """A cleared device flag of this context (``name`` keeps one per operator)."""
+    flag = getattr(context, name, None)
+    if flag is None:
+        flag = _Flag(context)
+        setattr(context, name, flag)
+    context.inner.select()
+    errors.check(lib().mote_cuda_memset_async(flag.tensor.pointer, 0, 4, context.stream),
+                 "clear error flag")
+    return flag.tensor.pointer
+
+
+def _raise_flagged(context: CudaContext, name: str, blocks: int) -> None:
+    import numpy as np
+
+    if int(np.frombuffer(context.read_bytes(getattr(context, name).tensor), np.uint32)[0]):
+        raise errors.IndexOutOfRange(vocab=blocks)
+
+
+def kv_cache_append_q8(context: CudaContext, k_new: Tensor, v_new: Tensor, k_cache: Tensor,
+                       v_cache: Tensor, k_scales: Tensor, v_scales: Tensor, block_tables: Tensor,
+                       seq_starts: Tensor, seq_lens: Tensor, check: bool = True) -> None:
+    """Appends rows to a paged KV cache held in 8 bits, with one f32 scale
+    for each block of tokens and head.
+
+    Caches int8 [num_blocks, kv_heads, block_tokens, head_dim], scales f32
+    [num_blocks, kv_heads] (a value is ``q * scale``), ``block_tables`` int32
+    [batch, max_blocks]: position ``p`` of sequence ``b`` is row
+    ``p % block_tokens`` of block ``block_tables[b, p // block_tokens]``.
+    Rows ``seq_starts[b] .. seq_starts[b + 1] - 1`` of ``k_new``/``v_new``
+    ([tokens, kv_heads, head_dim] f16) become the last positions of sequence
+    ``b``, whose length with them is ``seq_lens[b]``.  A block's scale is the
+    largest ``|x| / 127`` it received since its first row was written; when it
+    grows, the block's earlier rows are rounded again.  A block that is
+    appended to belongs to one sequence.  With ``check`` the call
+    synchronizes and raises :class:`errors.IndexOutOfRange` for offsets,
+    lengths or blocks out of range (those rows are skipped); without it they
+    set the device status."""
+    blocks, kvh, bt, hd, batch, width = _q8_cache(k_cache, v_cache, k_scales, v_scales,
+                                                  block_tables)
+    _plain(k_new, "k_new", DType.F16)
+    _rank(k_new, "k_new", 3)
+    tokens = k_new.shape[0]
+    _shape(k_new, "k_new", (tokens, kvh, hd))
+    _plain(v_new, "v_new", DType.F16)
+    _shape(v_new, "v_new", k_new.shape)
+    _i32_vector(seq_starts, "seq_starts", batch + 1)
+    _i32_vector(seq_lens, "seq_lens", batch)
+    _not_aliased(k_cache, "k_cache", v_cache, "v_cache")
+    _not_aliased(k_scales, "k_scales", v_scales, "v_scales")
+    storage = context.storage
+    ptrs = [storage(t).pointer for t in (k_new, v_new, k_cache, v_cache, k_scales, v_scales,
+                                         block_tables, seq_starts, seq_lens)]
+    if tokens == 0:
+        return
+    flag = _error_flag(context, "_append_q8_flag") if check else None
+    context.inner.select()
+    st = lib().mote_cuda_kv_cache_append_q8(*ptrs, tokens, batch, kvh, hd, blocks, bt, width,
+                                            flag, context.inner.stream)
+    if st:
+        errors.check(st, "launch 8-bit KV-cache append kernel")
+    if check:
+        _raise_flagged(context, "_append_q8_flag", blocks)
+
+
+def kv_cache_read_q8(context: CudaContext, k_cache: Tensor, v_cache: Tensor, k_scales: Tensor,
+                     v_scales: Tensor, block_tables: Tensor, starts: Tensor, k_out: Tensor,
+                     v_out: Tensor, check: bool = True) -> None:
+    """Reads the 8-bit cache back in f16: the first ``starts[b + 1] -
+    starts[b]`` positions of sequence ``b`` to rows ``starts[b] ..`` of
+    ``k_out``/``v_out`` [tokens, kv_heads, head_dim] -- the K and V that
+    :func:`gqa_attention_packed_f16` takes for prompts continued over cached
+    positions.  Rows of no sequence keep their values; ``check`` as in
+    :func:`kv_cache_append_q8`."""
+    blocks, kvh, bt, hd, batch, width = _q8_cache(k_cache, v_cache, k_scales, v_scales,
+                                                  block_tables)
+    _plain(k_out, "k_out", DType.F16)
+    _rank(k_out, "k_out", 3)
+    tokens = k_out.shape[0]
+    _shape(k_out, "k_out", (tokens, kvh, hd))
+    _plain(v_out, "v_out", DType.F16)
+    _shape(v_out, "v_out", k_out.shape)
+    _i32_vector(starts, "starts", batch + 1)
+    _not_aliased(k_out, "k_out", v_out, "v_out")
+    storage = context.storage
+    ptrs = [storage(t).pointer for t in (k_cache, v_cache, k_scales, v_scales, block_tables,
+                                         starts, k_out, v_out)]
+    if tokens == 0:
+        return
+    flag = _error_flag(context, "_read_q8_flag") if check else None
+    context.inner.select()
+    st = lib().mote_cuda_kv_cache_read_q8(*ptrs, tokens, batch, kvh, hd, blocks, bt, width, flag,
+                                          context.inner.stream)
+    if st:
+        errors.check(st, "launch 8-bit KV-cache read kernel")
+    if check:
+        _raise_flagged(context, "_read_q8_flag", blocks)
+
+
+def gqa_attention_decode_q8(context: CudaContext, q: Tensor, k_cache: Tensor, v_cache: Tensor,
+                            k_scales: Tensor, v_scales: Tensor, block_tables: Tensor,
+                            seq_lens: Tensor, output: Tensor, scale: float | None = None) -> None:
+    """One query token per sequence over the 8-bit cache of
+    :func:`kv_cache_append_q8` (grouped-query): ``output[b, h] =
+    softmax(scale * q[b, h] . K_b[:seq_lens[b], h // g]) . V_b`` with ``g =
+    q_heads // kv_heads``; q and output [batch, q_heads, head_dim] f16.  A
+    sequence of length 0 gets zeros; blocks out of range count as not there
+    and set the device status.  ``scale`` defaults to ``1 / sqrt(head_dim)``."""
+    blocks, kvh, bt, hd, batch, width = _q8_cache(k_cache, v_cache, k_scales, v_scales,
+                                                  block_tables)
+    _plain(q, "q", DType.F16)
+    _rank(q, "q", 3)
+    qh = q.shape[1]
+    _shape(q, "q", (batch, qh, hd))
+    _plain(output, "output", DType.F16)
+    _shape(output, "output", q.shape)
+    _i32_vector(seq_lens, "seq_lens", batch)
+    _not_aliased(output, "output", q, "q")
+    storage = context.storage
+    ptrs = [storage(t).pointer for t in (q, k_cache, v_cache, k_scales, v_scales, block_tables,
+                                         seq_lens, output)]
+    if batch == 0 or qh == 0:
+        return
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    need = context.decode_q8_workspace_bytes(batch, qh, kvh, hd)
+    ws_ptr, ws_bytes = context.decode_q8_workspace(need) if need else (None, 0)
+    context.inner.select()
+    st = lib().mote_cuda_gqa_attention_decode_q8(*ptrs, batch, qh, kvh, hd, blocks, bt, width,
+                                                 scale, ws_ptr, ws_bytes, context.inner.stream)
+    if st:
+        errors.check(st, "launch 8-bit GQA decode attention kernel")
+
+
+def gqa_attention_packed_f16(context: CudaContext, q: Tensor, k: Tensor, v: Tensor,
+                             q_starts: Tensor, kv_starts: Tensor, output: Tensor,
+                             scale: float | None = None) -> None:
+    """Causal attention over packed prompts of different lengths: sequence
+    ``b`` has rows ``q_starts[b] .. q_starts[b + 1] - 1`` of ``q``/``output``
+    [tokens, q_heads, head_dim] f16 and rows ``kv_starts[b] ..`` of ``k``/``v``
+    [kv_tokens, kv_heads, head_dim] f16; with ``n_q`` and ``n_k`` of them,
+    query ``i`` stands at position ``n_k - n_q + i`` and attends the
+    positions up to its own (``n_k == n_q``: a whole prompt; ``n_k > n_q``: a
+    prompt continued over cached positions).  A query before the first
+    position gets zeros; rows of no sequence keep their values.  Offsets
+    int32 [batch + 1]; a sequence with offsets out of range is skipped and
+    sets the device status.  ``scale`` defaults to ``1 / sqrt(head_dim)``."""
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _plain(t, name, DType.F16)
+        _rank(t, name, 3)
+    _plain(output, "output", DType.F16)
+    _shape(output, "output", q.shape)
+    tokens, qh, hd = q.shape
+    kv_tokens, kvh, _ = k.shape
+    _shape(k, "k", (kv_tokens, kvh, hd))
+    _shape(v, "v", k.shape)
+    _plain(q_starts, "q_starts", DType.I32)
+    _rank(q_starts, "q_starts", 1)
+    batch = q_starts.shape[0] - 1
+    if batch < 0:
+        raise errors.ShapeMismatch(tensor="q_starts", expected=(1,), actual=q_starts.shape)
+    _i32_vector(kv_starts, "kv_starts", batch + 1)
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _not_aliased(output, "output", t, name)
+    storage = context.storage
+    ptrs = [storage(t).pointer for t in (q, k, v, q_starts, kv_starts, output)]
+    if tokens == 0 or qh == 0 or batch == 0:
+        return
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    context.inner.select()
+    st = lib().mote_cuda_gqa_attention_packed_f16(*ptrs, tokens, kv_tokens, batch, qh, kvh, hd,
+                                                  scale, context.inner.stream)
+    if st:
+        errors.check(st, "launch packed GQA attention kernel")
