@@ -7,21 +7,21 @@
 // HBM-bound: K and V of the attended positions are read once; 8 query heads
 // share each read.  Everything else is arranged so that the stream never
 // waits:
-// * The work is cut in units of 2048 / head_dim positions (2 KB of K and 2 KB
-//   of V) of one (sequence, KV head, up to 8 query heads) "row".  Every CTA
-//   takes an equal run of consecutive units, found from the lengths on the
-//   device, so ragged batches balance and no length bound is needed on the
-//   host.  The 8 warps of a CTA take its units in turn, each through a ring of
-//   three stages filled with cp.async.
+// * The work is cut in units of 4096 / head_dim positions of one (sequence, KV head, up to
+//   8 query heads) "row".  One CTA per
+//   SM takes an equal share of consecutive units, found from the lengths on
+//   the device, so ragged batches balance and the host needs no bound on the
+//   lengths.  The 12 warps of a CTA take a row's units in turn, each through a
+//   ring of 16 KB that runs ahead across rows; the lane that holds a block's
+//   number issues its TMA loads (128-byte swizzle) and its scales.
 // * The 8-bit values become f16 exactly (the byte as the low bits of
 //   1024 + u, minus 1152) and feed mma.sync.m16n8k16 as the A operand:
 //   S^T = K Q^T with 16 positions as rows and 8 heads as columns, then
 //   O^T += V^T P^T with 16 dimensions as rows, so no row of the products is
 //   idle whatever the grouping.  K's dimensions and V's positions are taken
-//   in the order in which a thread's 16-byte shared loads hold them (the
-//   products do not depend on it); P^T gets from the accumulator layout to the
-//   operand's with movmatrix.  Shared rows are swizzled so that these loads
-//   have no bank conflicts.
+//   in the order in which a thread's wide shared loads hold them without bank
+//   conflicts (the products do not depend on it); P^T gets from the
+//   accumulator layout to the operand's with movmatrix.
 // * scale * sk multiplies S in f32; sv multiplies P, relative to a power of
 //   two, before P is split into f16 high and low parts (two products, 22
 //   bits).  The running maximum moves only when a score passes it by more
@@ -29,24 +29,27 @@
 // * Rows that lie in several CTAs leave unnormalised parts in the workspace;
 //   the last CTA to finish joins them in order (a counter per row, left at
 //   zero), so results do not depend on timing.
+// Every wait is bounded; one that expires is reported in the device status
+// and the CTA runs on without waiting.
 #include "mote_common.cuh"
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
 namespace mote {
 namespace attn8 {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 12;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kHeads = 8;     // query heads of a row (columns of the products)
-constexpr int kStages = 3;
-constexpr int kTile = 2048;   // bytes of K (and of V) in a unit
-constexpr int kCtasPerSm = 2;
-constexpr int kMaxCtas = 1024;
-constexpr int kMinUnits = 32; // a CTA's share of a row that it splits
+constexpr int kTile = 4096;   // bytes of K (and of V) in a unit: 4096 / head_dim positions
+constexpr int kStages = 2;
+constexpr int kMaxCtas = 512;
+constexpr int kMinUnits = 2 * kWarps;  // rows of up to this many units are not split
+constexpr int kRowCost = 14;  // what a row's end costs a CTA, in units (3 us of 0.2 us)
 
 struct Params {
     const __half* q;
-    const std::int8_t* k_cache;
-    const std::int8_t* v_cache;
     const float* k_scales;
     const float* v_scales;
     const std::int32_t* tables;
@@ -60,13 +63,22 @@ struct Params {
 };
 
 struct Smem {
-    static constexpr int kRing = 0;  // [warp][stage][K tile, V tile]
-    static constexpr int kScales = kRing + kWarps * kStages * 2 * kTile;  // [warp][stage][4] f32
-    static constexpr int kMl = kScales + kWarps * kStages * 16;           // [m, l][warp][head] f32
-    static constexpr int kScan = kMl + 2 * kWarps * kHeads * 4;           // [16] u32
-    static constexpr int kFound = kScan + 64;                             // b, its first unit, last
-    static constexpr int kBytes = kFound + 32;
+    static constexpr int kRing = 0;  // [warp][stage][K tile, V tile], 1024-byte aligned
+    static constexpr int kFlush = kRing + kWarps * kStages * 2 * kTile;  // [warp][4 heads][HD] f32
+    static constexpr int kMl = kFlush + kWarps * 4 * 128 * 4;   // [warp][4 heads][m, l] f32
+    static constexpr int kScales = kMl + kWarps * 4 * 8;        // [warp][stage][4 tiles][K, V] f32
+    static constexpr int kBars = kScales + kWarps * kStages * 32;  // [warp][stage]
+    static constexpr int kLast = kBars + kWarps * kStages * 8;
+    static constexpr int kBytes = kLast + 16 + 1008;  // + alignment slack (of a 16-byte base)
 };
+static_assert(Smem::kBytes <= 232448, "shared memory");
+static_assert((kMaxCtas * kHeads + kThreads * 4 + kHeads) * 4 <= Smem::kMl - Smem::kFlush, "the join's scratch");
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
+}
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -77,6 +89,12 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ std::uint32_t transpose8x8(std::uint32_t a) {
     std::uint32_t d;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+
+__device__ __forceinline__ std::uint32_t half2_of(float a, float b) {
+    std::uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
     return d;
 }
 
@@ -93,25 +111,30 @@ __device__ __forceinline__ uint4 lds128(std::uint32_t addr) {
     return v;
 }
 
-__device__ __forceinline__ float lds_f32(std::uint32_t addr) {
-    return __uint_as_float(lds32(addr));
+__device__ __forceinline__ void tma_load_2d(std::uint32_t dst, const CUtensorMap* map, int x,
+                                            int y, std::uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
 }
 
 __device__ __forceinline__ void cp_async_4(std::uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// Byte offsets of a 16-byte chunk c of row r inside a K or V tile.  A quarter
-// of a warp reads K rows i and i + 4, and V rows 0..3 (mod 4) at two chunks.
-template <int HD>
-__device__ __forceinline__ std::uint32_t k_at(std::uint32_t r, std::uint32_t c) {
-    return HD == 128 ? r * 128 + ((c ^ (((r >> 2) & 1) << 2)) << 4)
-                     : (r >> 1) * 128 + (((r ^ (r >> 2)) & 1) << 6) + (c << 4);
+__device__ __forceinline__ void mbar_expect(std::uint32_t bar, std::uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-template <int HD>
-__device__ __forceinline__ std::uint32_t v_at(std::uint32_t r, std::uint32_t c) {
-    return HD == 128 ? r * 128 + ((c ^ ((r & 3) << 1)) << 4)
-                     : r * 64 + ((c ^ (r & 2)) << 4);
+
+// One arrival on `bar` when this thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(std::uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(std::uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void mma_acc(float (&d)[4], std::uint32_t a0, std::uint32_t a1,
@@ -123,6 +146,25 @@ __device__ __forceinline__ void mma_acc(float (&d)[4], std::uint32_t a0, std::ui
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Where a tile of 16 positions lies in shared memory (the 128-byte swizzle: a
+// 16-byte chunk's place in its 128-byte line is exchanged by the line's number)
+// and which positions a thread's rows and columns of the products stand for.
+// head_dim 128: position r is line r, row r of S^T is position r; a thread's
+// K chunks are 2 t and 2 t + 1.  head_dim 64: two positions to a line, rows
+// 2 i and 2 i + 1 of S^T are the positions i % 2 + 4 (i / 2) and that ^ 3.
+// Either way a quarter of a warp (half, for 8-byte loads) meets all 32 banks.
+template <int HD>
+struct Tile {
+    static __device__ __forceinline__ std::uint32_t at(std::uint32_t r, std::uint32_t c) {
+        return HD == 128 ? r * 128 + ((c ^ (r & 7)) << 4)
+                         : (r >> 1) * 128 + ((((r & 1) << 2 | c) ^ ((r >> 1) & 7)) << 4);
+    }
+    // the position of row 2 i + e, i < 4 (rows 8 + 2 i + e: 8 more)
+    static __device__ __forceinline__ std::uint32_t position(std::uint32_t i, std::uint32_t e) {
+        return HD == 128 ? 2 * i + e : ((i & 1) + 4 * (i >> 1)) ^ (3 * e);
+    }
+};
+
 // One warp's state over its units of a row: O^T accumulators (dimension
 // HD / 8 * (lane / 4) + 2 i + e of heads 2 (lane % 4), + 1), this lane's part
 // of the sums, the reference maxima and V's reference scale.
@@ -133,122 +175,179 @@ struct State {
     float wref;  // power of two: P is held times sv * wref; 0 until the first V scale
 };
 
+// 32 positions more, the first `live` of them attended, in two tiles of 16
+// whose scores are S times f0 and f1 and whose V scales are sv0 and sv1
+// (-infinity: the tile's block is not there).
 template <int HD>
-__device__ __forceinline__ void attend16(State<HD>& s, const std::uint32_t (&qf)[HD / 8],
-                                         std::uint32_t ktile, std::uint32_t vtile, int row0,
-                                         float f, float sv, std::int32_t live) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    // S^T: rows are the positions in the order p(r) = r / 2 + 4 (r % 2), + 8
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const std::uint32_t r0 = row0 + (g >> 1) + 4 * (g & 1);
+__device__ __forceinline__ void attend32(State<HD>& s, const std::uint32_t (&qf)[HD / 8],
+                                         std::uint32_t ktile, std::uint32_t vtile, float f0,
+                                         float f1, float sv0, float sv1, std::int32_t live) {
+    const std::uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const std::uint32_t r0 = Tile<HD>::position(g >> 1, g & 1);
+    float acc[2][4];
 #pragma unroll
-    for (int j = 0; j < HD / 64; ++j) {
-        const uint4 a = lds128(ktile + k_at<HD>(r0, t + 4 * j));
-        const uint4 b = lds128(ktile + k_at<HD>(r0 + 8, t + 4 * j));
-        const std::uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+    for (int k = 0; k < 2; ++k) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const std::uint32_t xa = aw[i] ^ 0x80808080u, xb = bw[i] ^ 0x80808080u;
-            mma_acc(acc, bytes_to_half2(xa, 0x4140u), bytes_to_half2(xb, 0x4140u),
-                    bytes_to_half2(xa, 0x4342u), bytes_to_half2(xb, 0x4342u),
-                    qf[(4 * j + i) * 2], qf[(4 * j + i) * 2 + 1]);
+        for (int i = 0; i < 4; ++i) acc[k][i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < HD / 64; ++j) {
+            const std::uint32_t c = HD == 128 ? 2 * t + j : t;
+            const uint4 a = lds128(ktile + k * 16 * HD + Tile<HD>::at(r0, c));
+            const uint4 b = lds128(ktile + k * 16 * HD + Tile<HD>::at(r0 + 8, c));
+            const std::uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const std::uint32_t xa = aw[i] ^ 0x80808080u, xb = bw[i] ^ 0x80808080u;
+                mma_acc(acc[k], bytes_to_half2(xa, 0x4140u), bytes_to_half2(xb, 0x4140u),
+                        bytes_to_half2(xa, 0x4342u), bytes_to_half2(xb, 0x4342u),
+                        qf[(4 * j + i) * 2], qf[(4 * j + i) * 2 + 1]);
+            }
         }
     }
-    float x[4];
+    // scores above the reference maxima, +infinity (or NaN) before there is one
+    float x[2][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = acc[i] * f;
-    const std::int32_t p0 = (g >> 1) + 4 * (g & 1);
-    if (live < 16) {
-        if (p0 >= live) x[0] = x[1] = -INFINITY;
-        if (p0 + 8 >= live) x[2] = x[3] = -INFINITY;
-    }
-    float t0 = fmaxf(x[0], x[2]), t1 = fmaxf(x[1], x[3]);
-    if (__any_sync(0xffffffffu, t0 > s.m[0] + 8.f || t1 > s.m[1] + 8.f)) {
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) {
-            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, d));
-            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, d));
+        for (int i = 0; i < 4; ++i) x[k][i] = fmaf(acc[k][i], k ? f1 : f0, -s.m[i & 1]);
+    const bool tail = live < 32 || sv0 == -INFINITY || sv1 == -INFINITY;  // uniform
+    const auto mask = [&](float (&y)[2][4]) {
+        const std::int32_t n0 = sv0 == -INFINITY ? 0 : live, n1 = sv1 == -INFINITY ? 0 : live - 16;
+        const std::int32_t r = static_cast<std::int32_t>(r0);
+        if (r >= n0) y[0][0] = y[0][1] = -INFINITY;
+        if (r + 8 >= n0) y[0][2] = y[0][3] = -INFINITY;
+        if (r >= n1) y[1][0] = y[1][1] = -INFINITY;
+        if (r + 8 >= n1) y[1][2] = y[1][3] = -INFINITY;
+    };
+    if (tail) mask(x);
+    const float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                            fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    if (__any_sync(0xffffffffu, top > 8.f)) {
+        float y[2][4];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[k][i] = acc[k][i] * (k ? f1 : f0);
+        if (tail) mask(y);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float m = fmaxf(fmaxf(y[0][h], y[0][2 + h]), fmaxf(y[1][h], y[1][2 + h]));
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            m = fmaxf(m, s.m[h]);
+            const float f = s.m[h] == m ? 1.f : ex2(s.m[h] - m);  // 0 from -infinity
+            s.m[h] = m;
+            s.l[h] *= f;
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i) s.o[i][h] *= f, s.o[i][2 + h] *= f;
+            // a maximum can still be -infinity only where no score is a number
+#pragma unroll
+            for (int k = 0; k < 2; ++k) x[k][h] = y[k][h] - m, x[k][2 + h] = y[k][2 + h] - m;
         }
-        t0 = fmaxf(t0, s.m[0]), t1 = fmaxf(t1, s.m[1]);
-        const float f0 = s.m[0] == t0 ? 1.f : ex2(s.m[0] - t0);  // 0 from -infinity
-        const float f1 = s.m[1] == t1 ? 1.f : ex2(s.m[1] - t1);
-        s.m[0] = t0, s.m[1] = t1;
-        s.l[0] *= f0, s.l[1] *= f1;
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i) s.o[i][0] *= f0, s.o[i][2] *= f0, s.o[i][1] *= f1, s.o[i][3] *= f1;
+        if (tail) mask(x);
     }
-    // V's scale relative to the reference: sv * wref in (2^5, 2^6] where the
-    // reference was set, at most 2^7, so P (below 2^8) times it fits f16 and
+    // V's scales relative to the reference: sv * wref in [2^5, 2^6) where the
+    // reference was set, at most 2^7, so P (up to 2^8) times it fits f16 and
     // keeps 22 bits down to 2^-14 of the row's largest
-    if (!(sv * s.wref <= 128.f) || s.wref == 0.f) {
-        const int e = min(max((__float_as_int(fabsf(sv)) >> 23) - 127, -100), 100);
-        const float w = __int_as_float((5 - e + 127) << 23);
-        const float r = s.wref == 0.f ? 1.f : w / s.wref;
-        if (sv != 0.f) {
-            s.wref = w;
+    float w0 = sv0 * s.wref, w1 = sv1 * s.wref;
+    if (!(fmaxf(w0, w1) <= 128.f) || s.wref == 0.f || tail) {
+        const float sv = !(sv0 == sv0) || !(sv1 == sv1) ? NAN : fmaxf(fmaxf(sv0, sv1), 0.f);
+        if (sv != 0.f && (s.wref == 0.f || !(sv * s.wref <= 128.f))) {
+            const int e = min(max((__float_as_int(sv) >> 23 & 255) - 127, -100), 100);
+            const float ref = __int_as_float((5 - e + 127) << 23);
+            const float r = s.wref == 0.f ? 1.f : ref / s.wref;
+            s.wref = ref;
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) s.o[i][k] *= r;
         }
+        // P is 0 where there is no block
+        w0 = sv0 == -INFINITY ? 0.f : sv0 * s.wref, w1 = sv1 == -INFINITY ? 0.f : sv1 * s.wref;
     }
-    const float m0 = s.m[0] == -INFINITY ? 0.f : s.m[0], m1 = s.m[1] == -INFINITY ? 0.f : s.m[1];
-    x[0] = ex2(x[0] - m0), x[2] = ex2(x[2] - m0);
-    x[1] = ex2(x[1] - m1), x[3] = ex2(x[3] - m1);
-    s.l[0] += x[0] + x[2], s.l[1] += x[1] + x[3];
-    const float w = sv * s.wref;
-    std::uint32_t hi[2], lo[2];
+    std::uint32_t hi[2][2], lo[2][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const float a = x[2 * i] * w, b = x[2 * i + 1] * w;
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi[i]) : "f"(b), "f"(a));
-        const float ra = a - half_bits_to_float(hi[i] & 0xffffu), rb = b - half_bits_to_float(hi[i] >> 16);
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo[i]) : "f"(rb), "f"(ra));
-        hi[i] = transpose8x8(hi[i]);
-        lo[i] = transpose8x8(lo[i]);
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[k][i] = ex2(x[k][i]);
+        s.l[0] += x[k][0] + x[k][2], s.l[1] += x[k][1] + x[k][3];
+        const float w = k ? w1 : w0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float a = x[k][2 * i] * w, b = x[k][2 * i + 1] * w;
+            hi[k][i] = half2_of(a, b);
+            lo[k][i] = half2_of(a - half_bits_to_float(hi[k][i] & 0xffffu),
+                                b - half_bits_to_float(hi[k][i] >> 16));
+            hi[k][i] = transpose8x8(hi[k][i]);
+            lo[k][i] = transpose8x8(lo[k][i]);
+        }
     }
-    // O^T += V^T P^T: this thread's positions t, t + 4, t + 8, t + 12, its
-    // dimensions the HD / 8 from HD / 8 * g on
+    // O^T += V^T P^T: this thread's four positions of a tile, its HD / 8
+    // dimensions from HD / 8 * g on
     constexpr int W = HD / 32;  // 4-byte words of a position
-    std::uint32_t v[4][W];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (HD == 128) {
-            const uint4 a = lds128(vtile + v_at<HD>(row0 + t + 4 * i, g));
-            v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w;
-        } else {
-            const uint2 a = lds64(vtile + v_at<HD>(row0 + t + 4 * i, g >> 1) + 8 * (g & 1));
-            v[i][0] = a.x, v[i][1] = a.y;
+    for (int k = 0; k < 2; ++k) {
+        std::uint32_t v[4][W];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const std::uint32_t r = Tile<HD>::position(t, i & 1) + 8 * (i >> 1);
+            const std::uint32_t at = vtile + k * 16 * HD;
+            if constexpr (HD == 128) {
+                const uint4 a = lds128(at + Tile<HD>::at(r, g));
+                v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w;
+            } else {
+                const uint2 a = lds64(at + Tile<HD>::at(r, g >> 1) + 8 * (g & 1));
+                v[i][0] = a.x, v[i][1] = a.y;
+            }
         }
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const std::uint32_t sel = e ? 0x7362u : 0x5140u;  // bytes 2e, 2e + 1 of two positions
+                const std::uint32_t ab = prmt(v[0][j], v[1][j], sel) ^ 0x80808080u;
+                const std::uint32_t cd = prmt(v[2][j], v[3][j], sel) ^ 0x80808080u;
+                const std::uint32_t a0 = bytes_to_half2(ab, 0x4140u), a1 = bytes_to_half2(ab, 0x4342u);
+                const std::uint32_t a2 = bytes_to_half2(cd, 0x4140u), a3 = bytes_to_half2(cd, 0x4342u);
+                mma_acc(s.o[2 * j + e], a0, a1, a2, a3, hi[k][0], hi[k][1]);
+                mma_acc(s.o[2 * j + e], a0, a1, a2, a3, lo[k][0], lo[k][1]);
+            }
     }
-#pragma unroll
-    for (int j = 0; j < W; ++j)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const std::uint32_t sel = e ? 0x7362u : 0x5140u;  // bytes 2e, 2e + 1 of two positions
-            const std::uint32_t ab = prmt(v[0][j], v[1][j], sel) ^ 0x80808080u;
-            const std::uint32_t cd = prmt(v[2][j], v[3][j], sel) ^ 0x80808080u;
-            const std::uint32_t a0 = bytes_to_half2(ab, 0x4140u), a1 = bytes_to_half2(ab, 0x4342u);
-            const std::uint32_t a2 = bytes_to_half2(cd, 0x4140u), a3 = bytes_to_half2(cd, 0x4342u);
-            mma_acc(s.o[2 * j + e], a0, a1, a2, a3, hi[0], hi[1]);
-            mma_acc(s.o[2 * j + e], a0, a1, a2, a3, lo[0], lo[1]);
-        }
 }
 
+// A row of the work list: sequence b's KV head and head group r, its length
+// and units, and the virtual unit at which it begins.
+struct Row {
+    std::uint32_t b, r, len, n, begin;
+};
+
 template <int HD>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Params p) {
-    constexpr int U = kTile / HD;  // positions of a unit
-    constexpr int SUB = U / 16;
+__global__ void __launch_bounds__(kThreads, 1)
+    decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                  const Params p) {
+    constexpr int kUnit = kTile / HD;  // positions of a unit, in kSub tiles of 16
+    constexpr int kSub = kUnit / 16;
     constexpr int kPart = kHeads * (HD + 2);
-    extern __shared__ __align__(128) std::uint8_t smem[];
-    const std::uint32_t sbase = smem_u32(smem);
+    extern __shared__ std::uint8_t smem_raw[];
+    const std::uint32_t raw = smem_u32(smem_raw);
+    const std::uint32_t sbase = (raw + 1023u) & ~1023u;
+    std::uint8_t* const smem = smem_raw + (sbase - raw);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const std::uint32_t ring = sbase + Smem::kRing + warp * (kStages * 2 * kTile);
-    const std::uint32_t scl = sbase + Smem::kScales + warp * (kStages * 16);
-    float* sm_m = reinterpret_cast<float*>(smem + Smem::kMl);
-    float* sm_l = sm_m + kWarps * kHeads;
-    std::uint32_t* scan = reinterpret_cast<std::uint32_t*>(smem + Smem::kScan);
-    unsigned long long* found = reinterpret_cast<unsigned long long*>(smem + Smem::kFound);
+    const std::uint32_t scl = sbase + Smem::kScales + warp * (kStages * 32);
+    std::uint64_t* const full = reinterpret_cast<std::uint64_t*>(smem + Smem::kBars) + warp * kStages;
+    const std::uint32_t bars = smem_u32(full);
+    float* const flush = reinterpret_cast<float*>(smem + Smem::kFlush);
+    float* const ml = reinterpret_cast<float*>(smem + Smem::kMl);
+    volatile std::uint32_t* last_cta = reinterpret_cast<std::uint32_t*>(smem + Smem::kLast);
+    if (lane < kStages) {
+        mbar_init(&full[lane], 2 * kSub);
+        fence_mbarrier_init();
+    }
+    if (threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<std::uint64_t>(&map_k)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<std::uint64_t>(&map_v)) : "memory");
+    }
     pdl_launch_dependents();
     pdl_wait();
 
@@ -258,99 +357,211 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
     const auto length = [&](std::uint32_t b) {
         return min(static_cast<std::uint32_t>(max(__ldg(p.seq_lens + b), 0)), cap);
     };
-    const auto units = [&](std::uint32_t len) { return (len + U - 1) / U; };
+    const auto units = [&](std::uint32_t len) { return (len + kUnit - 1) / kUnit; };
+    const auto warp_sum = [](std::uint32_t x) {
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
+        return x;
+    };
 
-    // all units and the longest row's
+    // ---- the CTA's share (scratch: the flush area) -------------------------
+    volatile std::uint32_t* found = reinterpret_cast<std::uint32_t*>(flush);
+    volatile std::uint32_t* scan = found + 2 * kWarps + 4;
+    // all units, the longest row's, the sequences with any
     std::uint32_t longest = 0;
-    unsigned long long total = 0;
+    std::uint32_t total = 0, filled = 0;
     for (std::uint32_t b = threadIdx.x; b < batch; b += kThreads) {
         const std::uint32_t n = units(length(b));
         total += n;
+        filled += n > 0;
         longest = max(longest, n);
     }
     longest = __reduce_max_sync(0xffffffffu, longest);
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) total += __shfl_xor_sync(0xffffffffu, total, d);
+    total = warp_sum(total);
+    filled = warp_sum(filled);
     if (lane == 0) {
         scan[warp] = longest;
-        reinterpret_cast<unsigned long long*>(sm_m)[warp] = total;
+        found[2 * warp] = total;
+        found[2 * warp + 1] = filled;
     }
     __syncthreads();
-    total = 0, longest = 0;
+    total = 0, filled = 0, longest = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
         longest = max(longest, scan[w]);
-        total += reinterpret_cast<unsigned long long*>(sm_m)[w];
+        total += found[2 * w];
+        filled += found[2 * w + 1];
     }
     total *= rows;
-    // equal shares; rows of up to kMinUnits units stay whole where they can
-    const unsigned long long share = (total + gridDim.x - 1) / gridDim.x;
-    const unsigned long long per = max(share, static_cast<unsigned long long>(min(longest, static_cast<std::uint32_t>(kMinUnits))));
-    const unsigned long long u0 = per * blockIdx.x, u1 = min(total, u0 + per);
-
+    filled *= rows;
+    __syncthreads();
     // sequences without positions
     for (std::uint32_t b = blockIdx.x; b < batch; b += gridDim.x)
         if (length(b) == 0)
             for (std::uint32_t i = threadIdx.x; i < p.q_heads * (HD / 8); i += kThreads)
                 reinterpret_cast<uint4*>(p.out + static_cast<std::uint64_t>(b) * p.q_heads * HD)[i] =
                     make_uint4(0, 0, 0, 0);
-    if (u0 >= u1) return;
+    if (total == 0) return;
+    // Equal shares of the units, where a row's end counts as kRowCost units
+    // more; or, where the rows are few, equal pieces of each row, one to a
+    // CTA, of the smallest size (in steps of 1 / kWarps) that needs no more
+    // CTAs than there are, unless shares are smaller by more than a row's end.
+    const std::uint32_t least = min(longest, static_cast<std::uint32_t>(kMinUnits));
+    std::uint32_t per = max((total + filled * kRowCost + gridDim.x - 1) / gridDim.x, least);
+    bool pieces = false;
+    if (filled <= gridDim.x) {
+        const std::uint32_t low = max((total + gridDim.x - 1) / gridDim.x, least);
+        const auto size = [&](int w) { return low + (low * w + kWarps - 1) / kWarps; };
+        std::uint32_t need = 0;
+        for (std::uint32_t b = lane; b < batch; b += 32)
+            need += (units(length(b)) + size(warp) - 1) / size(warp);
+        need = warp_sum(need) * rows;
+        if (lane == 0) scan[warp] = need <= gridDim.x;
+        __syncthreads();
+        int w = 0;
+        while (w < kWarps && !scan[w]) ++w;
+        pieces = w < kWarps && size(w) <= per + kRowCost;
+        if (pieces) per = size(w);
+        __syncthreads();
+    }
+    const auto extent = [&](std::uint32_t n) -> std::uint32_t {  // a row in virtual units
+        return pieces ? (n + per - 1) / per * per : n == 0 ? 0 : n + kRowCost;
+    };
 
-    // the sequence of unit u0
-    unsigned long long before = 0;  // units of the sequences before the chunk
+    // the row of virtual unit u0
+    const std::uint32_t u0 = per * blockIdx.x, u1 = u0 + per;
+    std::uint32_t before = 0;  // extents of the sequences before the chunk
+    if (threadIdx.x == 0) found[1] = 0;
     for (std::uint32_t base = 0;; base += kThreads) {
         const std::uint32_t b = base + threadIdx.x;
         const std::uint32_t n = b < batch ? units(length(b)) : 0u;
-        std::uint32_t incl = n;
+        const std::uint32_t mine = extent(n);
+        std::uint32_t incl = mine;
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
             const std::uint32_t y = __shfl_up_sync(0xffffffffu, incl, d);
             if (lane >= d) incl += y;
         }
+        if (lane == 31) found[4 + warp] = incl;
         __syncthreads();
-        if (lane == 31) scan[warp] = incl;
-        if (threadIdx.x == 0) found[1] = 0;
-        __syncthreads();
-        unsigned long long lower = before;
-        for (int w = 0; w < warp; ++w) lower += scan[w];
-        const unsigned long long end = (lower + incl) * rows, begin = (lower + incl - n) * rows;
+        std::uint32_t lower = before;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) lower += found[4 + w];
+            before += found[4 + w];
+        }
+        const std::uint32_t end = (lower + incl) * rows, begin = (lower + incl - mine) * rows;
         if (n > 0 && begin <= u0 && u0 < end) {
             found[0] = begin;
             found[1] = 1;
             found[2] = b;
         }
-        for (int w = 0; w < kWarps; ++w) before += scan[w];
         __syncthreads();
         if (found[1] || base + kThreads >= batch) break;
     }
-    std::uint32_t b = static_cast<std::uint32_t>(found[2]);
-    unsigned long long row_begin = found[0];
-    std::uint32_t len = length(b), n = units(len);
-    std::uint32_t r = static_cast<std::uint32_t>((u0 - row_begin) / n);
-    row_begin += static_cast<unsigned long long>(r) * n;
-
-    for (unsigned long long u = u0; u < u1;) {
-        // this CTA's units [v0, v1) of row (b, r)
-        const std::uint32_t v0 = static_cast<std::uint32_t>(u - row_begin);
-        const std::uint32_t v1 = static_cast<std::uint32_t>(min(u1 - row_begin, static_cast<unsigned long long>(n)));
-        const std::uint32_t kvh = r / p.head_groups;
-        const std::uint32_t head0 = (r % p.head_groups) * kHeads;  // in the group
-        const std::uint32_t heads = min(p.group - head0, static_cast<std::uint32_t>(kHeads));
-        const std::uint64_t q_row = static_cast<std::uint64_t>(b) * p.q_heads + kvh * p.group + head0;
-
-        // Q^T as the B operand, dimensions in the order of K's loads
-        std::uint32_t qf[HD / 8];
-#pragma unroll
-        for (int j = 0; j < HD / 64; ++j) {
-            uint4 a = make_uint4(0, 0, 0, 0), c = a;
-            if (static_cast<std::uint32_t>(g) < heads) {
-                const uint4* src = reinterpret_cast<const uint4*>(p.q + (q_row + g) * HD + 64 * j + 16 * t);
-                a = __ldg(src), c = __ldg(src + 1);
+    if (!found[1]) return;  // past the last unit
+    const auto next = [&](Row& x) {  // the next row with positions, begin ~0 behind the last
+        x.begin += extent(x.n);
+        if (++x.r < rows) return;
+        x.r = 0;
+        do {
+            if (++x.b >= batch) {
+                x.begin = ~0u;
+                return;
             }
-            const std::uint32_t w[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) qf[8 * j + i] = w[i];
+            x.len = length(x.b);
+            x.n = units(x.len);
+        } while (x.n == 0);
+    };
+    // this CTA's units [first, last) of a row
+    const auto first_of = [&](const Row& x) {
+        return x.begin >= u0 ? 0u : min(u0 - x.begin, x.n);
+    };
+    const auto last_of = [&](const Row& x) {
+        return min(u1 - x.begin, x.n);
+    };
+    Row row;
+    row.b = found[2];
+    row.len = length(row.b);
+    row.n = units(row.len);
+    row.r = (u0 - found[0]) / extent(row.n);
+    row.begin = found[0] + row.r * extent(row.n);
+    __syncthreads();  // the scratch is read
+
+    // ---- the stream: each warp keeps its ring full, across rows -------------
+    // the blocks of 32 / kSub units of this warp, from held_unit of sequence
+    // held_b on: one lane for each 16 positions (-1: none)
+    std::uint32_t a_unit = first_of(row) + warp, a_last = last_of(row), a_slot = 0, a_stage = 0;
+    std::uint32_t a_kvh = row.r / p.head_groups;
+    Row ahead = row;
+    std::int32_t held_block = -1;
+    std::uint32_t held_row = 0, held_b = ~0u, held_unit = 0;
+    const auto issue = [&]() {
+        while (a_unit >= a_last) {
+            if (ahead.begin >= u1) return;
+            next(ahead);
+            if (ahead.begin >= u1) return;
+            a_unit = warp, a_last = last_of(ahead), a_slot = 0, a_kvh = ahead.r / p.head_groups;
         }
+        if (a_slot == 0 && (held_b != ahead.b || held_unit != a_unit)) {
+            held_b = ahead.b, held_unit = a_unit;
+            const std::uint32_t pos = (a_unit + lane / kSub * kWarps) * kUnit + 16 * (lane % kSub);
+            held_block = -1;
+            if (pos < ahead.len) {
+                const std::uint32_t i = pos / bt;
+                held_row = pos - i * bt;
+                held_block = __ldg(p.tables + static_cast<std::uint64_t>(ahead.b) * p.c.max_blocks + i);
+                if (held_block < 0 || static_cast<std::uint64_t>(held_block) >= p.c.num_blocks) {
+                    held_block = -1;
+                    atomicOr(&g_device_status, kDevIndexOutOfRange);
+                }
+            }
+        }
+        const std::uint32_t i = lane - a_slot;
+        if (i < kSub) {
+            const std::uint32_t bar = bars + 8 * a_stage;
+            const std::uint32_t kt = ring + a_stage * 2 * kTile + i * (kTile / kSub);
+            const std::uint32_t sc = scl + a_stage * 32 + i * 8;
+            if (held_block >= 0) {
+                const std::uint64_t tile = static_cast<std::uint64_t>(held_block) * p.c.kv_heads + a_kvh;
+                const int y = static_cast<int>((tile * bt + held_row) * HD / 128);
+                mbar_expect(bar, 2 * kTile / kSub);
+                tma_load_2d(kt, &map_k, 0, y, bar);
+                tma_load_2d(kt + kTile, &map_v, 0, y, bar);
+                cp_async_4(sc, p.k_scales + tile);
+                cp_async_4(sc + 4, p.v_scales + tile);
+                cp_async_arrive(bar);
+            } else {  // nothing there: a V scale that no block has
+                asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(sc), "f"(0.f), "f"(-INFINITY) : "memory");
+                mbar_arrive(bar);
+                mbar_arrive(bar);
+            }
+        }
+        a_unit += kWarps;
+        a_slot = (a_slot + kSub) % 32;
+        a_stage = a_stage == kStages - 1 ? 0 : a_stage + 1;
+    };
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < kStages - 1; ++k) issue();
+
+    // Q^T as the B operand, dimensions in the order of K's loads
+    std::uint32_t qf[HD / 8];
+    const auto load_q = [&](const Row& x) {
+        const std::uint32_t head = (x.r % p.head_groups) * kHeads + g;
+        const uint4* src = reinterpret_cast<const uint4*>(
+            p.q + (static_cast<std::uint64_t>(x.b) * p.q_heads + x.r / p.head_groups * p.group + head) * HD + HD / 4 * t);
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+            const uint4 a = head < p.group ? __ldg(src + j) : make_uint4(0, 0, 0, 0);
+            qf[4 * j] = a.x, qf[4 * j + 1] = a.y, qf[4 * j + 2] = a.z, qf[4 * j + 3] = a.w;
+        }
+    };
+    if (first_of(row) >= last_of(row)) next(row);  // only that row's end falls to this CTA
+    if (row.begin < u1) load_q(row);
+    std::uint32_t stage = 0, parity = 0;
+    bool waiting = true;
+    while (row.begin < u1) {
+        const std::uint32_t v0 = first_of(row), v1 = last_of(row);
         State<HD> s;
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i)
@@ -360,213 +571,173 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_kernel(const Para
         s.l[0] = s.l[1] = 0.f;
         s.wref = 0.f;
 
-        const std::uint32_t mine = v1 - v0 > static_cast<std::uint32_t>(warp)
-                                       ? (v1 - v0 - warp + kWarps - 1) / kWarps : 0u;
-        // blocks of the next 32 / SUB units, one per lane and 16 positions
-        std::int32_t ahead_block = -1;
-        std::uint32_t ahead_row = 0;
-        std::uint32_t ok_bits = 0;  // of the last units issued, newest lowest
-        const auto issue = [&](std::uint32_t k) {
-            if (k < mine) {
-                constexpr std::uint32_t kAhead = 32 / SUB;
-                if (k % kAhead == 0) {
-                    const std::uint32_t pos =
-                        (v0 + warp + (k + lane / SUB) * kWarps) * U + 16 * (lane % SUB);
-                    ahead_block = -1;
-                    if (k + lane / SUB < mine && pos < len) {
-                        const std::uint32_t i = pos / bt;
-                        ahead_row = pos - i * bt;
-                        ahead_block = __ldg(p.tables + static_cast<std::uint64_t>(b) * p.c.max_blocks + i);
-                        if (ahead_block < 0 || static_cast<std::uint64_t>(ahead_block) >= p.c.num_blocks) {
-                            ahead_block = -1;
-                            atomicOr(&g_device_status, kDevIndexOutOfRange);
-                        }
-                    }
-                }
-                const std::uint32_t st = k % kStages;
-                const std::uint32_t kt = ring + st * 2 * kTile, vt = kt + kTile;
+        for (std::uint32_t v = v0 + warp; v < v1; v += kWarps) {
+            if (waiting) waiting = mbar_wait_bounded(&full[stage], parity, &g_device_status);
+            __syncwarp();  // the unit has landed; the stage before it is read by all lanes
+            issue();
+            const std::uint32_t kt = ring + stage * 2 * kTile;
+            const std::int32_t live = static_cast<std::int32_t>(row.len - v * kUnit);
 #pragma unroll
-                for (int i = 0; i < SUB; ++i) {
-                    const int from = (k % kAhead) * SUB + i;
-                    const std::int32_t block = __shfl_sync(0xffffffffu, ahead_block, from);
-                    const std::uint32_t row = __shfl_sync(0xffffffffu, ahead_row, from);
-                    ok_bits = ok_bits << 1 | (block >= 0 ? 1u : 0u);
-                    if (block >= 0) {
-                        const std::uint64_t tile = static_cast<std::uint64_t>(block) * p.c.kv_heads + kvh;
-                        const std::uint64_t at = (tile * bt + row) * HD + 16 * lane;
-#pragma unroll
-                        for (int j = 0; j < HD / 32; ++j) {  // 512 bytes a step
-                            const std::uint32_t byte = 512 * j + 16 * lane;
-                            const std::uint32_t rr = 16 * i + byte / HD, cc = byte % HD / 16;
-                            cp_async_16_default(kt + k_at<HD>(rr, cc), p.k_cache + at + 512 * j);
-                            cp_async_16_default(vt + v_at<HD>(rr, cc), p.v_cache + at + 512 * j);
-                        }
-                        if (lane < 2)
-                            cp_async_4(scl + st * 16 + i * 8 + lane * 4,
-                                       (lane ? p.v_scales : p.k_scales) + tile);
-                    }
-                }
-            } else {
-                ok_bits <<= SUB;
+            for (int k = 0; k < kSub / 2; ++k) {
+                if (k > 0 && live <= 32 * k) break;
+                const uint4 sc = lds128(scl + stage * 32 + k * 16);
+                attend32<HD>(s, qf, kt + k * 32 * HD, kt + kTile + k * 32 * HD,
+                             __uint_as_float(sc.x) * p.scale_log2, __uint_as_float(sc.z) * p.scale_log2,
+                             __uint_as_float(sc.y), __uint_as_float(sc.w), live - 32 * k);
             }
-            cp_async_commit();
-        };
-#pragma unroll
-        for (int k = 0; k < kStages - 1; ++k) issue(k);
-        for (std::uint32_t k = 0; k < mine; ++k) {
-            cp_async_wait<kStages - 2>();
-            __syncwarp();  // unit k has landed for all lanes; the stage before it is read
-            issue(k + kStages - 1);
-            const std::uint32_t st = k % kStages;
-            const std::uint32_t kt = ring + st * 2 * kTile;
-            const std::uint32_t pos = (v0 + warp + k * kWarps) * U;
-#pragma unroll
-            for (int i = 0; i < SUB; ++i)
-                if (ok_bits >> ((kStages - 1) * SUB + SUB - 1 - i) & 1u) {
-                    const float sk = lds_f32(scl + st * 16 + i * 8), sv = lds_f32(scl + st * 16 + i * 8 + 4);
-                    attend16<HD>(s, qf, kt, kt + kTile, 16 * i, sk * p.scale_log2, sv,
-                                 static_cast<std::int32_t>(len - pos) - 16 * i);
-                }
+            if (++stage == kStages) stage = 0, parity ^= 1;
         }
-        cp_async_wait<0>();
-        __syncwarp();
 
-        // the warps' states meet: each leaves O, its maxima and sums
+        // ---- the warps' states meet, four heads at a time -------------------
+        // (the ring already holds the next row's units, and its queries load)
+        const std::uint32_t head0 = (row.r % p.head_groups) * kHeads;  // in the group
+        const std::uint32_t heads = min(p.group - head0, static_cast<std::uint32_t>(kHeads));
+        const std::uint64_t q_row = static_cast<std::uint64_t>(row.b) * p.q_heads +
+                                    row.r / p.head_groups * p.group + head0;
+        const bool whole = v0 == 0 && v1 == row.n;
+        const std::uint32_t cta0 = row.begin / per, count = (row.begin + row.n - 1) / per - cta0 + 1;
+        next(row);
+        if (row.begin < u1) load_q(row);
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) {
             s.l[0] += __shfl_xor_sync(0xffffffffu, s.l[0], d);
             s.l[1] += __shfl_xor_sync(0xffffffffu, s.l[1], d);
         }
         const float unref = s.wref == 0.f ? 0.f : 1.f / s.wref;
-        float* mine_o = reinterpret_cast<float*>(smem + Smem::kRing + warp * (kStages * 2 * kTile));
-#pragma unroll
-        for (int i = 0; i < HD / 16; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                *reinterpret_cast<float2*>(mine_o + (2 * t + e) * HD + HD / 8 * g + 2 * i) =
-                    make_float2(s.o[i][e] * unref, s.o[i][2 + e] * unref);
-        if (g == 0) {
-            sm_m[warp * kHeads + 2 * t] = s.m[0], sm_m[warp * kHeads + 2 * t + 1] = s.m[1];
-            sm_l[warp * kHeads + 2 * t] = s.l[0], sm_l[warp * kHeads + 2 * t + 1] = s.l[1];
-        }
-        __syncthreads();
-        const bool whole = v0 == 0 && v1 == n;
-        const unsigned long long row_end = row_begin + n;
-        const std::uint32_t first = static_cast<std::uint32_t>(row_begin / per);
-        const std::uint32_t count = static_cast<std::uint32_t>((row_end - 1) / per) - first + 1;
         float* part = p.parts + static_cast<std::uint64_t>(2 * blockIdx.x + (v0 == 0 ? 1 : 0)) * kPart;
-        for (std::uint32_t i = threadIdx.x; i < heads * (HD / 4); i += kThreads) {
-            const std::uint32_t h = i / (HD / 4), d = i % (HD / 4) * 4;
-            float mt = -INFINITY, lt = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (std::uint32_t quad = 0; quad * 4 < heads; ++quad) {
+            // [head][pair of dimensions i][g]; the second two heads with i's
+            // lowest bit turned, for the banks
+            if (static_cast<std::uint32_t>(t >> 1) == quad) {
+                float* mine = flush + (warp * 4 + 2 * (t & 1)) * HD + 2 * g;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, sm_m[w * kHeads + h]);
+                for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                // a warp without a position has -infinity and zeros (NaN scores
-                // keep -infinity, and their NaN sums)
-                const float mw = sm_m[w * kHeads + h];
-                const float fw = mw == mt ? 1.f : mw == -INFINITY ? 0.f : ex2(mw - mt);
-                const float lw = sm_l[w * kHeads + h];
-                if (mw == -INFINITY && lw == 0.f) continue;
-                const float4 x = *reinterpret_cast<const float4*>(
-                    smem + Smem::kRing + w * (kStages * 2 * kTile) + (h * HD + d) * 4);
-                const float gw = lw != lw ? 1.f : fw;
-                lt = fmaf(lw, gw, lt);
-                o.x = fmaf(x.x, gw, o.x), o.y = fmaf(x.y, gw, o.y);
-                o.z = fmaf(x.z, gw, o.z), o.w = fmaf(x.w, gw, o.w);
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<float2*>(mine + e * HD + 16 * (i ^ (t & 1))) =
+                            make_float2(s.o[i][e] * unref, s.o[i][2 + e] * unref);
+                if (g == 0)
+                    *reinterpret_cast<float4*>(ml + (warp * 4 + 2 * (t & 1)) * 2) =
+                        make_float4(s.m[0], s.l[0], s.m[1], s.l[1]);
             }
-            if (whole) {
-                const float inv = lt == 0.f ? 0.f : 1.f / lt;
-                std::uint32_t y0, y1;
-                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y0) : "f"(o.y * inv), "f"(o.x * inv));
-                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y1) : "f"(o.w * inv), "f"(o.z * inv));
-                *reinterpret_cast<uint2*>(p.out + (q_row + h) * HD + d) = make_uint2(y0, y1);
-            } else {
-                *reinterpret_cast<float4*>(part + h * HD + d) = o;
-                if (d == 0) {
-                    part[kHeads * HD + h] = mt;
-                    part[kHeads * HD + kHeads + h] = lt;
+            __syncthreads();
+            const std::uint32_t hq = threadIdx.x / (HD / 2), c = threadIdx.x % (HD / 2);
+            const std::uint32_t h = quad * 4 + hq;
+            if (hq < 4 && h < heads) {
+                float mt = -INFINITY, lt = 0.f;
+                float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) mt = fmaxf(mt, ml[(w * 4 + hq) * 2]);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    // a warp without a position has -infinity and zeros (NaN
+                    // scores keep -infinity, and their NaN sums)
+                    const float2 a = *reinterpret_cast<const float2*>(ml + (w * 4 + hq) * 2);
+                    const float fw = a.y != a.y || a.x == mt ? 1.f : ex2(a.x - mt);
+                    const float2 x = *reinterpret_cast<const float2*>(flush + (w * 4 + hq) * HD + 2 * (c ^ (hq >> 1 << 3)));
+                    lt = fmaf(a.y, fw, lt);
+                    o.x = fmaf(x.x, fw, o.x), o.y = fmaf(x.y, fw, o.y);
+                }
+                if (whole) {
+                    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+                    *reinterpret_cast<std::uint32_t*>(p.out + (q_row + h) * HD + HD / 8 * (c & 7) + 2 * (c >> 3)) =
+                        half2_of(o.x * inv, o.y * inv);
+                } else {
+                    *reinterpret_cast<float2*>(part + h * HD + 2 * c) = o;
+                    if (c == 0)
+                        *reinterpret_cast<float2*>(part + kHeads * HD + 2 * h) = make_float2(mt, lt);
                 }
             }
+            if (quad * 4 + 4 < heads) __syncthreads();
         }
         if (!whole) {
-            __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
-                const unsigned done = atomicAdd(p.counters + first, 1u);
-                if (done == count - 1) p.counters[first] = 0;
-                scan[0] = done == count - 1;
+                __threadfence();  // the CTA's part, which the barrier has gathered
+                const unsigned done = atomicAdd(p.counters + cta0, 1u);
+                if (done == count - 1) p.counters[cta0] = 0;
+                *last_cta = done == count - 1;
+                __threadfence();
             }
             __syncthreads();
-            if (scan[0]) {
-                // join the row's parts: weights, then sums over every kGroups-th part
-                __threadfence();
+            if (*last_cta) {
+                // the last of the row's CTAs joins the parts: weights, then sums
+                // over every `groups`-th part, then over the groups
                 const auto part_of = [&](std::uint32_t j) {
-                    return p.parts + static_cast<std::uint64_t>(2 * (first + j) + (j == 0 ? 1 : 0)) * kPart;
+                    return p.parts + static_cast<std::uint64_t>(2 * (cta0 + j) + (j == 0 ? 1 : 0)) * kPart;
                 };
-                float* wts = reinterpret_cast<float*>(smem);  // [count][heads]
-                float* red = wts + kMaxCtas * kHeads;         // [kThreads][4]
-                if (static_cast<std::uint32_t>(warp) < heads) {
-                    float mt = -INFINITY, lt = 0.f;
-                    for (std::uint32_t j = lane; j < count; j += 32)
-                        mt = fmaxf(mt, __ldcg(part_of(j) + kHeads * HD + warp));
-#pragma unroll
-                    for (int d = 16; d > 0; d /= 2) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, d));
-                    for (std::uint32_t j = lane; j < count; j += 32) {
-                        const float mj = __ldcg(part_of(j) + kHeads * HD + warp);
-                        const float lj = __ldcg(part_of(j) + kHeads * HD + kHeads + warp);
-                        const float w = lj != lj ? 1.f : mj == mt ? 1.f : mj == -INFINITY ? 0.f : ex2(mj - mt);
-                        lt += lj * w;
-                        wts[j * kHeads + warp] = w;
-                    }
-#pragma unroll
-                    for (int d = 16; d > 0; d /= 2) lt += __shfl_xor_sync(0xffffffffu, lt, d);
-                    if (lane == 0) sm_l[warp] = lt == 0.f ? 0.f : 1.f / lt;
-                }
-                __syncthreads();
+                float* wts = flush;                    // [count][kHeads]
+                float* red = wts + kMaxCtas * kHeads;  // [kThreads][4]
+                float* invs = red + kThreads * 4;      // [kHeads]
                 const std::uint32_t cols = heads * (HD / 4);
                 const std::uint32_t groups = kThreads / cols;
                 const std::uint32_t col = threadIdx.x % cols, grp = threadIdx.x / cols;
-                const std::uint32_t h = col / (HD / 4), d = col % (HD / 4) * 4;
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (grp < groups)
-#pragma unroll 8
-                    for (std::uint32_t j = grp; j < count; j += groups) {
-                        const float4 x = __ldcg(reinterpret_cast<const float4*>(part_of(j) + h * HD + d));
-                        const float w = wts[j * kHeads + h];
-                        if (w != 0.f) {
-                            o.x = fmaf(x.x, w, o.x), o.y = fmaf(x.y, w, o.y);
-                            o.z = fmaf(x.z, w, o.z), o.w = fmaf(x.w, w, o.w);
-                        }
+                const std::uint32_t h = col / (HD / 4);
+                const auto load = [&](std::uint32_t j) {
+                    return __ldcg(reinterpret_cast<const float4*>(part_of(j)) + col);
+                };
+                constexpr int kFirst = 6;  // loads that run while the weights are found
+                float4 x[kFirst];
+#pragma unroll
+                for (int k = 0; k < kFirst; ++k)
+                    if (grp < groups && grp + k * groups < count) x[k] = load(grp + k * groups);
+                if (static_cast<std::uint32_t>(warp) < heads) {
+                    constexpr int kHeld = 8;  // of up to 256 parts in registers
+                    const auto ml_of = [&](std::uint32_t j) {
+                        return __ldcg(reinterpret_cast<const float2*>(part_of(j) + kHeads * HD) + warp);
+                    };
+                    float2 held[kHeld];
+                    float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+                    for (int k = 0; k < kHeld; ++k) {
+                        held[k] = lane + 32 * k < count ? ml_of(lane + 32 * k) : make_float2(-INFINITY, 0.f);
+                        mt = fmaxf(mt, held[k].x);
                     }
+                    for (std::uint32_t j = lane + 32 * kHeld; j < count; j += 32) mt = fmaxf(mt, ml_of(j).x);
+                    mt = warp_max(mt);
+                    const auto weigh = [&](const float2& a, std::uint32_t j) {
+                        const float w = a.y != a.y || a.x == mt ? 1.f : ex2(a.x - mt);
+                        lt += a.y * w;
+                        wts[j * kHeads + warp] = w;
+                    };
+#pragma unroll
+                    for (int k = 0; k < kHeld; ++k)
+                        if (lane + 32 * k < count) weigh(held[k], lane + 32 * k);
+                    for (std::uint32_t j = lane + 32 * kHeld; j < count; j += 32) weigh(ml_of(j), j);
+#pragma unroll
+                    for (int d = 16; d > 0; d /= 2) lt += __shfl_xor_sync(0xffffffffu, lt, d);
+                    if (lane == 0) invs[warp] = lt == 0.f ? 0.f : 1.f / lt;
+                }
+                __syncthreads();
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                const auto add = [&](const float4& y, std::uint32_t j) {
+                    const float w = wts[j * kHeads + h];
+                    o.x = fmaf(y.x, w, o.x), o.y = fmaf(y.y, w, o.y);
+                    o.z = fmaf(y.z, w, o.z), o.w = fmaf(y.w, w, o.w);
+                };
+                if (grp < groups) {
+#pragma unroll
+                    for (int k = 0; k < kFirst; ++k)
+                        if (grp + k * groups < count) add(x[k], grp + k * groups);
+#pragma unroll 4
+                    for (std::uint32_t j = grp + kFirst * groups; j < count; j += groups) add(load(j), j);
+                }
                 reinterpret_cast<float4*>(red)[threadIdx.x] = o;
                 __syncthreads();
                 if (threadIdx.x < cols) {
                     for (std::uint32_t k = 1; k < groups; ++k) {
-                        const float4 x = reinterpret_cast<const float4*>(red)[threadIdx.x + k * cols];
-                        o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+                        const float4 y = reinterpret_cast<const float4*>(red)[threadIdx.x + k * cols];
+                        o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
                     }
-                    const float inv = sm_l[h];
-                    std::uint32_t y0, y1;
-                    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y0) : "f"(o.y * inv), "f"(o.x * inv));
-                    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y1) : "f"(o.w * inv), "f"(o.z * inv));
-                    *reinterpret_cast<uint2*>(p.out + (q_row + h) * HD + d) = make_uint2(y0, y1);
+                    const float inv = invs[h];
+                    const std::uint32_t c = threadIdx.x % (HD / 4) * 2;  // pairs c and c + 1
+                    __half* dst = p.out + (q_row + h) * HD + HD / 8 * (c & 7) + 2 * (c >> 3);
+                    *reinterpret_cast<std::uint32_t*>(dst) = half2_of(o.x * inv, o.y * inv);
+                    *reinterpret_cast<std::uint32_t*>(dst + HD / 8) = half2_of(o.z * inv, o.w * inv);
                 }
             }
         }
-        __syncthreads();
-        // the next row
-        u = row_begin + v1;
-        if (u >= u1) break;
-        row_begin = row_end;
-        if (++r == rows) {
-            r = 0;
-            do {
-                len = length(++b);
-                n = units(len);
-            } while (n == 0);
-        }
+        __syncthreads();  // the flush area is free again
     }
 }
 
@@ -574,7 +745,7 @@ inline int ctas(int& n) {
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    n = sms * kCtasPerSm < kMaxCtas ? sms * kCtasPerSm : kMaxCtas;
+    n = sms < kMaxCtas ? sms : kMaxCtas;
     return static_cast<int>(e);
 }
 
@@ -582,14 +753,35 @@ inline std::uint64_t workspace_bytes(int n, std::uint64_t head_dim) {
     return kMaxCtas * 4 + static_cast<std::uint64_t>(n) * 2 * kHeads * (head_dim + 2) * 4;
 }
 
+// A cache as 128-byte lines, in boxes of 16 positions.
+inline int make_map(CUtensorMap* map, const void* cache, const kvq8::CacheShape& c) {
+    auto encode = gemm::encode_fn();
+    if (encode == nullptr) return static_cast<int>(cudaErrorNotSupported);
+    const std::uint64_t lines =
+        c.num_blocks * c.kv_heads * c.block_tokens * static_cast<std::uint64_t>(c.head_dim) / 128;
+    const cuuint32_t box[2] = {128, c.head_dim / 8};
+    const cuuint64_t dims[2] = {128, lines < box[1] ? box[1] : lines};  // no blocks: never loaded
+    const cuuint64_t strides[1] = {128};
+    const cuuint32_t estr[2] = {1, 1};
+    if (lines > 0x7fffffffull ||
+        encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(cache), dims, strides, box,
+               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return kInvalidValue;
+    return kSuccess;
+}
+
 template <int HD>
-int launch(const Params& p, int n, cudaStream_t stream) {
-    static_assert(Smem::kBytes >= (kMaxCtas * kHeads + kThreads * 4) * 4, "the join's scratch");
+int launch(const Params& p, const void* k_cache, const void* v_cache, int n, cudaStream_t stream) {
+    CUtensorMap map_k{}, map_v{};
+    int st = make_map(&map_k, k_cache, p.c);
+    if (st == kSuccess) st = make_map(&map_v, v_cache, p.c);
+    if (st != kSuccess) return st;
     static std::atomic<std::uint64_t> done{0};
-    const int st = ensure_dynamic_smem(decode_kernel<HD>, Smem::kBytes, done);
+    st = ensure_dynamic_smem(decode_kernel<HD>, Smem::kBytes, done);
     if (st != kSuccess) return st;
     return launch_pdl_smem(decode_kernel<HD>, dim3(static_cast<unsigned>(n)), dim3(kThreads),
-                           Smem::kBytes, stream, p);
+                           Smem::kBytes, stream, map_k, map_v, p);
 }
 
 }  // namespace attn8
@@ -635,8 +827,6 @@ extern "C" int mote_cuda_gqa_attention_decode_q8(
         return kInvalidValue;
     attn8::Params p{};
     p.q = static_cast<const __half*>(q);
-    p.k_cache = static_cast<const std::int8_t*>(k_cache);
-    p.v_cache = static_cast<const std::int8_t*>(v_cache);
     p.k_scales = static_cast<const float*>(k_scales);
     p.v_scales = static_cast<const float*>(v_scales);
     p.tables = static_cast<const std::int32_t*>(block_tables);
@@ -646,9 +836,14 @@ extern "C" int mote_cuda_gqa_attention_decode_q8(
     p.q_heads = static_cast<std::uint32_t>(q_heads);
     p.group = static_cast<std::uint32_t>(q_heads / kv_heads);
     p.head_groups = (p.group + attn8::kHeads - 1) / attn8::kHeads;
+    // units of every row at the tables' full length, with the rows' ends
+    const std::uint64_t rows = batch * kv_heads * p.head_groups;
+    const std::uint64_t units = max_blocks * block_tokens * head_dim / attn8::kTile + 1 + attn8::kRowCost;
+    if (rows > 0x7fffffffull / units) return kInvalidValue;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.counters = static_cast<unsigned*>(workspace);
     p.parts = static_cast<float*>(workspace) + attn8::kMaxCtas;
     const auto s = static_cast<cudaStream_t>(stream);
-    return head_dim == 64 ? attn8::launch<64>(p, n, s) : attn8::launch<128>(p, n, s);
+    return head_dim == 64 ? attn8::launch<64>(p, k_cache, v_cache, n, s)
+                          : attn8::launch<128>(p, k_cache, v_cache, n, s);
 }
