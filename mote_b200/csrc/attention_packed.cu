@@ -7,65 +7,621 @@
 // A query before the first position (n_k < n_q) gets zeros; rows of out that
 // belong to no sequence keep their values.
 //
-// One warp per (query, head), lanes across head_dim.
+// On the tcgen05 tensor cores, head_dim 64 and 128.  A query tile is 128 rows:
+// floor(128 / g) tokens of one sequence times the g query heads of one KV
+// head (one TMA box of q), so K and V are read once for the group and short
+// prompts fill the tile.  A work item is two consecutive query tiles, which
+// share every K/V tile of 128 positions; persistent CTAs, one per SM, walk
+// the items:
+// * warp 8 loads Q and the K and V tiles (TMA, 128-byte swizzle);
+// * warp 9 owns tensor memory; one thread issues S_i = Q_i K^T and
+//   O_i += P_i V (P_i read from tensor memory, over the first half of S_i).
+//   While the softmax of one query tile runs, the products of the other do;
+// * warps 0-3 and 4-7 run the softmax of query tiles 0 and 1, one thread per
+//   row: the maximum moves (and O_i is rescaled) only when a score passes it
+//   by more than 8 in log2 units;
+// * warps 10 and 11 look through the V tiles that some row sees in part (the
+//   last of each item) before they are used: 0 times an infinity or NaN of a
+//   masked position would be NaN, so such values are taken out, and the
+//   rows that do attend them add them at the end (rare, from global memory).
+// The offsets are read on the device; query tiles of sequence b are numbered
+// from floor(q_starts[b] / tokens of an item) + b on, so an item finds its
+// sequence by one search and no prefix sum is needed.
+// Every wait is bounded; an expired wait aborts the CTA, which waits for its
+// issued MMAs (bounded) and frees its tensor memory.  No load uses cluster
+// multicast.
 #include "mote_common.cuh"
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
 namespace mote {
 namespace attnv {
 
+using attnp::ex2f;
+using attnp::max3f;
+using attnp::tma_load_3d;
+using attnp::tmem_ld32_nowait;
+using attnp::tmem_st32;
+using attnp::tmem_wait_ld;
+using attnp::tmem_wait_st;
+using attnp::umma_f16_ss;
+using gemm::wait_or_abort;
+
+constexpr int kBM = 128;  // rows of a query tile (TMEM lanes)
+constexpr int kBN = 128;  // positions of a K/V tile
+constexpr int kProducerWarp = 8;
+constexpr int kMmaWarp = 9;
+constexpr int kCleanWarps = 2;  // 10 and 11
+constexpr int kThreads = 12 * 32;
+// Register split (setmaxnreg, per warpgroup): launched at 168 a thread;
+// 384 x 168 = 256 x 216 + 128 x 72, and 32 x (216 + 216 + 72) <= 16384.
+constexpr int kLaunchRegs = 168;
+constexpr int kSoftmaxRegs = 216;
+constexpr int kOtherRegs = 72;
+static_assert(kThreads * kLaunchRegs == 256 * kSoftmaxRegs + 128 * kOtherRegs, "register split");
+static_assert(32 * (2 * kSoftmaxRegs + kOtherRegs) <= 16384, "registers of a sub-partition");
+constexpr int kFlags = 8;  // items whose "V holds something not finite" flags are kept; a
+                           // flag is used again when the item 6 before is long written
+
+// TMEM columns: S_i at 128 i, O_i at 256 + 128 i; P_i over the first 64 of S_i.
+constexpr std::uint32_t kColO = 256;
+constexpr std::uint32_t kTmemCols = 512;
+
+template <int HD>
+struct Smem {
+    static constexpr int kHalf = 128 * 128;           // 128 rows of 64 f16
+    static constexpr int kTile = HD / 64 * kHalf;     // a Q, K or V tile
+    static constexpr int kKV = HD == 64 ? 4 : 2;      // K and V stages
+    static constexpr int kQ = 0;                      // [2] query tiles
+    static constexpr int kK = kQ + 2 * kTile;
+    static constexpr int kV = kK + kKV * kTile;
+    static constexpr int kBar = kV + kKV * kTile;
+    // q_full, q_empty, k_full, k_empty, v_full, v_empty, v_clean [kKV], s_full[2],
+    // p_ready[2], o_done[2], epi_done[2], drained
+    static constexpr int kNumBars = 2 + 5 * kKV + 8 + 1;
+    static constexpr int kTmemSlot = kBar + kNumBars * 8;
+    static constexpr int kAbort = kTmemSlot + 4;
+    static constexpr int kFlag = kAbort + 4;          // [kFlags][kCleanWarps]
+    static constexpr int kUsed = kFlag + 4 * kFlags * kCleanWarps + 1008;  // + alignment slack
+    // one CTA per SM: its 512 TMEM columns never wait for another's
+    static constexpr int kBytes = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
+    static_assert(kBytes <= 232448, "shared memory");
+};
+
 struct Params {
-    const __half* q;
-    const __half* k;
-    const __half* v;
     const std::int32_t* q_starts;
     const std::int32_t* kv_starts;
+    const __half* v;
     __half* out;
     std::uint32_t tokens, kv_tokens, batch, q_heads, kv_heads, group;
+    std::uint32_t tile_tokens;  // floor(128 / group)
+    std::uint32_t slots;        // of query tile pairs: tokens / (2 tile_tokens) + batch
     float scale_log2;
 };
 
+// Two query tiles of one sequence and KV head.
+struct Item {
+    std::uint32_t kvh;
+    std::uint32_t q0;      // packed row of the first token
+    std::uint32_t left;    // the sequence's tokens from there on (0: no item)
+    std::int32_t pos0;     // the first token's position
+    std::uint32_t k0, nk;  // first row and number of the positions
+    std::uint32_t n[2];    // K/V tiles that each query tile attends
+    std::uint32_t masked;  // the first tile that some row sees in part
+    __device__ __forceinline__ std::uint32_t tiles() const { return max(n[0], n[1]); }
+};
+
+__device__ __forceinline__ bool sequence_ok(const Params& p, std::int32_t q0, std::int32_t q1,
+                                            std::int32_t k0, std::int32_t k1) {
+    return q0 >= 0 && q1 >= q0 && static_cast<std::uint32_t>(q1) <= p.tokens && k0 >= 0 &&
+           k1 >= k0 && static_cast<std::uint32_t>(k1) <= p.kv_tokens;
+}
+
+// Item i, later tiles first (they attend more); by a whole warp.
+__device__ __forceinline__ Item item_at(const Params& p, std::uint32_t i) {
+    Item it;
+    it.left = 0;
+    it.kvh = i % p.kv_heads;
+    const std::uint32_t slot = p.slots - 1 - i / p.kv_heads;
+    const std::uint32_t span = 2 * p.tile_tokens;
+    const auto first = [&](std::uint32_t b) {
+        return static_cast<std::uint32_t>(max(__ldg(p.q_starts + b), 0)) / span + b;
+    };
+    const std::uint32_t b = kvq8::warp_search(p.batch, slot, first);
+    const std::int32_t q0 = __ldg(p.q_starts + b), q1 = __ldg(p.q_starts + b + 1);
+    const std::int32_t k0 = __ldg(p.kv_starts + b), k1 = __ldg(p.kv_starts + b + 1);
+    const std::uint32_t f = first(b);
+    if (!sequence_ok(p, q0, q1, k0, k1) || slot < f) return it;
+    const std::uint64_t t0 = static_cast<std::uint64_t>(slot - f) * span;
+    const std::uint32_t nq = static_cast<std::uint32_t>(q1 - q0);
+    if (t0 >= nq) return it;
+    it.left = nq - static_cast<std::uint32_t>(t0);
+    it.q0 = static_cast<std::uint32_t>(q0) + static_cast<std::uint32_t>(t0);
+    it.k0 = static_cast<std::uint32_t>(k0);
+    it.nk = static_cast<std::uint32_t>(k1 - k0);
+    it.pos0 = static_cast<std::int32_t>(it.nk) - static_cast<std::int32_t>(it.left);
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        const std::uint32_t from = m * p.tile_tokens;
+        const std::int32_t last = it.pos0 + static_cast<std::int32_t>(min(from + p.tile_tokens, it.left)) - 1;
+        it.n[m] = from >= it.left || last < 0 ? 0u : static_cast<std::uint32_t>(last) / kBN + 1;
+    }
+    it.masked = static_cast<std::uint32_t>(max(it.pos0 + 1, 0)) / kBN;
+    return it;
+}
+
+__device__ __forceinline__ void arrive(std::uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// B operand of P V: V rows (positions) of 64 dimensions; the second 64
+// dimensions lie a half tile further (the leading-dimension offset).
 template <int HD>
-__global__ void __launch_bounds__(128) packed_kernel(const Params p) {
-    constexpr int E = HD / 32;
+__device__ __forceinline__ std::uint64_t v_desc(std::uint32_t addr) {
+    const std::uint64_t d = gemm::smem_desc_sw128(addr);
+    return HD == 64 ? d : (d & ~(0x3fffull << 16)) | static_cast<std::uint64_t>(Smem<HD>::kHalf >> 4) << 16;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1)
+    packed_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const Params p) {
+    using L = Smem<HD>;
+    constexpr int kKV = L::kKV;
+    // kind::f16, f32 accumulators: S: M = 128, N = 128, K-major operands; PV: N = HD, B MN-major
+    constexpr std::uint32_t kIdescS = (1u << 4) | ((kBN >> 3) << 17) | ((kBM >> 4) << 24);
+    constexpr std::uint32_t kIdescPV = (1u << 4) | (1u << 16) | ((HD >> 3) << 17) | ((kBM >> 4) << 24);
+    extern __shared__ std::uint8_t smem_raw[];
+    const std::uint32_t raw_base = smem_u32(smem_raw);
+    const std::uint32_t base = (raw_base + 1023u) & ~1023u;
+    std::uint8_t* smem = smem_raw + (base - raw_base);
+    std::uint64_t* bars = reinterpret_cast<std::uint64_t*>(smem + L::kBar);
+    std::uint64_t* q_full = bars;
+    std::uint64_t* q_empty = bars + 1;
+    std::uint64_t* k_full = bars + 2;
+    std::uint64_t* k_empty = k_full + kKV;
+    std::uint64_t* v_full = k_empty + kKV;
+    std::uint64_t* v_empty = v_full + kKV;
+    std::uint64_t* v_clean = v_empty + kKV;
+    std::uint64_t* s_full = v_clean + kKV;
+    std::uint64_t* p_ready = s_full + 2;
+    std::uint64_t* o_done = p_ready + 2;
+    std::uint64_t* epi_done = o_done + 2;
+    std::uint64_t* drained = epi_done + 2;
+    volatile std::uint32_t* tmem_slot = reinterpret_cast<volatile std::uint32_t*>(smem + L::kTmemSlot);
+    volatile std::uint32_t* abort_flag = reinterpret_cast<volatile std::uint32_t*>(smem + L::kAbort);
+    volatile std::uint32_t* not_finite = reinterpret_cast<volatile std::uint32_t*>(smem + L::kFlag);
+
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        for (int s = 0; s < kKV; ++s) {
+            mbar_init(&k_full[s], 1);
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_full[s], 1);
+            mbar_init(&v_empty[s], 1 + kCleanWarps);  // the last P V, and warps 10 and 11 keep step
+            mbar_init(&v_clean[s], kCleanWarps);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&s_full[s], 1);
+            mbar_init(&p_ready[s], 4);
+            mbar_init(&o_done[s], 1);
+            mbar_init(&epi_done[s], 4);
+        }
+        mbar_init(drained, 1);
+        *abort_flag = 0u;
+        fence_mbarrier_init();
+    }
+    if (p.tile_tokens * p.group < kBM) {  // rows of a query tile that no box fills stay zero
+        for (int i = threadIdx.x; i < 2 * L::kTile / 16; i += kThreads)
+            reinterpret_cast<uint4*>(smem + L::kQ)[i] = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();
+    }
+    if (warp == kMmaWarp) gemm::tmem_alloc(base + L::kTmemSlot, kTmemCols);
+    gemm::tc_fence_before();
+    __syncthreads();
+    gemm::tc_fence_after();
+    const std::uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();
     pdl_wait();
-    const int lane = threadIdx.x % 32;
-    if (blockIdx.x == 0 && blockIdx.y == 0)
-        for (std::uint32_t b = threadIdx.x; b < p.batch; b += blockDim.x) {
-            const std::int32_t q0 = p.q_starts[b], q1 = p.q_starts[b + 1];
-            const std::int32_t k0 = p.kv_starts[b], k1 = p.kv_starts[b + 1];
-            if (q0 < 0 || q1 < q0 || static_cast<std::uint32_t>(q1) > p.tokens || k0 < 0 || k1 < k0 ||
-                static_cast<std::uint32_t>(k1) > p.kv_tokens)
-                atomicOr(&g_device_status, kDevIndexOutOfRange);
+
+    const std::uint32_t items = p.slots * p.kv_heads;
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+        if (warp == kProducerWarp) {
+            if (blockIdx.x == 0)  // offsets that the items skip are reported
+                for (std::uint32_t b = lane; b < p.batch; b += 32)
+                    if (!sequence_ok(p, p.q_starts[b], p.q_starts[b + 1], p.kv_starts[b], p.kv_starts[b + 1]))
+                        atomicOr(&g_device_status, kDevIndexOutOfRange);
+            std::uint32_t c = 0, n = 0;  // K/V tiles and items loaded
+            bool ok = true;
+            for (std::uint32_t i = blockIdx.x; ok && i < items; i += gridDim.x) {
+                const Item it = item_at(p, i);
+                const std::uint32_t tiles = it.left ? it.tiles() : 0;
+                if (tiles == 0) continue;
+                if (lane == 0) {
+                    ok = n == 0 || wait_or_abort(q_empty, (n - 1) & 1u, abort_flag);
+                    if (ok) {
+                        const std::uint32_t box = p.tile_tokens * p.group * 128;
+                        mbar_arrive_expect_tx(q_full, ((it.n[0] > 0) + (it.n[1] > 0)) * (HD / 64) * box);
+                        for (int m = 0; m < 2; ++m)
+                            for (int h = 0; h < HD / 64 && it.n[m] > 0; ++h)
+                                tma_load_3d(base + L::kQ + m * L::kTile + h * L::kHalf, &map_q, 64 * h,
+                                            static_cast<int>(it.kvh * p.group),
+                                            static_cast<int>(it.q0 + m * p.tile_tokens), smem_u32(q_full));
+                    }
+                    for (std::uint32_t j = 0; ok && j < tiles; ++j) {
+                        const std::uint32_t t = c + j, s = t % kKV, ph = (t / kKV - 1) & 1u;
+                        const int row = static_cast<int>(it.k0 + j * kBN);
+                        if (t >= kKV && !wait_or_abort(&k_empty[s], ph, abort_flag)) ok = false;
+                        if (!ok) break;
+                        mbar_arrive_expect_tx(&k_full[s], L::kTile);
+                        for (int h = 0; h < HD / 64; ++h)
+                            tma_load_3d(base + L::kK + s * L::kTile + h * L::kHalf, &map_k, 64 * h,
+                                        static_cast<int>(it.kvh), row, smem_u32(&k_full[s]));
+                        if (t >= kKV && !wait_or_abort(&v_empty[s], ph, abort_flag)) ok = false;
+                        if (!ok) break;
+                        mbar_arrive_expect_tx(&v_full[s], L::kTile);
+                        for (int h = 0; h < HD / 64; ++h)
+                            tma_load_3d(base + L::kV + s * L::kTile + h * L::kHalf, &map_v, 64 * h,
+                                        static_cast<int>(it.kvh), row, smem_u32(&v_full[s]));
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                c += tiles;
+                ++n;
+            }
+        } else if (warp == kMmaWarp) {
+            std::uint32_t c = 0, n = 0, clean = 0;
+            // per query tile: P V issued, items with any, and whether the last
+            // one's epilogue has yet to be waited for
+            std::uint32_t done[2] = {0, 0}, outs[2] = {0, 0};
+            bool unread[2] = {false, false};
+            bool ok = true;
+            for (std::uint32_t i = blockIdx.x; ok && i < items; i += gridDim.x) {
+                const Item it = item_at(p, i);
+                const std::uint32_t tiles = it.left ? it.tiles() : 0;
+                if (tiles == 0) continue;
+                if (lane == 0) {
+                    const auto issue_s = [&](int m, std::uint32_t j) {
+                        const std::uint32_t kaddr = base + L::kK + ((c + j) % kKV) * L::kTile;
+                        const std::uint32_t qaddr = base + L::kQ + m * L::kTile;
+#pragma unroll
+                        for (int k = 0; k < HD / 16; ++k) {
+                            const std::uint32_t at = k / 4 * L::kHalf + k % 4 * 32;
+                            umma_f16_ss(tmem + 128u * m, gemm::smem_desc_sw128(qaddr + at),
+                                        gemm::smem_desc_sw128(kaddr + at), kIdescS, k != 0 ? 1u : 0u);
+                        }
+                        gemm::umma_commit(smem_u32(&s_full[m]));
+                    };
+                    const auto wait_k = [&](std::uint32_t j) {
+                        const std::uint32_t t = c + j;
+                        return wait_or_abort(&k_full[t % kKV], (t / kKV) & 1u, abort_flag);
+                    };
+                    // after the last S on K tile j / of the item
+                    const auto s_done = [&](int m, std::uint32_t j) {
+                        if (m == 1 || j >= it.n[1]) {
+                            gemm::umma_commit(smem_u32(&k_empty[(c + j) % kKV]));
+                            if (j + 1 == tiles) gemm::umma_commit(smem_u32(q_empty));
+                        }
+                    };
+                    ok = wait_or_abort(q_full, n & 1u, abort_flag) && wait_k(0);
+                    if (ok) {
+                        gemm::tc_fence_after();
+                        for (int m = 0; m < 2; ++m)
+                            if (it.n[m] > 0) issue_s(m, 0), s_done(m, 0);
+                    }
+                    for (std::uint32_t j = 0; ok && j < tiles; ++j) {
+                        const std::uint32_t t = c + j, s = t % kKV;
+                        // V tile j has landed, and is looked through where rows see it in part
+                        // (its barriers go round with the tiles that are)
+                        ok = wait_or_abort(&v_full[s], (t / kKV) & 1u, abort_flag);
+                        if (ok && j >= it.masked) {
+                            ok = wait_or_abort(&v_clean[clean % kKV], (clean / kKV) & 1u, abort_flag);
+                            ++clean;
+                        }
+                        for (int m = 0; ok && m < 2; ++m) {
+                            // the last O is read (of both query tiles, so that neither
+                            // softmax group falls behind by more than an item)
+                            if (unread[m] && j == 0) {
+                                ok = wait_or_abort(&epi_done[m], (outs[m] - 1) & 1u, abort_flag);
+                                unread[m] = false;
+                            }
+                            if (j >= it.n[m]) continue;
+                            ok = ok && wait_or_abort(&p_ready[m], done[m] & 1u, abort_flag);
+                            if (!ok) break;
+                            gemm::tc_fence_after();
+                            const std::uint32_t vaddr = base + L::kV + s * L::kTile;
+#pragma unroll
+                            for (int k = 0; k < kBN / 16; ++k)
+                                gemm::umma_f16_ta(tmem + kColO + 128u * m, tmem + 128u * m + k * 8,
+                                                  v_desc<HD>(vaddr + k * 2048), kIdescPV, (j | k) != 0 ? 1u : 0u);
+                            gemm::umma_commit(smem_u32(&o_done[m]));
+                            ++done[m];
+                            if (j == 0) ++outs[m], unread[m] = true;
+                            if (m == 1 || j >= it.n[1]) gemm::umma_commit(smem_u32(&v_empty[s]));
+                            if (j + 1 < it.n[m]) {
+                                ok = wait_k(j + 1);
+                                if (!ok) break;
+                                gemm::tc_fence_after();
+                                issue_s(m, j + 1), s_done(m, j + 1);
+                            }
+                        }
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                c += tiles;
+                ++n;
+            }
+            // every issued MMA completes before the tensor memory is freed
+            if (lane == 0) {
+                gemm::umma_commit(smem_u32(drained));
+                mbar_wait_bounded(drained, 0, &g_device_status);
+            }
+            __syncwarp();
+        } else {
+            std::uint32_t c = 0, n = 0, clean = 0;
+            bool ok = true;
+            const int me = threadIdx.x - 10 * 32;  // of 64
+            for (std::uint32_t i = blockIdx.x; ok && i < items; i += gridDim.x) {
+                const Item it = item_at(p, i);
+                const std::uint32_t tiles = it.left ? it.tiles() : 0;
+                if (tiles == 0) continue;
+                volatile std::uint32_t* flag = not_finite + n % kFlags * kCleanWarps + (warp - 10);
+                if (lane == 0) *flag = 0u;
+                for (std::uint32_t j = 0; ok && j < tiles; ++j) {
+                    const std::uint32_t t = c + j, s = t % kKV;
+                    ok = __all_sync(0xffffffffu, wait_or_abort(&v_full[s], (t / kKV) & 1u, abort_flag));
+                    if (!ok) break;
+                    if (j >= it.masked) {
+                        uint4* tile = reinterpret_cast<uint4*>(smem + L::kV + s * L::kTile);
+                        std::uint32_t bad = 0;  // an exponent of all ones carries into bit 15
+#pragma unroll 4
+                        for (int x = me; x < L::kTile / 16; x += 32 * kCleanWarps) {
+                            const uint4 v = tile[x];
+                            bad |= ((v.x & 0x7c007c00u) + 0x04000400u) | ((v.y & 0x7c007c00u) + 0x04000400u) |
+                                   ((v.z & 0x7c007c00u) + 0x04000400u) | ((v.w & 0x7c007c00u) + 0x04000400u);
+                        }
+                        if (__any_sync(0xffffffffu, (bad & 0x80008000u) != 0)) {
+                            // 16-byte chunk x belongs to row x / 8 of its half tile
+                            const std::uint32_t rows = it.nk - j * kBN;  // of the sequence
+                            bool found = false;
+                            for (int x = me; x < L::kTile / 16; x += 32 * kCleanWarps) {
+                                const uint4 v = tile[x];
+                                std::uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                                bool any = false;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    if ((w[e] & 0x7c00u) == 0x7c00u) w[e] &= 0xffff0000u, any = true;
+                                    if ((w[e] & 0x7c000000u) == 0x7c000000u) w[e] &= 0x0000ffffu, any = true;
+                                }
+                                if (any) tile[x] = make_uint4(w[0], w[1], w[2], w[3]);
+                                found |= any && static_cast<std::uint32_t>(x / 8 % kBN) < rows;
+                            }
+                            fence_proxy_async_smem();
+                            if (found) *flag = 1u;
+                        }
+                        __syncwarp();
+                        if (lane == 0) arrive(&v_clean[clean % kKV]);
+                        ++clean;
+                    }
+                    if (lane == 0) arrive(&v_empty[s]);
+                }
+                c += tiles;
+                ++n;
+            }
         }
-    const std::uint32_t h = blockIdx.y * 4 + threadIdx.x / 32, row = blockIdx.x;
-    if (h >= p.q_heads) return;
-    const std::uint32_t b = kvq8::warp_search(p.batch, row, [&](std::uint32_t i) {
-        return static_cast<std::uint32_t>(max(p.q_starts[i], 0));
-    });
-    const std::int32_t q0 = p.q_starts[b], q1 = p.q_starts[b + 1];
-    const std::int32_t k0 = p.kv_starts[b], k1 = p.kv_starts[b + 1];
-    if (q0 < 0 || static_cast<std::int64_t>(row) < q0 || static_cast<std::int64_t>(row) >= q1 ||
-        static_cast<std::uint32_t>(q1) > p.tokens || k0 < 0 || k1 < k0 ||
-        static_cast<std::uint32_t>(k1) > p.kv_tokens)
-        return;
-    const std::int64_t last = static_cast<std::int64_t>(k1) - k0 - (q1 - static_cast<std::int64_t>(row));
-    const std::uint64_t qa = (static_cast<std::uint64_t>(row) * p.q_heads + h) * HD + lane * E;
-    float qv[E], o[E], m = -INFINITY, l = 0.f;
-    for (int e = 0; e < E; ++e) qv[e] = __half2float(p.q[qa + e]), o[e] = 0.f;
-    for (std::int64_t pos = 0; pos <= last; ++pos) {
-        const std::uint64_t at =
-            (static_cast<std::uint64_t>(k0 + pos) * p.kv_heads + h / p.group) * HD + lane * E;
-        float s = 0.f;
-        for (int e = 0; e < E; ++e) s += qv[e] * __half2float(p.k[at + e]);
-        for (int d = 16; d > 0; d /= 2) s += __shfl_xor_sync(0xffffffffu, s, d);
-        s *= p.scale_log2;
-        const float mn = fmaxf(m, s), f = mn == m ? 1.f : exp2f(m - mn), w = exp2f(s - mn);
-        m = mn;
-        l = l * f + w;
-        for (int e = 0; e < E; ++e) o[e] = o[e] * f + w * __half2float(p.v[at + e]);
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        // softmax: warps 4 m .. 4 m + 3 take query tile m, one thread per row
+        const int m = warp / 4;
+        const int r = 32 * (warp % 4) + lane;
+        const std::uint32_t row_tmem = tmem + (static_cast<std::uint32_t>(32 * (warp % 4)) << 16);
+        const std::uint32_t s_col = row_tmem + 128u * m, o_col = row_tmem + kColO + 128u * m;
+        const std::uint32_t tok = r / p.group, head = r % p.group;
+        const float sc = p.scale_log2;
+        std::uint32_t cnt = 0, n = 0;  // tiles of this query tile, items
+        bool ok = true;
+        for (std::uint32_t i = blockIdx.x; i < items; i += gridDim.x) {
+            const Item it = item_at(p, i);
+            if (it.left == 0) continue;
+            const std::uint32_t token = m * p.tile_tokens + tok;  // from the item's first
+            const bool mine = tok < p.tile_tokens && token < it.left;
+            const std::int32_t limit = it.pos0 + static_cast<std::int32_t>(token);  // its position
+            const std::int32_t first = it.pos0 + static_cast<std::int32_t>(m * p.tile_tokens);
+            const std::uint32_t tiles = it.n[m];
+            float mx_ref = -INFINITY, l = 0.f;
+            for (std::uint32_t j = 0; j < tiles && ok; ++j, ++cnt) {
+                ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[m], cnt & 1u, abort_flag));
+                if (!ok) break;
+                gemm::tc_fence_after();
+                std::uint32_t v[4][32];
+#pragma unroll
+                for (int cc = 0; cc < 4; ++cc) tmem_ld32_nowait(s_col + 32 * cc, v[cc]);
+                tmem_wait_ld();
+                // causal mask; the scale is positive, so the maximum of the raw
+                // scores gives that of the scaled ones
+                const std::int32_t kbase = static_cast<std::int32_t>(j * kBN);
+                if (kbase + kBN - 1 > first) {
+#pragma unroll
+                    for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (kbase + 32 * cc + e > limit) v[cc][e] = __float_as_uint(-INFINITY);
+                }
+                float mx8[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx8[e] = -INFINITY;
+#pragma unroll
+                for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2)
+                        mx8[(e / 2) % 8] = max3f(mx8[(e / 2) % 8], __uint_as_float(v[cc][e]),
+                                                 __uint_as_float(v[cc][e + 1]));
+                const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
+                                       fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+                // the reference moves only when a score passes it by more than 8
+                // (P stays below 2^8); -infinity while the row has seen nothing
+                const float mnew = fmaxf(mx_ref, mx);
+                const bool grow = (mnew - mx_ref) * sc > 8.f;  // false while both are -inf (NaN)
+                float alpha = 1.f;
+                if (grow) {
+                    alpha = ex2f((mx_ref - mnew) * sc);  // 0 from -infinity
+                    mx_ref = mnew;
+                }
+                const float neg = mx_ref == -INFINITY ? 0.f : -mx_ref * sc;
+                const std::uint64_t sc2 = attnp::pack_f32x2(sc, sc), neg2 = attnp::pack_f32x2(neg, neg);
+                std::uint64_t acc2[4] = {0, 0, 0, 0};
+                std::uint32_t pk[2][32];
+#pragma unroll
+                for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        float xa, xb;
+                        attnp::unpack_f32x2(attnp::fma_f32x2(attnp::pack_f32x2(__uint_as_float(v[cc][e]),
+                                                                               __uint_as_float(v[cc][e + 1])),
+                                                             sc2, neg2),
+                                            xa, xb);
+                        const float a = ex2f(xa), b = ex2f(xb);
+                        acc2[(e / 2) % 4] = attnp::add_f32x2(acc2[(e / 2) % 4], attnp::pack_f32x2(a, b));
+                        std::uint32_t h2;
+                        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h2) : "f"(b), "f"(a));
+                        pk[cc / 2][(cc % 2) * 16 + e / 2] = h2;
+                    }
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x0, x1;
+                    attnp::unpack_f32x2(acc2[e], x0, x1);
+                    sum += x0 + x1;
+                }
+                l = fmaf(l, alpha, sum);
+                tmem_st32(s_col, pk[0]);
+                tmem_st32(s_col + 32, pk[1]);
+                tmem_wait_st();
+                if (j > 0 && __any_sync(0xffffffffu, grow)) {
+                    // the previous P V is complete before O moves
+                    ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[m], (cnt - 1) & 1u, abort_flag));
+                    if (!ok) break;
+                    gemm::tc_fence_after();
+#pragma unroll
+                    for (int cc = 0; cc < HD / 32; ++cc) {
+                        std::uint32_t o[32];
+                        tmem_ld32_nowait(o_col + 32 * cc, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tmem_st32(o_col + 32 * cc, o);
+                    }
+                    tmem_wait_st();
+                }
+                gemm::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(&p_ready[m]);
+            }
+            // O / sum; rows before the first position have no sum and get zeros
+            if (it.tiles() > 0) ++n;
+            if (tiles > 0 && ok)
+                ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[m], (cnt - 1) & 1u, abort_flag));
+            if (ok) {
+                gemm::tc_fence_after();
+                const bool some = tiles > 0 && limit >= 0;
+                const float inv = some ? 1.f / l : 0.f;
+                const volatile std::uint32_t* flags = not_finite + (n - 1) % kFlags * kCleanWarps;
+                const bool add = some && (flags[0] | flags[1]) != 0u;
+                __half* dst = p.out + (static_cast<std::uint64_t>(it.q0 + token) * p.q_heads +
+                                       it.kvh * p.group + head) * HD;
+#pragma unroll 1
+                for (int cc = 0; cc < HD / 32; ++cc) {
+                    std::uint32_t o[32];
+                    if (tiles > 0) {
+                        tmem_ld32_nowait(o_col + 32 * cc, o);
+                        tmem_wait_ld();
+                    }
+                    if (!mine) continue;
+                    if (add) {
+                        // what warps 10 and 11 took out of the V tiles that this row attends
+                        for (std::uint32_t pos = it.masked * kBN; pos <= static_cast<std::uint32_t>(limit); ++pos) {
+                            const __half* src = p.v + (static_cast<std::uint64_t>(it.k0 + pos) * p.kv_heads + it.kvh) * HD + 32 * cc;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const float x = __half2float(src[e]);
+                                if (!isfinite(x)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        std::uint32_t w[4];
+#pragma unroll
+                        for (int e2 = 0; e2 < 4; ++e2) {
+                            const float x0 = some ? __uint_as_float(o[e + 2 * e2]) * inv : 0.f;
+                            const float x1 = some ? __uint_as_float(o[e + 2 * e2 + 1]) * inv : 0.f;
+                            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[e2]) : "f"(x1), "f"(x0));
+                        }
+                        *reinterpret_cast<uint4*>(dst + 32 * cc + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                gemm::tc_fence_before();
+                __syncwarp();
+                if (lane == 0 && tiles > 0) arrive(&epi_done[m]);  // O may be overwritten
+            }
+        }
     }
-    for (int e = 0; e < E; ++e) p.out[qa + e] = __float2half_rn(last >= 0 ? o[e] / l : 0.f);
+    gemm::tc_fence_before();
+    __syncthreads();
+    gemm::tc_fence_after();
+    if (warp == kMmaWarp) gemm::tmem_dealloc(tmem, kTmemCols);
+}
+
+// [rows, heads, HD] f16 in boxes of `tokens` rows x `group` heads x 64; rows
+// past the last read zeros.
+inline int make_map(CUtensorMap* map, const void* ptr, std::uint64_t rows, std::uint64_t heads,
+                    std::uint32_t head_dim, std::uint32_t group, std::uint32_t tokens) {
+    auto encode = gemm::encode_fn();
+    if (encode == nullptr) return static_cast<int>(cudaErrorNotSupported);
+    const cuuint64_t dims[3] = {head_dim, heads, rows < 1 ? 1 : rows};
+    const cuuint64_t strides[2] = {head_dim * 2ull, heads * head_dim * 2ull};
+    const cuuint32_t box[3] = {64, group, tokens};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    if (encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(ptr), dims, strides, box,
+               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return kInvalidValue;
+    return kSuccess;
+}
+
+template <int HD>
+int launch(const Params& p, const void* q, const void* k, cudaStream_t stream) {
+    CUtensorMap map_q{}, map_k{}, map_v{};
+    int st = make_map(&map_q, q, p.tokens, p.q_heads, HD, p.group, p.tile_tokens);
+    if (st == kSuccess) st = make_map(&map_k, k, p.kv_tokens, p.kv_heads, HD, 1, kBN);
+    if (st == kSuccess) st = make_map(&map_v, p.v, p.kv_tokens, p.kv_heads, HD, 1, kBN);
+    if (st != kSuccess) return st;
+    static std::atomic<std::uint64_t> smem_done{0};
+    st = ensure_dynamic_smem(packed_kernel<HD>, Smem<HD>::kBytes, smem_done);
+    if (st != kSuccess) return st;
+    // The register split is exact for a launch at kLaunchRegs a thread; a build
+    // that allocated another count is never launched.
+    static std::atomic<int> regs_checked{0};
+    if (regs_checked.load(std::memory_order_acquire) == 0) {
+        cudaFuncAttributes fa{};
+        const cudaError_t ea = cudaFuncGetAttributes(&fa, packed_kernel<HD>);
+        if (ea != cudaSuccess) return static_cast<int>(ea);
+        if (fa.numRegs != kLaunchRegs) return kInvalidConfiguration;
+        regs_checked.store(1, std::memory_order_release);
+    }
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const std::uint64_t items = static_cast<std::uint64_t>(p.slots) * p.kv_heads;
+    const unsigned grid = static_cast<unsigned>(items < static_cast<std::uint64_t>(sms) ? items : sms);
+    return launch_pdl_smem(packed_kernel<HD>, dim3(grid), dim3(kThreads), Smem<HD>::kBytes, stream,
+                           map_q, map_k, map_v, p);
 }
 
 }  // namespace attnv
@@ -89,11 +645,9 @@ extern "C" int mote_cuda_gqa_attention_packed_f16(const void* q, const void* k, 
         return kInvalidValue;
     if (tokens == 0 || batch == 0 || q_heads == 0) return kSuccess;
     attnv::Params p{};
-    p.q = static_cast<const __half*>(q);
-    p.k = static_cast<const __half*>(k);
-    p.v = static_cast<const __half*>(v);
     p.q_starts = static_cast<const std::int32_t*>(q_starts);
     p.kv_starts = static_cast<const std::int32_t*>(kv_starts);
+    p.v = static_cast<const __half*>(v);
     p.out = static_cast<__half*>(out);
     p.tokens = static_cast<std::uint32_t>(tokens);
     p.kv_tokens = static_cast<std::uint32_t>(kv_tokens);
@@ -101,9 +655,10 @@ extern "C" int mote_cuda_gqa_attention_packed_f16(const void* q, const void* k, 
     p.q_heads = static_cast<std::uint32_t>(q_heads);
     p.kv_heads = static_cast<std::uint32_t>(kv_heads);
     p.group = static_cast<std::uint32_t>(q_heads / kv_heads);
+    p.tile_tokens = attnv::kBM / p.group;
+    p.slots = static_cast<std::uint32_t>(tokens / (2 * p.tile_tokens) + batch);
     p.scale_log2 = scale * 1.4426950408889634f;
-    const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>((q_heads + 3) / 4));
+    if (static_cast<std::uint64_t>(p.slots) * kv_heads > 0x7fffffffull) return kInvalidValue;
     const auto s = static_cast<cudaStream_t>(stream);
-    return head_dim == 64 ? launch_pdl(attnv::packed_kernel<64>, grid, dim3(128), s, p)
-                          : launch_pdl(attnv::packed_kernel<128>, grid, dim3(128), s, p);
+    return head_dim == 64 ? attnv::launch<64>(p, q, k, s) : attnv::launch<128>(p, q, k, s);
 }
