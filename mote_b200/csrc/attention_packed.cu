@@ -151,6 +151,13 @@ __device__ __forceinline__ Item item_at(const Params& p, std::uint32_t i) {
     return it;
 }
 
+// One lane of the (converged) warp, always the same.
+__device__ __forceinline__ bool elect_one() {
+    std::uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ void arrive(std::uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -275,89 +282,103 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ++n;
             }
         } else if (warp == kMmaWarp) {
+            // The whole warp walks the loops, on values that the compiler knows to
+            // be uniform, and one elected lane issues: operands then come from
+            // uniform registers (moving each to one cost 100 cycles an MMA).
+            const std::uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
             std::uint32_t c = 0, n = 0, clean = 0;
             // per query tile: P V issued, items with any, and whether the last
             // one's epilogue has yet to be waited for
             std::uint32_t done[2] = {0, 0}, outs[2] = {0, 0};
             bool unread[2] = {false, false};
+            const auto wait = [&](std::uint64_t* bar, std::uint32_t parity) {
+                return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag)) != 0;
+            };
             bool ok = true;
             for (std::uint32_t i = blockIdx.x; ok && i < items; i += gridDim.x) {
                 const Item it = item_at(p, i);
-                const std::uint32_t tiles = it.left ? it.tiles() : 0;
+                const std::uint32_t n0 = __reduce_max_sync(0xffffffffu, it.left ? it.n[0] : 0u);
+                const std::uint32_t n1 = __reduce_max_sync(0xffffffffu, it.left ? it.n[1] : 0u);
+                const std::uint32_t masked = __reduce_max_sync(0xffffffffu, it.masked);
+                const std::uint32_t tiles = max(n0, n1);
                 if (tiles == 0) continue;
-                if (lane == 0) {
-                    const auto issue_s = [&](int m, std::uint32_t j) {
-                        const std::uint32_t kaddr = base + L::kK + ((c + j) % kKV) * L::kTile;
-                        const std::uint32_t qaddr = base + L::kQ + m * L::kTile;
+                // S_m on K tile j of the item, then what its last use frees
+                const auto issue_s = [&](int m, std::uint32_t j) {
+                    const std::uint32_t s = (c + j) % kKV;
+                    const std::uint64_t ad = gemm::smem_desc_sw128(base + L::kQ + m * L::kTile);
+                    const std::uint64_t bd = gemm::smem_desc_sw128(base + L::kK + s * L::kTile);
+                    const bool last = m == 1 || j >= n1;
+                    if (elect_one()) {
 #pragma unroll
                         for (int k = 0; k < HD / 16; ++k) {
-                            const std::uint32_t at = k / 4 * L::kHalf + k % 4 * 32;
-                            umma_f16_ss(tmem + 128u * m, gemm::smem_desc_sw128(qaddr + at),
-                                        gemm::smem_desc_sw128(kaddr + at), kIdescS, k != 0 ? 1u : 0u);
+                            constexpr std::uint32_t kStep = 32 >> 4, kNext = L::kHalf >> 4;
+                            const std::uint32_t at = k / 4 * kNext + k % 4 * kStep;
+                            umma_f16_ss(tm + 128u * m, ad + at, bd + at, kIdescS, k != 0 ? 1u : 0u);
                         }
                         gemm::umma_commit(smem_u32(&s_full[m]));
-                    };
-                    const auto wait_k = [&](std::uint32_t j) {
-                        const std::uint32_t t = c + j;
-                        return wait_or_abort(&k_full[t % kKV], (t / kKV) & 1u, abort_flag);
-                    };
-                    // after the last S on K tile j / of the item
-                    const auto s_done = [&](int m, std::uint32_t j) {
-                        if (m == 1 || j >= it.n[1]) {
-                            gemm::umma_commit(smem_u32(&k_empty[(c + j) % kKV]));
-                            if (j + 1 == tiles) gemm::umma_commit(smem_u32(q_empty));
-                        }
-                    };
-                    ok = wait_or_abort(q_full, n & 1u, abort_flag) && wait_k(0);
-                    if (ok) {
-                        gemm::tc_fence_after();
-                        for (int m = 0; m < 2; ++m)
-                            if (it.n[m] > 0) issue_s(m, 0), s_done(m, 0);
+                        if (last) gemm::umma_commit(smem_u32(&k_empty[s]));
+                        if (last && j + 1 == tiles) gemm::umma_commit(smem_u32(q_empty));
                     }
-                    for (std::uint32_t j = 0; ok && j < tiles; ++j) {
-                        const std::uint32_t t = c + j, s = t % kKV;
-                        // V tile j has landed, and is looked through where rows see it in part
-                        // (its barriers go round with the tiles that are)
-                        ok = wait_or_abort(&v_full[s], (t / kKV) & 1u, abort_flag);
-                        if (ok && j >= it.masked) {
-                            ok = wait_or_abort(&v_clean[clean % kKV], (clean / kKV) & 1u, abort_flag);
-                            ++clean;
+                    __syncwarp();
+                };
+                const auto wait_k = [&](std::uint32_t j) {
+                    const std::uint32_t t = c + j;
+                    return wait(&k_full[t % kKV], (t / kKV) & 1u);
+                };
+                ok = wait(q_full, n & 1u) && wait_k(0);
+                if (ok) {
+                    gemm::tc_fence_after();
+                    if (n0 > 0) issue_s(0, 0);
+                    if (n1 > 0) issue_s(1, 0);
+                }
+                for (std::uint32_t j = 0; ok && j < tiles; ++j) {
+                    const std::uint32_t t = c + j, s = t % kKV;
+                    // V tile j has landed, and is looked through where rows see it in part
+                    // (its barriers go round with the tiles that are)
+                    ok = wait(&v_full[s], (t / kKV) & 1u);
+                    if (ok && j >= masked) {
+                        ok = wait(&v_clean[clean % kKV], (clean / kKV) & 1u);
+                        ++clean;
+                    }
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        // the last O is read (of both query tiles, so that neither
+                        // softmax group falls behind by more than an item)
+                        if (ok && unread[m] && j == 0) {
+                            ok = wait(&epi_done[m], (outs[m] - 1) & 1u);
+                            unread[m] = false;
                         }
-                        for (int m = 0; ok && m < 2; ++m) {
-                            // the last O is read (of both query tiles, so that neither
-                            // softmax group falls behind by more than an item)
-                            if (unread[m] && j == 0) {
-                                ok = wait_or_abort(&epi_done[m], (outs[m] - 1) & 1u, abort_flag);
-                                unread[m] = false;
-                            }
-                            if (j >= it.n[m]) continue;
-                            ok = ok && wait_or_abort(&p_ready[m], done[m] & 1u, abort_flag);
-                            if (!ok) break;
-                            gemm::tc_fence_after();
-                            const std::uint32_t vaddr = base + L::kV + s * L::kTile;
+                        if (!ok || j >= (m ? n1 : n0)) continue;
+                        ok = wait(&p_ready[m], done[m] & 1u);
+                        if (!ok) continue;
+                        gemm::tc_fence_after();
+                        const std::uint64_t vd = v_desc<HD>(base + L::kV + s * L::kTile);
+                        const bool last = m == 1 || j >= n1;
+                        if (elect_one()) {
 #pragma unroll
                             for (int k = 0; k < kBN / 16; ++k)
-                                gemm::umma_f16_ta(tmem + kColO + 128u * m, tmem + 128u * m + k * 8,
-                                                  v_desc<HD>(vaddr + k * 2048), kIdescPV, (j | k) != 0 ? 1u : 0u);
+                                gemm::umma_f16_ta(tm + kColO + 128u * m, tm + 128u * m + k * 8,
+                                                  vd + k * (2048 >> 4), kIdescPV, (j | k) != 0 ? 1u : 0u);
                             gemm::umma_commit(smem_u32(&o_done[m]));
-                            ++done[m];
-                            if (j == 0) ++outs[m], unread[m] = true;
-                            if (m == 1 || j >= it.n[1]) gemm::umma_commit(smem_u32(&v_empty[s]));
-                            if (j + 1 < it.n[m]) {
-                                ok = wait_k(j + 1);
-                                if (!ok) break;
-                                gemm::tc_fence_after();
-                                issue_s(m, j + 1), s_done(m, j + 1);
-                            }
+                            if (last) gemm::umma_commit(smem_u32(&v_empty[s]));
+                        }
+                        __syncwarp();
+                        ++done[m];
+                        if (j == 0) ++outs[m], unread[m] = true;
+                        if (j + 1 < (m ? n1 : n0)) {
+                            ok = wait_k(j + 1);
+                            if (!ok) continue;
+                            gemm::tc_fence_after();
+                            issue_s(m, j + 1);
                         }
                     }
                 }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
                 c += tiles;
                 ++n;
             }
-            // every issued MMA completes before the tensor memory is freed
-            if (lane == 0) {
+            // every issued MMA completes before the tensor memory is freed (commit
+            // by the lane that issued)
+            if (elect_one()) {
                 gemm::umma_commit(smem_u32(drained));
                 mbar_wait_bounded(drained, 0, &g_device_status);
             }
