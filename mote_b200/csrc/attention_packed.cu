@@ -13,7 +13,10 @@
 // prompts fill the tile.  A work item is two consecutive query tiles, which
 // share every K/V tile of 128 positions; persistent CTAs, one per SM, walk
 // the items:
-// * warp 8 loads Q and the K and V tiles (TMA, 128-byte swizzle);
+// * warp 8 finds the items, from the largest down (the offsets are read on the
+//   device; of up to 256 sequences the pairs of query tiles are ranked by
+//   counting, without a sort), hands them on and loads Q and the K and V
+//   tiles (TMA, 128-byte swizzle);
 // * warp 9 owns tensor memory; one thread issues S_i = Q_i K^T and
 //   O_i += P_i V (P_i read from tensor memory, over the first half of S_i).
 //   While the softmax of one query tile runs, the products of the other do;
@@ -24,9 +27,6 @@
 //   last of each item) before they are used: 0 times an infinity or NaN of a
 //   masked position would be NaN, so such values are taken out, and the
 //   rows that do attend them add them at the end (rare, from global memory).
-// The offsets are read on the device; query tiles of sequence b are numbered
-// from floor(q_starts[b] / tokens of an item) + b on, so an item finds its
-// sequence by one search and no prefix sum is needed.
 // Every wait is bounded; an expired wait aborts the CTA, which waits for its
 // issued MMAs (bounded) and frees its tensor memory.  No load uses cluster
 // multicast.
@@ -61,12 +61,36 @@ constexpr int kSoftmaxRegs = 216;
 constexpr int kOtherRegs = 72;
 static_assert(kThreads * kLaunchRegs == 256 * kSoftmaxRegs + 128 * kOtherRegs, "register split");
 static_assert(32 * (2 * kSoftmaxRegs + kOtherRegs) <= 16384, "registers of a sub-partition");
+constexpr int kItems = 4;          // items that the producer may be ahead
+constexpr std::uint32_t kSorted = 256;  // sequences up to which items are sorted
 constexpr int kFlags = 8;  // items whose "V holds something not finite" flags are kept; a
                            // flag is used again when the item 6 before is long written
 
 // TMEM columns: S_i at 128 i, O_i at 256 + 128 i; P_i over the first 64 of S_i.
 constexpr std::uint32_t kColO = 256;
 constexpr std::uint32_t kTmemCols = 512;
+
+struct Params {
+    const std::int32_t* q_starts;
+    const std::int32_t* kv_starts;
+    const __half* v;
+    __half* out;
+    std::uint32_t tokens, kv_tokens, batch, q_heads, kv_heads, group;
+    std::uint32_t tile_tokens;  // floor(128 / group)
+    float scale_log2;
+};
+
+// Two query tiles of one sequence and KV head.
+struct Item {
+    std::uint32_t left;    // the sequence's tokens from the first on; 0: no more items
+    std::uint32_t kvh;
+    std::uint32_t q0;      // packed row of the first token
+    std::int32_t pos0;     // its position
+    std::uint32_t k0, nk;  // first row and number of the positions
+    std::uint32_t n[2];    // K/V tiles that each query tile attends
+    std::uint32_t masked;  // the first tile that some row sees in part
+    __device__ __forceinline__ std::uint32_t tiles() const { return max(n[0], n[1]); }
+};
 
 template <int HD>
 struct Smem {
@@ -78,38 +102,16 @@ struct Smem {
     static constexpr int kV = kK + kKV * kTile;
     static constexpr int kBar = kV + kKV * kTile;
     // q_full, q_empty, k_full, k_empty, v_full, v_empty, v_clean [kKV], s_full[2],
-    // p_ready[2], o_done[2], epi_done[2], drained
-    static constexpr int kNumBars = 2 + 5 * kKV + 8 + 1;
+    // p_ready[2], o_done[2], epi_done[2], drained, item_full[kItems], item_empty[kItems]
+    static constexpr int kNumBars = 2 + 5 * kKV + 8 + 1 + 2 * kItems;
     static constexpr int kTmemSlot = kBar + kNumBars * 8;
     static constexpr int kAbort = kTmemSlot + 4;
     static constexpr int kFlag = kAbort + 4;          // [kFlags][kCleanWarps]
-    static constexpr int kUsed = kFlag + 4 * kFlags * kCleanWarps + 1008;  // + alignment slack
+    static constexpr int kItem = kFlag + 4 * kFlags * kCleanWarps;  // [kItems]
+    static constexpr int kUsed = kItem + kItems * static_cast<int>(sizeof(Item)) + 1008;  // + alignment slack
     // one CTA per SM: its 512 TMEM columns never wait for another's
     static constexpr int kBytes = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
     static_assert(kBytes <= 232448, "shared memory");
-};
-
-struct Params {
-    const std::int32_t* q_starts;
-    const std::int32_t* kv_starts;
-    const __half* v;
-    __half* out;
-    std::uint32_t tokens, kv_tokens, batch, q_heads, kv_heads, group;
-    std::uint32_t tile_tokens;  // floor(128 / group)
-    std::uint32_t slots;        // of query tile pairs: tokens / (2 tile_tokens) + batch
-    float scale_log2;
-};
-
-// Two query tiles of one sequence and KV head.
-struct Item {
-    std::uint32_t kvh;
-    std::uint32_t q0;      // packed row of the first token
-    std::uint32_t left;    // the sequence's tokens from there on (0: no item)
-    std::int32_t pos0;     // the first token's position
-    std::uint32_t k0, nk;  // first row and number of the positions
-    std::uint32_t n[2];    // K/V tiles that each query tile attends
-    std::uint32_t masked;  // the first tile that some row sees in part
-    __device__ __forceinline__ std::uint32_t tiles() const { return max(n[0], n[1]); }
 };
 
 __device__ __forceinline__ bool sequence_ok(const Params& p, std::int32_t q0, std::int32_t q1,
@@ -118,25 +120,30 @@ __device__ __forceinline__ bool sequence_ok(const Params& p, std::int32_t q0, st
            k1 >= k0 && static_cast<std::uint32_t>(k1) <= p.kv_tokens;
 }
 
-// Item i, later tiles first (they attend more); by a whole warp.
-__device__ __forceinline__ Item item_at(const Params& p, std::uint32_t i) {
-    Item it;
-    it.left = 0;
-    it.kvh = i % p.kv_heads;
-    const std::uint32_t slot = p.slots - 1 - i / p.kv_heads;
-    const std::uint32_t span = 2 * p.tile_tokens;
-    const auto first = [&](std::uint32_t b) {
-        return static_cast<std::uint32_t>(max(__ldg(p.q_starts + b), 0)) / span + b;
-    };
-    const std::uint32_t b = kvq8::warp_search(p.batch, slot, first);
+// Query tile pairs of sequence b, and the level of the first: pair i of a
+// sequence is at level i + (positions before its queries) / (tokens of a
+// pair), which orders the pairs of all sequences by the tiles they attend.
+struct Pairs {
+    std::uint32_t count, level;
+};
+__device__ __forceinline__ Pairs pairs_of(const Params& p, std::uint32_t b) {
     const std::int32_t q0 = __ldg(p.q_starts + b), q1 = __ldg(p.q_starts + b + 1);
     const std::int32_t k0 = __ldg(p.kv_starts + b), k1 = __ldg(p.kv_starts + b + 1);
-    const std::uint32_t f = first(b);
-    if (!sequence_ok(p, q0, q1, k0, k1) || slot < f) return it;
-    const std::uint64_t t0 = static_cast<std::uint64_t>(slot - f) * span;
-    const std::uint32_t nq = static_cast<std::uint32_t>(q1 - q0);
-    if (t0 >= nq) return it;
-    it.left = nq - static_cast<std::uint32_t>(t0);
+    if (!sequence_ok(p, q0, q1, k0, k1)) return Pairs{0, 0};
+    const std::uint32_t span = 2 * p.tile_tokens, nq = q1 - q0, nk = k1 - k0;
+    return Pairs{(nq + span - 1) / span, nk > nq ? (nk - nq) / span : 0};
+}
+
+// Pair `i` of sequence b for one KV head.
+__device__ __forceinline__ Item make_item(const Params& p, std::uint32_t b, std::uint32_t i,
+                                          std::uint32_t kvh) {
+    Item it{};
+    const std::int32_t q0 = __ldg(p.q_starts + b), q1 = __ldg(p.q_starts + b + 1);
+    const std::int32_t k0 = __ldg(p.kv_starts + b), k1 = __ldg(p.kv_starts + b + 1);
+    const std::uint64_t t0 = static_cast<std::uint64_t>(i) * (2 * p.tile_tokens);
+    if (!sequence_ok(p, q0, q1, k0, k1) || t0 >= static_cast<std::uint32_t>(q1 - q0)) return it;
+    it.kvh = kvh;
+    it.left = static_cast<std::uint32_t>(q1 - q0) - static_cast<std::uint32_t>(t0);
     it.q0 = static_cast<std::uint32_t>(q0) + static_cast<std::uint32_t>(t0);
     it.k0 = static_cast<std::uint32_t>(k0);
     it.nk = static_cast<std::uint32_t>(k1 - k0);
@@ -149,6 +156,55 @@ __device__ __forceinline__ Item item_at(const Params& p, std::uint32_t i) {
     }
     it.masked = static_cast<std::uint32_t>(max(it.pos0 + 1, 0)) / kBN;
     return it;
+}
+
+// Of up to kSorted sequences, the pair of rank r by falling level: N(d) pairs
+// are at level d or above, so r's level is the largest d with N(d) > r, and
+// it is number r - N(d + 1) of the sequences there.  By a whole warp.
+__device__ __forceinline__ Item sorted_item(const Params& p, std::uint32_t r, std::uint32_t levels,
+                                            std::uint32_t kvh) {
+    const std::uint32_t lane = threadIdx.x & 31;
+    const auto at_least = [&](std::uint32_t d) {  // N(d)
+        std::uint32_t n = 0;
+        for (std::uint32_t b = lane; b < p.batch; b += 32) {
+            const Pairs x = pairs_of(p, b);
+            const std::uint32_t end = x.level + x.count;
+            n += end > d ? min(end - d, x.count) : 0u;
+        }
+        return __reduce_add_sync(0xffffffffu, n);
+    };
+    std::uint32_t lo = 0, hi = levels;  // N(lo) > r, N(hi) <= r
+    while (hi - lo > 1) {
+        const std::uint32_t mid = (lo + hi) / 2;
+        if (at_least(mid) > r) lo = mid; else hi = mid;
+    }
+    std::uint32_t e = r - at_least(lo + 1);
+    for (std::uint32_t base = 0; base < p.batch; base += 32) {
+        const std::uint32_t b = base + lane;
+        const Pairs x = b < p.batch ? pairs_of(p, b) : Pairs{0, 0};
+        const bool here = x.level <= lo && lo < x.level + x.count;
+        const unsigned mask = __ballot_sync(0xffffffffu, here);
+        const std::uint32_t k = __popc(mask);
+        if (e >= k) {
+            e -= k;
+            continue;
+        }
+        const int src = __fns(mask, 0, static_cast<int>(e) + 1);
+        return make_item(p, base + src, lo - __shfl_sync(0xffffffffu, x.level, src), kvh);
+    }
+    return Item{};
+}
+
+// Of more, pairs in the order of the sequences: those of sequence b are
+// numbered from floor(q_starts[b] / tokens of a pair) + b on, with gaps.
+__device__ __forceinline__ Item plain_item(const Params& p, std::uint32_t slot, std::uint32_t kvh) {
+    const std::uint32_t span = 2 * p.tile_tokens;
+    const auto first = [&](std::uint32_t b) {
+        return static_cast<std::uint32_t>(max(__ldg(p.q_starts + b), 0)) / span + b;
+    };
+    const std::uint32_t b = kvq8::warp_search(p.batch, slot, first);
+    const std::uint32_t f = first(b);
+    return slot < f ? Item{} : make_item(p, b, slot - f, kvh);
 }
 
 // One lane of the (converged) warp, always the same.
@@ -196,6 +252,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     std::uint64_t* o_done = p_ready + 2;
     std::uint64_t* epi_done = o_done + 2;
     std::uint64_t* drained = epi_done + 2;
+    std::uint64_t* item_full = drained + 1;
+    std::uint64_t* item_empty = item_full + kItems;
+    Item* ring = reinterpret_cast<Item*>(smem + L::kItem);
     volatile std::uint32_t* tmem_slot = reinterpret_cast<volatile std::uint32_t*>(smem + L::kTmemSlot);
     volatile std::uint32_t* abort_flag = reinterpret_cast<volatile std::uint32_t*>(smem + L::kAbort);
     volatile std::uint32_t* not_finite = reinterpret_cast<volatile std::uint32_t*>(smem + L::kFlag);
@@ -218,6 +277,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&o_done[s], 1);
             mbar_init(&epi_done[s], 4);
         }
+        for (int s = 0; s < kItems; ++s) {
+            mbar_init(&item_full[s], 1);
+            mbar_init(&item_empty[s], 11);  // every warp but the producer
+        }
         mbar_init(drained, 1);
         *abort_flag = 0u;
         fence_mbarrier_init();
@@ -235,7 +298,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_launch_dependents();
     pdl_wait();
 
-    const std::uint32_t items = p.slots * p.kv_heads;
+    // item i of this CTA, as the producer found it (by a whole warp other than
+    // the producer's); left == 0 ends the loops, after an abort too
+    const auto item_at = [&](std::uint32_t i) {
+        Item it{};
+        const std::uint32_t s = i % kItems;
+        if (__all_sync(0xffffffffu, wait_or_abort(&item_full[s], (i / kItems) & 1u, abort_flag))) it = ring[s];
+        __syncwarp();
+        if (lane == 0) arrive(&item_empty[s]);
+        return it;
+    };
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == kProducerWarp) {
@@ -243,12 +315,48 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (std::uint32_t b = lane; b < p.batch; b += 32)
                     if (!sequence_ok(p, p.q_starts[b], p.q_starts[b + 1], p.kv_starts[b], p.kv_starts[b + 1]))
                         atomicOr(&g_device_status, kDevIndexOutOfRange);
-            std::uint32_t c = 0, n = 0;  // K/V tiles and items loaded
+            // Items of falling size to the CTAs in turn, forwards and backwards.
+            const std::uint32_t span = 2 * p.tile_tokens;
+            const bool sorted = p.batch <= kSorted;
+            std::uint32_t pairs = p.tokens / span + p.batch, levels = 0;
+            if (sorted) {
+                std::uint32_t count = 0;
+                for (std::uint32_t b = lane; b < p.batch; b += 32) {
+                    const Pairs x = pairs_of(p, b);
+                    count += x.count;
+                    levels = max(levels, x.level + x.count);
+                }
+                pairs = __reduce_add_sync(0xffffffffu, count);
+                levels = __reduce_max_sync(0xffffffffu, levels);
+            }
+            const std::uint32_t items = pairs * p.kv_heads;
+            std::uint32_t c = 0, n = 0, sent = 0;  // K/V tiles, items with any and items so far
             bool ok = true;
-            for (std::uint32_t i = blockIdx.x; ok && i < items; i += gridDim.x) {
-                const Item it = item_at(p, i);
-                const std::uint32_t tiles = it.left ? it.tiles() : 0;
-                if (tiles == 0) continue;
+            for (std::uint32_t round = 0; ok; ++round) {
+                const std::uint64_t at = static_cast<std::uint64_t>(round) * gridDim.x +
+                                         (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                Item it{};
+                if (at < items) {
+                    const std::uint32_t r = static_cast<std::uint32_t>(at) / p.kv_heads;
+                    const std::uint32_t kvh = static_cast<std::uint32_t>(at) % p.kv_heads;
+                    it = sorted ? sorted_item(p, r, levels, kvh) : plain_item(p, r, kvh);
+                    if (it.left == 0) continue;
+                } else if (static_cast<std::uint64_t>(round) * gridDim.x < items) {
+                    continue;  // the last round is not full
+                }
+                if (lane == 0) {
+                    const std::uint32_t s = sent % kItems;
+                    ok = sent < kItems || wait_or_abort(&item_empty[s], (sent / kItems - 1) & 1u, abort_flag);
+                    if (ok) {
+                        ring[s] = it;
+                        arrive(&item_full[s]);
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+                ++sent;
+                if (it.left == 0) break;
+                const std::uint32_t tiles = it.tiles();
+                if (tiles == 0 || !ok) continue;
                 if (lane == 0) {
                     ok = n == 0 || wait_or_abort(q_empty, (n - 1) & 1u, abort_flag);
                     if (ok) {
@@ -295,10 +403,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag)) != 0;
             };
             bool ok = true;
-            for (std::uint32_t i = blockIdx.x; ok && i < items; i += gridDim.x) {
-                const Item it = item_at(p, i);
-                const std::uint32_t n0 = __reduce_max_sync(0xffffffffu, it.left ? it.n[0] : 0u);
-                const std::uint32_t n1 = __reduce_max_sync(0xffffffffu, it.left ? it.n[1] : 0u);
+            for (std::uint32_t i = 0; ok; ++i) {
+                const Item it = item_at(i);
+                if (it.left == 0) break;
+                const std::uint32_t n0 = __reduce_max_sync(0xffffffffu, it.n[0]);
+                const std::uint32_t n1 = __reduce_max_sync(0xffffffffu, it.n[1]);
                 const std::uint32_t masked = __reduce_max_sync(0xffffffffu, it.masked);
                 const std::uint32_t tiles = max(n0, n1);
                 if (tiles == 0) continue;
@@ -387,9 +496,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             std::uint32_t c = 0, n = 0, clean = 0;
             bool ok = true;
             const int me = threadIdx.x - 10 * 32;  // of 64
-            for (std::uint32_t i = blockIdx.x; ok && i < items; i += gridDim.x) {
-                const Item it = item_at(p, i);
-                const std::uint32_t tiles = it.left ? it.tiles() : 0;
+            for (std::uint32_t i = 0; ok; ++i) {
+                const Item it = item_at(i);
+                if (it.left == 0) break;
+                const std::uint32_t tiles = it.tiles();
                 if (tiles == 0) continue;
                 volatile std::uint32_t* flag = not_finite + n % kFlags * kCleanWarps + (warp - 10);
                 if (lane == 0) *flag = 0u;
@@ -446,9 +556,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float sc = p.scale_log2;
         std::uint32_t cnt = 0, n = 0;  // tiles of this query tile, items
         bool ok = true;
-        for (std::uint32_t i = blockIdx.x; i < items; i += gridDim.x) {
-            const Item it = item_at(p, i);
-            if (it.left == 0) continue;
+        for (std::uint32_t i = 0;; ++i) {
+            const Item it = item_at(i);
+            if (it.left == 0) break;
             const std::uint32_t token = m * p.tile_tokens + tok;  // from the item's first
             const bool mine = tok < p.tile_tokens && token < it.left;
             const std::int32_t limit = it.pos0 + static_cast<std::int32_t>(token);  // its position
@@ -639,7 +749,9 @@ int launch(const Params& p, const void* q, const void* k, cudaStream_t stream) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return static_cast<int>(e);
-    const std::uint64_t items = static_cast<std::uint64_t>(p.slots) * p.kv_heads;
+    // (at most; how many there are is known on the device)
+    const std::uint64_t items = (static_cast<std::uint64_t>(p.tokens) / (2 * p.tile_tokens) + p.batch) * p.kv_heads;
+    if (items > 0x7fffffffull) return kInvalidValue;
     const unsigned grid = static_cast<unsigned>(items < static_cast<std::uint64_t>(sms) ? items : sms);
     return launch_pdl_smem(packed_kernel<HD>, dim3(grid), dim3(kThreads), Smem<HD>::kBytes, stream,
                            map_q, map_k, map_v, p);
@@ -677,9 +789,7 @@ extern "C" int mote_cuda_gqa_attention_packed_f16(const void* q, const void* k, 
     p.kv_heads = static_cast<std::uint32_t>(kv_heads);
     p.group = static_cast<std::uint32_t>(q_heads / kv_heads);
     p.tile_tokens = attnv::kBM / p.group;
-    p.slots = static_cast<std::uint32_t>(tokens / (2 * p.tile_tokens) + batch);
     p.scale_log2 = scale * 1.4426950408889634f;
-    if (static_cast<std::uint64_t>(p.slots) * kv_heads > 0x7fffffffull) return kInvalidValue;
     const auto s = static_cast<cudaStream_t>(stream);
     return head_dim == 64 ? attnv::launch<64>(p, q, k, s) : attnv::launch<128>(p, q, k, s);
 }
