@@ -42,7 +42,6 @@ using attnp::ex2f;
 using attnp::max3f;
 using attnp::tma_load_3d;
 using attnp::tmem_ld32_nowait;
-using attnp::tmem_st32;
 using attnp::tmem_wait_ld;
 using attnp::tmem_wait_st;
 using attnp::umma_f16_ss;
@@ -102,8 +101,8 @@ struct Smem {
     static constexpr int kV = kK + kKV * kTile;
     static constexpr int kBar = kV + kKV * kTile;
     // q_full, q_empty, k_full, k_empty, v_full, v_empty, v_clean [kKV], s_full[2],
-    // p_ready[2], o_done[2], epi_done[2], drained, item_full[kItems], item_empty[kItems]
-    static constexpr int kNumBars = 2 + 5 * kKV + 8 + 1 + 2 * kItems;
+    // p_ready[2], p_half[2], o_done[2], epi_done[2], drained, item_full[kItems], item_empty[kItems]
+    static constexpr int kNumBars = 2 + 5 * kKV + 10 + 1 + 2 * kItems;
     static constexpr int kTmemSlot = kBar + kNumBars * 8;
     static constexpr int kAbort = kTmemSlot + 4;
     static constexpr int kFlag = kAbort + 4;          // [kFlags][kCleanWarps]
@@ -158,18 +157,19 @@ __device__ __forceinline__ Item make_item(const Params& p, std::uint32_t b, std:
     return it;
 }
 
-// Of up to kSorted sequences, the pair of rank r by falling level: N(d) pairs
-// are at level d or above, so r's level is the largest d with N(d) > r, and
-// it is number r - N(d + 1) of the sequences there.  By a whole warp.
-__device__ __forceinline__ Item sorted_item(const Params& p, std::uint32_t r, std::uint32_t levels,
-                                            std::uint32_t kvh) {
-    const std::uint32_t lane = threadIdx.x & 31;
+// Of up to kSorted sequences, whose pairs the lanes hold (sequence 32 i + lane
+// in x[i]): the pair of rank r by falling level.  N(d) pairs are at level d
+// or above, so r's level is the largest d with N(d) > r, and it is number
+// r - N(d + 1) of the sequences there.  By a whole warp.
+constexpr int kHeld = kSorted / 32;
+__device__ __forceinline__ Item sorted_item(const Params& p, const Pairs (&x)[kHeld], std::uint32_t r,
+                                            std::uint32_t levels, std::uint32_t kvh) {
     const auto at_least = [&](std::uint32_t d) {  // N(d)
         std::uint32_t n = 0;
-        for (std::uint32_t b = lane; b < p.batch; b += 32) {
-            const Pairs x = pairs_of(p, b);
-            const std::uint32_t end = x.level + x.count;
-            n += end > d ? min(end - d, x.count) : 0u;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) {
+            const std::uint32_t end = x[i].level + x[i].count;
+            n += end > d ? min(end - d, x[i].count) : 0u;
         }
         return __reduce_add_sync(0xffffffffu, n);
     };
@@ -178,21 +178,24 @@ __device__ __forceinline__ Item sorted_item(const Params& p, std::uint32_t r, st
         const std::uint32_t mid = (lo + hi) / 2;
         if (at_least(mid) > r) lo = mid; else hi = mid;
     }
-    std::uint32_t e = r - at_least(lo + 1);
-    for (std::uint32_t base = 0; base < p.batch; base += 32) {
-        const std::uint32_t b = base + lane;
-        const Pairs x = b < p.batch ? pairs_of(p, b) : Pairs{0, 0};
-        const bool here = x.level <= lo && lo < x.level + x.count;
+    std::uint32_t e = r - at_least(lo + 1), b = 0, first = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const bool here = x[i].level <= lo && lo < x[i].level + x[i].count;
         const unsigned mask = __ballot_sync(0xffffffffu, here);
         const std::uint32_t k = __popc(mask);
-        if (e >= k) {
-            e -= k;
-            continue;
+        // the lane with e such sequences below it
+        const unsigned below = mask & ((1u << (threadIdx.x & 31)) - 1u);
+        const unsigned pick = __ballot_sync(0xffffffffu, here && __popc(below) == e);
+        if (!found && e < k) {
+            const int src = __ffs(pick) - 1;
+            found = true, b = 32 * i + src;
+            first = __shfl_sync(0xffffffffu, x[i].level, src);
         }
-        const int src = __fns(mask, 0, static_cast<int>(e) + 1);
-        return make_item(p, base + src, lo - __shfl_sync(0xffffffffu, x.level, src), kvh);
+        if (!found) e -= k;
     }
-    return Item{};
+    return make_item(p, b, lo - first, kvh);
 }
 
 // Of more, pairs in the order of the sequences: those of sequence b are
@@ -205,6 +208,26 @@ __device__ __forceinline__ Item plain_item(const Params& p, std::uint32_t slot, 
     const std::uint32_t b = kvq8::warp_search(p.batch, slot, first);
     const std::uint32_t f = first(b);
     return slot < f ? Item{} : make_item(p, b, slot - f, kvh);
+}
+
+// 32 lanes x 16 consecutive columns.
+__device__ __forceinline__ void tmem_ld16(std::uint32_t taddr, std::uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(std::uint32_t taddr, const std::uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15])
+        : "memory");
 }
 
 // One lane of the (converged) warp, always the same.
@@ -249,7 +272,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     std::uint64_t* v_clean = v_empty + kKV;
     std::uint64_t* s_full = v_clean + kKV;
     std::uint64_t* p_ready = s_full + 2;
-    std::uint64_t* o_done = p_ready + 2;
+    std::uint64_t* p_half = p_ready + 2;
+    std::uint64_t* o_done = p_half + 2;
     std::uint64_t* epi_done = o_done + 2;
     std::uint64_t* drained = epi_done + 2;
     std::uint64_t* item_full = drained + 1;
@@ -274,6 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int s = 0; s < 2; ++s) {
             mbar_init(&s_full[s], 1);
             mbar_init(&p_ready[s], 4);
+            mbar_init(&p_half[s], 4);
             mbar_init(&o_done[s], 1);
             mbar_init(&epi_done[s], 4);
         }
@@ -319,12 +344,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             const std::uint32_t span = 2 * p.tile_tokens;
             const bool sorted = p.batch <= kSorted;
             std::uint32_t pairs = p.tokens / span + p.batch, levels = 0;
+            Pairs held[kHeld];
+#pragma unroll
+            for (int x = 0; x < kHeld; ++x)
+                held[x] = sorted && 32u * x + lane < p.batch ? pairs_of(p, 32 * x + lane) : Pairs{0, 0};
             if (sorted) {
                 std::uint32_t count = 0;
-                for (std::uint32_t b = lane; b < p.batch; b += 32) {
-                    const Pairs x = pairs_of(p, b);
-                    count += x.count;
-                    levels = max(levels, x.level + x.count);
+#pragma unroll
+                for (int x = 0; x < kHeld; ++x) {
+                    count += held[x].count;
+                    levels = max(levels, held[x].level + held[x].count);
                 }
                 pairs = __reduce_add_sync(0xffffffffu, count);
                 levels = __reduce_max_sync(0xffffffffu, levels);
@@ -339,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (at < items) {
                     const std::uint32_t r = static_cast<std::uint32_t>(at) / p.kv_heads;
                     const std::uint32_t kvh = static_cast<std::uint32_t>(at) % p.kv_heads;
-                    it = sorted ? sorted_item(p, r, levels, kvh) : plain_item(p, r, kvh);
+                    it = sorted ? sorted_item(p, held, r, levels, kvh) : plain_item(p, r, kvh);
                     if (it.left == 0) continue;
                 } else if (static_cast<std::uint64_t>(round) * gridDim.x < items) {
                     continue;  // the last round is not full
@@ -362,6 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (ok) {
                         const std::uint32_t box = p.tile_tokens * p.group * 128;
                         mbar_arrive_expect_tx(q_full, ((it.n[0] > 0) + (it.n[1] > 0)) * (HD / 64) * box);
+#pragma unroll
                         for (int m = 0; m < 2; ++m)
                             for (int h = 0; h < HD / 64 && it.n[m] > 0; ++h)
                                 tma_load_3d(base + L::kQ + m * L::kTile + h * L::kHalf, &map_q, 64 * h,
@@ -458,14 +488,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                             unread[m] = false;
                         }
                         if (!ok || j >= (m ? n1 : n0)) continue;
-                        ok = wait(&p_ready[m], done[m] & 1u);
+                        ok = wait(&p_half[m], done[m] & 1u);
                         if (!ok) continue;
                         gemm::tc_fence_after();
                         const std::uint64_t vd = v_desc<HD>(base + L::kV + s * L::kTile);
                         const bool last = m == 1 || j >= n1;
                         if (elect_one()) {
 #pragma unroll
-                            for (int k = 0; k < kBN / 16; ++k)
+                            for (int k = 0; k < kBN / 32; ++k)
+                                gemm::umma_f16_ta(tm + kColO + 128u * m, tm + 128u * m + k * 8,
+                                                  vd + k * (2048 >> 4), kIdescPV, (j | k) != 0 ? 1u : 0u);
+                        }
+                        __syncwarp();
+                        ok = wait(&p_ready[m], done[m] & 1u);
+                        if (!ok) continue;
+                        gemm::tc_fence_after();
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = kBN / 32; k < kBN / 16; ++k)
                                 gemm::umma_f16_ta(tm + kColO + 128u * m, tm + 128u * m + k * 8,
                                                   vd + k * (2048 >> 4), kIdescPV, (j | k) != 0 ? 1u : 0u);
                             gemm::umma_commit(smem_u32(&o_done[m]));
@@ -562,8 +602,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const std::uint32_t token = m * p.tile_tokens + tok;  // from the item's first
             const bool mine = tok < p.tile_tokens && token < it.left;
             const std::int32_t limit = it.pos0 + static_cast<std::int32_t>(token);  // its position
-            const std::int32_t first = it.pos0 + static_cast<std::int32_t>(m * p.tile_tokens);
-            const std::uint32_t tiles = it.n[m];
+            // the least position of the warp's rows
+            const std::int32_t least = it.pos0 + static_cast<std::int32_t>(
+                m * p.tile_tokens + 32u * (warp % 4) / p.group);
+            const std::uint32_t tiles = m ? it.n[1] : it.n[0];
             float mx_ref = -INFINITY, l = 0.f;
             for (std::uint32_t j = 0; j < tiles && ok; ++j, ++cnt) {
                 ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[m], cnt & 1u, abort_flag));
@@ -573,15 +615,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int cc = 0; cc < 4; ++cc) tmem_ld32_nowait(s_col + 32 * cc, v[cc]);
                 tmem_wait_ld();
-                // causal mask; the scale is positive, so the maximum of the raw
-                // scores gives that of the scaled ones
+                // causal mask, only in the 32 columns where the warp's rows differ
+                // from all or nothing; the scale is positive, so the maximum of the
+                // raw scores gives that of the scaled ones
                 const std::int32_t kbase = static_cast<std::int32_t>(j * kBN);
-                if (kbase + kBN - 1 > first) {
+                if (kbase + kBN - 1 > least) {
 #pragma unroll
-                    for (int cc = 0; cc < 4; ++cc)
+                    for (int cc = 0; cc < 4; ++cc) {
+                        const std::int32_t seen = limit - (kbase + 32 * cc) + 1;  // of these columns
+                        if (least - (kbase + 32 * cc) + 1 >= 32) continue;
+                        const std::uint32_t bits = seen >= 32 ? 0xffffffffu : seen <= 0 ? 0u : (1u << seen) - 1u;
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (kbase + 32 * cc + e > limit) v[cc][e] = __float_as_uint(-INFINITY);
+                            if (!(bits >> e & 1u)) v[cc][e] = __float_as_uint(-INFINITY);
+                    }
                 }
                 float mx8[8];
 #pragma unroll
@@ -592,23 +639,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int e = 0; e < 32; e += 2)
                         mx8[(e / 2) % 8] = max3f(mx8[(e / 2) % 8], __uint_as_float(v[cc][e]),
                                                  __uint_as_float(v[cc][e + 1]));
-                const float mx = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                                       fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
+                const float mx = max3f(max3f(mx8[0], mx8[1], mx8[2]), max3f(mx8[3], mx8[4], mx8[5]),
+                                       fmaxf(mx8[6], mx8[7]));
                 // the reference moves only when a score passes it by more than 8
                 // (P stays below 2^8); -infinity while the row has seen nothing
                 const float mnew = fmaxf(mx_ref, mx);
                 const bool grow = (mnew - mx_ref) * sc > 8.f;  // false while both are -inf (NaN)
-                float alpha = 1.f;
-                if (grow) {
-                    alpha = ex2f((mx_ref - mnew) * sc);  // 0 from -infinity
-                    mx_ref = mnew;
+                if (__any_sync(0xffffffffu, grow)) {
+                    float alpha = 1.f;
+                    if (grow) {
+                        alpha = ex2f((mx_ref - mnew) * sc);  // 0 from -infinity
+                        mx_ref = mnew;
+                        l *= alpha;
+                    }
+                    if (j > 0) {
+                        // the previous P V is complete before O moves
+                        ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[m], (cnt - 1) & 1u, abort_flag));
+                        if (!ok) break;
+                        gemm::tc_fence_after();
+#pragma unroll
+                        for (int cc = 0; cc < HD / 16; ++cc) {
+                            std::uint32_t o[16];
+                            tmem_ld16(o_col + 16 * cc, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                            tmem_st16(o_col + 16 * cc, o);
+                        }
+                    }
                 }
                 const float neg = mx_ref == -INFINITY ? 0.f : -mx_ref * sc;
                 const std::uint64_t sc2 = attnp::pack_f32x2(sc, sc), neg2 = attnp::pack_f32x2(neg, neg);
-                std::uint64_t acc2[4] = {0, 0, 0, 0};
-                std::uint32_t pk[2][32];
+                std::uint64_t acc2[2] = {0, 0};
+                // P of 32 columns at a time; the first P V steps start on the first
+                // half of P while the second is computed
 #pragma unroll
-                for (int cc = 0; cc < 4; ++cc)
+                for (int cc = 0; cc < 4; ++cc) {
+                    std::uint32_t pk[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         float xa, xb;
@@ -617,41 +684,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                              sc2, neg2),
                                             xa, xb);
                         const float a = ex2f(xa), b = ex2f(xb);
-                        acc2[(e / 2) % 4] = attnp::add_f32x2(acc2[(e / 2) % 4], attnp::pack_f32x2(a, b));
-                        std::uint32_t h2;
-                        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h2) : "f"(b), "f"(a));
-                        pk[cc / 2][(cc % 2) * 16 + e / 2] = h2;
+                        acc2[e / 2 % 2] = attnp::add_f32x2(acc2[e / 2 % 2], attnp::pack_f32x2(a, b));
+                        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(pk[e / 2]) : "f"(b), "f"(a));
                     }
-                float sum = 0.f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x0, x1;
-                    attnp::unpack_f32x2(acc2[e], x0, x1);
-                    sum += x0 + x1;
+                    if (cc == 2) {  // the stores of the first half have landed meanwhile
+                        tmem_wait_st();
+                        gemm::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) arrive(&p_half[m]);
+                    }
+                    tmem_st16(s_col + 16 * cc, pk);
                 }
-                l = fmaf(l, alpha, sum);
-                tmem_st32(s_col, pk[0]);
-                tmem_st32(s_col + 32, pk[1]);
                 tmem_wait_st();
-                if (j > 0 && __any_sync(0xffffffffu, grow)) {
-                    // the previous P V is complete before O moves
-                    ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[m], (cnt - 1) & 1u, abort_flag));
-                    if (!ok) break;
-                    gemm::tc_fence_after();
-#pragma unroll
-                    for (int cc = 0; cc < HD / 32; ++cc) {
-                        std::uint32_t o[32];
-                        tmem_ld32_nowait(o_col + 32 * cc, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tmem_st32(o_col + 32 * cc, o);
-                    }
-                    tmem_wait_st();
-                }
                 gemm::tc_fence_before();
                 __syncwarp();
                 if (lane == 0) arrive(&p_ready[m]);
+                float x0, x1, y0, y1;
+                attnp::unpack_f32x2(acc2[0], x0, x1);
+                attnp::unpack_f32x2(acc2[1], y0, y1);
+                l += (x0 + x1) + (y0 + y1);
             }
             // O / sum; rows before the first position have no sum and get zeros
             if (it.tiles() > 0) ++n;
