@@ -289,16 +289,20 @@ class CudaContext:
                                   head_dim: int) -> int:
         """mote_cuda_gqa_attention_decode_q8_workspace_bytes, memoised (it
         depends only on the shape and this context's device)."""
-        cache = self.__dict__.setdefault("_q8_need", {})
         key = (batch, q_heads, kv_heads, head_dim)
-        need = cache.get(key)
-        if need is None:
+        try:
+            return self._q8_need[key]
+        except AttributeError:
+            self._q8_need = {}
+        except KeyError:
+            pass
+        if key not in self._q8_need:
             out = ctypes.c_uint64(0)
             self.inner.select()
             errors.check(lib().mote_cuda_gqa_attention_decode_q8_workspace_bytes(
                 *key, ctypes.byref(out)), "query 8-bit attention workspace")
-            need = cache[key] = out.value
-        return need
+            self._q8_need[key] = out.value
+        return self._q8_need[key]
 
     def decode_q8_workspace(self, nbytes: int) -> tuple[int, int]:
         """A zeroed device workspace of at least ``nbytes`` for the 8-bit

@@ -121,6 +121,7 @@ __device__ __forceinline__ void check_starts(const CacheShape& c, const std::int
 }
 
 constexpr int kThreads = 128;
+constexpr int kHeld = 8;  // 16-byte vectors of a thread
 
 __device__ __forceinline__ std::uint32_t round_to_int8(float x, float m) {
     return static_cast<std::uint32_t>(__float_as_int(__fmaf_rn(x, m, 12582912.f))) & 0xffu;
@@ -150,13 +151,28 @@ __global__ void __launch_bounds__(kThreads)
     float* scale = (blockIdx.z ? v_scales : k_scales) + tile;
     const float s_old = part.off == 0 ? 0.f : *scale;
 
-    // the largest |x|: f16 magnitudes order as their bits, NaN above infinity
+    // the largest |x|: f16 magnitudes order as their bits, NaN above infinity.
+    // The first kHeld vectors of a thread stay in registers (all of them, for
+    // blocks of up to 64 tokens), so they are in flight together and read once.
+    const std::uint32_t total = part.count * vecs;
+    const auto load = [&](std::uint32_t i) {
+        return __ldg(reinterpret_cast<const uint4*>(src + (i / vecs) * row_stride) + i % vecs);
+    };
+    const auto largest = [](const uint4& x) {
+        return __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
+                        __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+    };
     std::uint32_t top = 0;
-    for (std::uint32_t i = threadIdx.x; i < part.count * vecs; i += kThreads) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + (i / vecs) * row_stride) + i % vecs);
-        top = __vmaxu2(top, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu),
-                                     __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+    uint4 held[kHeld];
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+        const std::uint32_t i = threadIdx.x + k * kThreads;
+        held[k] = i < total ? load(i) : make_uint4(0, 0, 0, 0);
     }
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) top = __vmaxu2(top, largest(held[k]));
+    for (std::uint32_t i = threadIdx.x + kHeld * kThreads; i < total; i += kThreads)
+        top = __vmaxu2(top, largest(load(i)));
     top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16));
     if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x / 32] = top;
     __syncthreads();  // every thread has read the old scale
@@ -168,18 +184,23 @@ __global__ void __launch_bounds__(kThreads)
                                : __int_as_float(0x7fc00000);
     const float inv = s_new > 0.f ? __fdiv_rn(1.f, s_new) : 0.f;
     if (threadIdx.x == 0) *scale = s_new;
-    for (std::uint32_t i = threadIdx.x; i < part.count * vecs; i += kThreads) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(src + (i / vecs) * row_stride) + i % vecs);
+    const auto store = [&](const uint4& x, std::uint32_t i) {
         const std::uint32_t w[4] = {x.x, x.y, x.z, x.w};
         std::uint32_t q[2] = {0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            q[e / 4] |= round_to_int8(half_bits_to_float(w[e / 2] >> (16 * (e & 1)) & 0xffffu), inv)
-                        << (8 * (e & 3));
+        for (int e = 0; e < 4; ++e) {
+            const float a = half_bits_to_float(w[e] & 0xffffu), b = half_bits_to_float(w[e] >> 16);
+            q[e / 2] |= (round_to_int8(a, inv) | round_to_int8(b, inv) << 8) << (16 * (e & 1));
+        }
         if (!finite) q[0] = q[1] = 0;
-        reinterpret_cast<uint2*>(dst + (part.off + i / vecs) * c.head_dim)[i % vecs] =
-            make_uint2(q[0], q[1]);
+        reinterpret_cast<uint2*>(dst + part.off * c.head_dim)[i] = make_uint2(q[0], q[1]);
+    };
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+        const std::uint32_t i = threadIdx.x + k * kThreads;
+        if (i < total) store(held[k], i);
     }
+    for (std::uint32_t i = threadIdx.x + kHeld * kThreads; i < total; i += kThreads) store(load(i), i);
     if (part.off != 0 && !(s_new == s_old)) {  // rows already there, on the new scale
         const float ratio = finite ? __fmul_rn(s_old, inv) : 0.f;
         uint4* old = reinterpret_cast<uint4*>(dst);
@@ -214,24 +235,33 @@ __global__ void __launch_bounds__(kThreads)
                   [&](std::uint32_t, std::uint32_t n) -> std::int64_t { return n; });
     if (part.block < 0) return;
     const std::uint32_t h = blockIdx.y;
-    const std::uint32_t vecs = c.head_dim / 8;
+    const std::uint32_t vecs = c.head_dim / 8;  // 8 bytes of a cached row, 16 of the result's
     const std::uint64_t row_stride = static_cast<std::uint64_t>(c.kv_heads) * c.head_dim;
     const std::uint64_t tile = static_cast<std::uint64_t>(part.block) * c.kv_heads + h;
     const std::int8_t* src = (blockIdx.z ? v_cache : k_cache) + (tile * c.block_tokens + part.off) * c.head_dim;
     const float scale = (blockIdx.z ? v_scales : k_scales)[tile];
     __half* dst = (blockIdx.z ? v_out : k_out) + part.row * row_stride + h * c.head_dim;
-    for (std::uint32_t i = threadIdx.x; i < part.count * vecs; i += kThreads) {
-        const uint2 x = reinterpret_cast<const uint2*>(src)[i];
-        std::uint32_t o[4];
+    const std::uint32_t total = part.count * vecs;
+    for (std::uint32_t base = threadIdx.x; base < total; base += kHeld * kThreads) {
+        uint2 held[kHeld];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const std::uint32_t w = (e < 2 ? x.x : x.y) >> (16 * (e & 1));
-            const float a = static_cast<float>(static_cast<std::int8_t>(w)) * scale;
-            const float b = static_cast<float>(static_cast<std::int8_t>(w >> 8)) * scale;
-            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(o[e]) : "f"(b), "f"(a));
+        for (int k = 0; k < kHeld; ++k)
+            if (base + k * kThreads < total) held[k] = __ldg(reinterpret_cast<const uint2*>(src) + base + k * kThreads);
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            const std::uint32_t i = base + k * kThreads;
+            if (i >= total) break;
+            std::uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const std::uint32_t y = (e < 2 ? held[k].x : held[k].y) >> (16 * (e & 1));
+                const float a = static_cast<float>(static_cast<std::int8_t>(y)) * scale;
+                const float b = static_cast<float>(static_cast<std::int8_t>(y >> 8)) * scale;
+                asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(o[e]) : "f"(b), "f"(a));
+            }
+            reinterpret_cast<uint4*>(dst + (i / vecs) * row_stride)[i % vecs] =
+                make_uint4(o[0], o[1], o[2], o[3]);
         }
-        reinterpret_cast<uint4*>(dst + (i / vecs) * row_stride)[i % vecs] =
-            make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 

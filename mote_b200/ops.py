@@ -21,7 +21,7 @@ import math
 
 from . import errors
 from ._native import lib
-from .context import CudaContext, Tensor
+from .context import CudaContext, CudaStorage, Tensor
 from .types import DType, QuantFormat, RopeLayout, TensorDesc
 
 U32_MAX = 0xFFFFFFFF
@@ -771,26 +771,32 @@ def gqa_attention_prefill_f16(context: CudaContext, q: Tensor, k_cache: Tensor, 
 
 
 # ------------------------------------------------ KV cache held in 8 bits --
-def _q8_cache(k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: Tensor,
-              block_tables: Tensor) -> tuple[int, ...]:
-    """(num_blocks, kv_heads, block_tokens, head_dim, batch, max_blocks)."""
-    _plain(k_cache, "k_cache", DType.I8)
-    _rank(k_cache, "k_cache", 4)
-    _plain(v_cache, "v_cache", DType.I8)
-    _shape(v_cache, "v_cache", k_cache.shape)
-    blocks, kvh, bt, hd = k_cache.shape
-    _plain(k_scales, "k_scales", DType.F32)
-    _shape(k_scales, "k_scales", (blocks, kvh))
-    _plain(v_scales, "v_scales", DType.F32)
-    _shape(v_scales, "v_scales", (blocks, kvh))
-    _plain(block_tables, "block_tables", DType.I32)
-    _rank(block_tables, "block_tables", 2)
-    return (blocks, kvh, bt, hd, *block_tables.shape)
+def _operands(context: CudaContext, *operands) -> list[int]:
+    """The pointers of ``(tensor, name, dtype, shape)`` operands after the
+    checks of the other operators (plain encoding, rank, shape, ownership,
+    offset, layout), in one pass: calls of a few microseconds count here."""
+    inner = getattr(context, "inner", None)
+    pointers = []
+    for tensor, name, dtype, shape in operands:
+        desc = tensor.desc
+        if desc.encoding.plain is not dtype or desc.shape != shape:
+            _plain(tensor, name, dtype)
+            _rank(tensor, name, len(shape))
+            _shape(tensor, name, shape)
+        storage = tensor.storage
+        if (storage.__class__ is CudaStorage and storage.context is inner
+                and tensor.byte_offset == 0 and desc.is_contiguous):
+            pointers.append(storage.pointer)
+    if len(pointers) != len(operands):  # let the context name what is wrong
+        return [context.storage(operand[0]).pointer for operand in operands]
+    return pointers
 
 
-def _i32_vector(tensor: Tensor, name: str, length: int) -> None:
-    _plain(tensor, name, DType.I32)
-    _shape(tensor, name, (length,))
+def _dims(tensor: Tensor, name: str, rank: int) -> tuple[int, ...]:
+    shape = tensor.desc.shape
+    if len(shape) != rank:
+        _rank(tensor, name, rank)
+    return shape
 
 
 def _error_flag(context: CudaContext, name: str) -> int:
@@ -831,27 +837,26 @@ def kv_cache_append_q8(context: CudaContext, k_new: Tensor, v_new: Tensor, k_cac
     synchronizes and raises :class:`errors.IndexOutOfRange` for offsets,
     lengths or blocks out of range (those rows are skipped); without it they
     set the device status."""
-    blocks, kvh, bt, hd, batch, width = _q8_cache(k_cache, v_cache, k_scales, v_scales,
-                                                  block_tables)
-    _plain(k_new, "k_new", DType.F16)
-    _rank(k_new, "k_new", 3)
-    tokens = k_new.shape[0]
-    _shape(k_new, "k_new", (tokens, kvh, hd))
-    _plain(v_new, "v_new", DType.F16)
-    _shape(v_new, "v_new", k_new.shape)
-    _i32_vector(seq_starts, "seq_starts", batch + 1)
-    _i32_vector(seq_lens, "seq_lens", batch)
+    blocks, kvh, bt, hd = cache = _dims(k_cache, "k_cache", 4)
+    batch, width = tables = _dims(block_tables, "block_tables", 2)
+    tokens = _dims(k_new, "k_new", 3)[0]
+    rows, scales = (tokens, kvh, hd), (blocks, kvh)
+    f16, i8, f32, i32 = DType.F16, DType.I8, DType.F32, DType.I32
     _not_aliased(k_cache, "k_cache", v_cache, "v_cache")
     _not_aliased(k_scales, "k_scales", v_scales, "v_scales")
-    storage = context.storage
-    ptrs = [storage(t).pointer for t in (k_new, v_new, k_cache, v_cache, k_scales, v_scales,
-                                         block_tables, seq_starts, seq_lens)]
+    ptrs = _operands(context, (k_new, "k_new", f16, rows), (v_new, "v_new", f16, rows),
+                     (k_cache, "k_cache", i8, cache), (v_cache, "v_cache", i8, cache),
+                     (k_scales, "k_scales", f32, scales), (v_scales, "v_scales", f32, scales),
+                     (block_tables, "block_tables", i32, tables),
+                     (seq_starts, "seq_starts", i32, (batch + 1,)),
+                     (seq_lens, "seq_lens", i32, (batch,)))
     if tokens == 0:
         return
     flag = _error_flag(context, "_append_q8_flag") if check else None
-    context.inner.select()
+    inner = context.inner
+    inner.select()
     st = lib().mote_cuda_kv_cache_append_q8(*ptrs, tokens, batch, kvh, hd, blocks, bt, width,
-                                            flag, context.inner.stream)
+                                            flag, inner.stream)
     if st:
         errors.check(st, "launch 8-bit KV-cache append kernel")
     if check:
@@ -867,25 +872,24 @@ def kv_cache_read_q8(context: CudaContext, k_cache: Tensor, v_cache: Tensor, k_s
     :func:`gqa_attention_packed_f16` takes for prompts continued over cached
     positions.  Rows of no sequence keep their values; ``check`` as in
     :func:`kv_cache_append_q8`."""
-    blocks, kvh, bt, hd, batch, width = _q8_cache(k_cache, v_cache, k_scales, v_scales,
-                                                  block_tables)
-    _plain(k_out, "k_out", DType.F16)
-    _rank(k_out, "k_out", 3)
-    tokens = k_out.shape[0]
-    _shape(k_out, "k_out", (tokens, kvh, hd))
-    _plain(v_out, "v_out", DType.F16)
-    _shape(v_out, "v_out", k_out.shape)
-    _i32_vector(starts, "starts", batch + 1)
+    blocks, kvh, bt, hd = cache = _dims(k_cache, "k_cache", 4)
+    batch, width = tables = _dims(block_tables, "block_tables", 2)
+    tokens = _dims(k_out, "k_out", 3)[0]
+    rows, scales = (tokens, kvh, hd), (blocks, kvh)
+    f16, i8, f32, i32 = DType.F16, DType.I8, DType.F32, DType.I32
     _not_aliased(k_out, "k_out", v_out, "v_out")
-    storage = context.storage
-    ptrs = [storage(t).pointer for t in (k_cache, v_cache, k_scales, v_scales, block_tables,
-                                         starts, k_out, v_out)]
+    ptrs = _operands(context, (k_cache, "k_cache", i8, cache), (v_cache, "v_cache", i8, cache),
+                     (k_scales, "k_scales", f32, scales), (v_scales, "v_scales", f32, scales),
+                     (block_tables, "block_tables", i32, tables),
+                     (starts, "starts", i32, (batch + 1,)),
+                     (k_out, "k_out", f16, rows), (v_out, "v_out", f16, rows))
     if tokens == 0:
         return
     flag = _error_flag(context, "_read_q8_flag") if check else None
-    context.inner.select()
+    inner = context.inner
+    inner.select()
     st = lib().mote_cuda_kv_cache_read_q8(*ptrs, tokens, batch, kvh, hd, blocks, bt, width, flag,
-                                          context.inner.stream)
+                                          inner.stream)
     if st:
         errors.check(st, "launch 8-bit KV-cache read kernel")
     if check:
@@ -901,27 +905,26 @@ def gqa_attention_decode_q8(context: CudaContext, q: Tensor, k_cache: Tensor, v_
     q_heads // kv_heads``; q and output [batch, q_heads, head_dim] f16.  A
     sequence of length 0 gets zeros; blocks out of range count as not there
     and set the device status.  ``scale`` defaults to ``1 / sqrt(head_dim)``."""
-    blocks, kvh, bt, hd, batch, width = _q8_cache(k_cache, v_cache, k_scales, v_scales,
-                                                  block_tables)
-    _plain(q, "q", DType.F16)
-    _rank(q, "q", 3)
-    qh = q.shape[1]
-    _shape(q, "q", (batch, qh, hd))
-    _plain(output, "output", DType.F16)
-    _shape(output, "output", q.shape)
-    _i32_vector(seq_lens, "seq_lens", batch)
+    blocks, kvh, bt, hd = cache = _dims(k_cache, "k_cache", 4)
+    batch, width = tables = _dims(block_tables, "block_tables", 2)
+    qh = _dims(q, "q", 3)[1]
+    rows, scales = (batch, qh, hd), (blocks, kvh)
+    f16, i8, f32, i32 = DType.F16, DType.I8, DType.F32, DType.I32
     _not_aliased(output, "output", q, "q")
-    storage = context.storage
-    ptrs = [storage(t).pointer for t in (q, k_cache, v_cache, k_scales, v_scales, block_tables,
-                                         seq_lens, output)]
+    ptrs = _operands(context, (q, "q", f16, rows), (k_cache, "k_cache", i8, cache),
+                     (v_cache, "v_cache", i8, cache), (k_scales, "k_scales", f32, scales),
+                     (v_scales, "v_scales", f32, scales),
+                     (block_tables, "block_tables", i32, tables),
+                     (seq_lens, "seq_lens", i32, (batch,)), (output, "output", f16, rows))
     if batch == 0 or qh == 0:
         return
     scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
     need = context.decode_q8_workspace_bytes(batch, qh, kvh, hd)
     ws_ptr, ws_bytes = context.decode_q8_workspace(need) if need else (None, 0)
-    context.inner.select()
+    inner = context.inner
+    inner.select()
     st = lib().mote_cuda_gqa_attention_decode_q8(*ptrs, batch, qh, kvh, hd, blocks, bt, width,
-                                                 scale, ws_ptr, ws_bytes, context.inner.stream)
+                                                 scale, ws_ptr, ws_bytes, inner.stream)
     if st:
         errors.check(st, "launch 8-bit GQA decode attention kernel")
 
@@ -939,30 +942,25 @@ def gqa_attention_packed_f16(context: CudaContext, q: Tensor, k: Tensor, v: Tens
     position gets zeros; rows of no sequence keep their values.  Offsets
     int32 [batch + 1]; a sequence with offsets out of range is skipped and
     sets the device status.  ``scale`` defaults to ``1 / sqrt(head_dim)``."""
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _plain(t, name, DType.F16)
-        _rank(t, name, 3)
-    _plain(output, "output", DType.F16)
-    _shape(output, "output", q.shape)
-    tokens, qh, hd = q.shape
-    kv_tokens, kvh, _ = k.shape
-    _shape(k, "k", (kv_tokens, kvh, hd))
-    _shape(v, "v", k.shape)
-    _plain(q_starts, "q_starts", DType.I32)
-    _rank(q_starts, "q_starts", 1)
-    batch = q_starts.shape[0] - 1
+    tokens, qh, hd = rows = _dims(q, "q", 3)
+    kv_tokens, kvh, _ = _dims(k, "k", 3)
+    kv_rows, starts = (kv_tokens, kvh, hd), _dims(q_starts, "q_starts", 1)
+    batch = starts[0] - 1
     if batch < 0:
-        raise errors.ShapeMismatch(tensor="q_starts", expected=(1,), actual=q_starts.shape)
-    _i32_vector(kv_starts, "kv_starts", batch + 1)
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _not_aliased(output, "output", t, name)
-    storage = context.storage
-    ptrs = [storage(t).pointer for t in (q, k, v, q_starts, kv_starts, output)]
+        raise errors.ShapeMismatch(tensor="q_starts", expected=(1,), actual=starts)
+    _not_aliased(output, "output", q, "q")
+    _not_aliased(output, "output", k, "k")
+    _not_aliased(output, "output", v, "v")
+    f16, i32 = DType.F16, DType.I32
+    ptrs = _operands(context, (q, "q", f16, rows), (k, "k", f16, kv_rows), (v, "v", f16, kv_rows),
+                     (q_starts, "q_starts", i32, starts), (kv_starts, "kv_starts", i32, starts),
+                     (output, "output", f16, rows))
     if tokens == 0 or qh == 0 or batch == 0:
         return
     scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
-    context.inner.select()
+    inner = context.inner
+    inner.select()
     st = lib().mote_cuda_gqa_attention_packed_f16(*ptrs, tokens, kv_tokens, batch, qh, kvh, hd,
-                                                  scale, context.inner.stream)
+                                                  scale, inner.stream)
     if st:
         errors.check(st, "launch packed GQA attention kernel")

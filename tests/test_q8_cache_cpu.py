@@ -94,12 +94,12 @@ class _Storage:
 class _Tensor:
     def __init__(self, shape, dtype):
         self.desc = plain(shape, dtype)
-        self._storage = _Storage()
+        self.storage = _Storage()
 
     shape = property(lambda self: self.desc.shape)
 
     def shares_storage_with(self, other):
-        return self._storage is other._storage
+        return self.storage is other.storage
 
 
 def tensors():
