@@ -103,6 +103,14 @@ __device__ __forceinline__ std::uint32_t bytes_to_half2(std::uint32_t w, std::ui
     return hsub2_u32(prmt(w, 0x64646464u, sel), 0x64806480u);
 }
 
+template <int OFF>
+__device__ __forceinline__ uint4 lds128i(std::uint32_t base) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4+%5];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(base), "n"(OFF));
+    return v;
+}
 __device__ __forceinline__ uint4 lds128(std::uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -165,6 +173,30 @@ struct Tile {
     }
 };
 
+// What a lane reads of a tile of 16 positions, as bytes from its start (the
+// rest is immediate: head_dim 128 has the positions 8 further 1024 bytes on).
+template <int HD>
+struct Offsets {
+    std::uint32_t k[2];            // head_dim 128: chunks 2 t, 2 t + 1; 64: positions r, r + 8
+    std::uint32_t v[HD == 128 ? 2 : 4];
+    __device__ __forceinline__ explicit Offsets(std::uint32_t lane) {
+        const std::uint32_t g = lane >> 2, t = lane & 3;
+        const std::uint32_t r0 = Tile<HD>::position(g >> 1, g & 1);
+        if constexpr (HD == 128) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                k[i] = Tile<HD>::at(r0, 2 * t + i);
+                v[i] = Tile<HD>::at(Tile<HD>::position(t, i), g);
+            }
+        } else {
+            k[0] = Tile<HD>::at(r0, t), k[1] = Tile<HD>::at(r0 + 8, t);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[i] = Tile<HD>::at(Tile<HD>::position(t, i & 1) + 8 * (i >> 1), g >> 1) + 8 * (g & 1);
+        }
+    }
+};
+
 // One warp's state over its units of a row: O^T accumulators (dimension
 // HD / 8 * (lane / 4) + 2 i + e of heads 2 (lane % 4), + 1), this lane's part
 // of the sums, the reference maxima and V's reference scale.
@@ -180,29 +212,33 @@ struct State {
 // (-infinity: the tile's block is not there).
 template <int HD>
 __device__ __forceinline__ void attend32(State<HD>& s, const std::uint32_t (&qf)[HD / 8],
-                                         std::uint32_t ktile, std::uint32_t vtile, float f0,
-                                         float f1, float sv0, float sv1, std::int32_t live) {
-    const std::uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+                                         const Offsets<HD>& off, std::uint32_t ktile,
+                                         std::uint32_t vtile, float f0, float f1, float sv0,
+                                         float sv1, std::int32_t live) {
+    const std::uint32_t lane = threadIdx.x & 31, g = lane >> 2;
     const std::uint32_t r0 = Tile<HD>::position(g >> 1, g & 1);
+    const std::uint32_t ka = ktile + off.k[0], kb = ktile + off.k[1];
     float acc[2][4];
+    const auto score = [&](int k, int j, const uint4& a, const uint4& b) {
+        const std::uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[k][i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < HD / 64; ++j) {
-            const std::uint32_t c = HD == 128 ? 2 * t + j : t;
-            const uint4 a = lds128(ktile + k * 16 * HD + Tile<HD>::at(r0, c));
-            const uint4 b = lds128(ktile + k * 16 * HD + Tile<HD>::at(r0 + 8, c));
-            const std::uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const std::uint32_t xa = aw[i] ^ 0x80808080u, xb = bw[i] ^ 0x80808080u;
-                mma_acc(acc[k], bytes_to_half2(xa, 0x4140u), bytes_to_half2(xb, 0x4140u),
-                        bytes_to_half2(xa, 0x4342u), bytes_to_half2(xb, 0x4342u),
-                        qf[(4 * j + i) * 2], qf[(4 * j + i) * 2 + 1]);
-            }
+        for (int i = 0; i < 4; ++i) {
+            const std::uint32_t xa = aw[i] ^ 0x80808080u, xb = bw[i] ^ 0x80808080u;
+            mma_acc(acc[k], bytes_to_half2(xa, 0x4140u), bytes_to_half2(xb, 0x4140u),
+                    bytes_to_half2(xa, 0x4342u), bytes_to_half2(xb, 0x4342u),
+                    qf[(4 * j + i) * 2], qf[(4 * j + i) * 2 + 1]);
         }
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[0][i] = acc[1][i] = 0.f;
+    if constexpr (HD == 128) {
+        const uint4 a0 = lds128i<0>(ka), b0 = lds128i<1024>(ka), a1 = lds128i<2048>(ka), b1 = lds128i<3072>(ka);
+        score(0, 0, a0, b0), score(1, 0, a1, b1);
+        const uint4 c0 = lds128i<0>(kb), d0 = lds128i<1024>(kb), c1 = lds128i<2048>(kb), d1 = lds128i<3072>(kb);
+        score(0, 1, c0, d0), score(1, 1, c1, d1);
+    } else {
+        const uint4 a0 = lds128i<0>(ka), b0 = lds128i<0>(kb), a1 = lds128i<1024>(ka), b1 = lds128i<1024>(kb);
+        score(0, 0, a0, b0), score(1, 0, a1, b1);
     }
     // scores above the reference maxima, +infinity (or NaN) before there is one
     float x[2][4];
@@ -288,16 +324,18 @@ __device__ __forceinline__ void attend32(State<HD>& s, const std::uint32_t (&qf)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         std::uint32_t v[4][W];
+        if constexpr (HD == 128) {
+            const std::uint32_t va = vtile + off.v[0], vb = vtile + off.v[1];
+            const uint4 x0 = k ? lds128i<2048>(va) : lds128i<0>(va), x1 = k ? lds128i<2048>(vb) : lds128i<0>(vb);
+            const uint4 x2 = k ? lds128i<3072>(va) : lds128i<1024>(va), x3 = k ? lds128i<3072>(vb) : lds128i<1024>(vb);
+            const uint4 y[4] = {x0, x1, x2, x3};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const std::uint32_t r = Tile<HD>::position(t, i & 1) + 8 * (i >> 1);
-            const std::uint32_t at = vtile + k * 16 * HD;
-            if constexpr (HD == 128) {
-                const uint4 a = lds128(at + Tile<HD>::at(r, g));
-                v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w;
-            } else {
-                const uint2 a = lds64(at + Tile<HD>::at(r, g >> 1) + 8 * (g & 1));
-                v[i][0] = a.x, v[i][1] = a.y;
+            for (int i = 0; i < 4; ++i) v[i][0] = y[i].x, v[i][1] = y[i].y, v[i][2] = y[i].z, v[i][3] = y[i].w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint2 y = k ? lds64i<1024>(vtile + off.v[i]) : lds64i<0>(vtile + off.v[i]);
+                v[i][0] = y.x, v[i][1] = y.y;
             }
         }
 #pragma unroll
@@ -558,6 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     if (first_of(row) >= last_of(row)) next(row);  // only that row's end falls to this CTA
     if (row.begin < u1) load_q(row);
+    const Offsets<HD> off(lane);
     std::uint32_t stage = 0, parity = 0;
     bool waiting = true;
     while (row.begin < u1) {
@@ -581,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < kSub / 2; ++k) {
                 if (k > 0 && live <= 32 * k) break;
                 const uint4 sc = lds128(scl + stage * 32 + k * 16);
-                attend32<HD>(s, qf, kt + k * 32 * HD, kt + kTile + k * 32 * HD,
+                attend32<HD>(s, qf, off, kt + k * 32 * HD, kt + kTile + k * 32 * HD,
                              __uint_as_float(sc.x) * p.scale_log2, __uint_as_float(sc.z) * p.scale_log2,
                              __uint_as_float(sc.y), __uint_as_float(sc.w), live - 32 * k);
             }
