@@ -20,6 +20,7 @@
 // * warp 9 owns tensor memory; one thread issues S_i = Q_i K^T and
 //   O_i += P_i V (P_i read from tensor memory, over the first half of S_i).
 //   While the softmax of one query tile runs, the products of the other do;
+//   at head_dim 64 a third S buffer keeps the next S ready for each;
 // * warps 0-3 and 4-7 run the softmax of query tiles 0 and 1, one thread per
 //   row: the maximum moves (and O_i is rescaled) only when a score passes it
 //   by more than 8 in log2 units;
@@ -65,8 +66,7 @@ constexpr std::uint32_t kSorted = 256;  // sequences up to which items are sorte
 constexpr int kFlags = 8;  // items whose "V holds something not finite" flags are kept; a
                            // flag is used again when the item 6 before is long written
 
-// TMEM columns: S_i at 128 i, O_i at 256 + 128 i; P_i over the first 64 of S_i.
-constexpr std::uint32_t kColO = 256;
+// TMEM columns: S buffers of 128, then O_0 and O_1; P over the first 64 of its S.
 constexpr std::uint32_t kTmemCols = 512;
 
 struct Params {
@@ -96,13 +96,17 @@ struct Smem {
     static constexpr int kHalf = 128 * 128;           // 128 rows of 64 f16
     static constexpr int kTile = HD / 64 * kHalf;     // a Q, K or V tile
     static constexpr int kKV = HD == 64 ? 4 : 2;      // K and V stages
+    // S buffers: what tensor memory holds beside the two O
+    static constexpr int kS = HD == 64 ? 3 : 2;
+    static constexpr std::uint32_t kColO = 128 * kS;  // O_i at kColO + HD i
+    static_assert(kColO + 2 * HD <= kTmemCols, "tensor memory");
     static constexpr int kQ = 0;                      // [2] query tiles
     static constexpr int kK = kQ + 2 * kTile;
     static constexpr int kV = kK + kKV * kTile;
     static constexpr int kBar = kV + kKV * kTile;
-    // q_full, q_empty, k_full, k_empty, v_full, v_empty, v_clean [kKV], s_full[2],
-    // p_ready[2], p_half[2], o_done[2], epi_done[2], drained, item_full[kItems], item_empty[kItems]
-    static constexpr int kNumBars = 2 + 5 * kKV + 10 + 1 + 2 * kItems;
+    // q_full, q_empty, k_full, k_empty, v_full, v_empty, v_clean [kKV], s_full,
+    // p_half, p_ready, o_done [kS], epi_done[2], drained, item_full, item_empty [kItems]
+    static constexpr int kNumBars = 2 + 5 * kKV + 4 * kS + 2 + 1 + 2 * kItems;
     static constexpr int kTmemSlot = kBar + kNumBars * 8;
     static constexpr int kAbort = kTmemSlot + 4;
     static constexpr int kFlag = kAbort + 4;          // [kFlags][kCleanWarps]
@@ -271,10 +275,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     std::uint64_t* v_empty = v_full + kKV;
     std::uint64_t* v_clean = v_empty + kKV;
     std::uint64_t* s_full = v_clean + kKV;
-    std::uint64_t* p_ready = s_full + 2;
-    std::uint64_t* p_half = p_ready + 2;
-    std::uint64_t* o_done = p_half + 2;
-    std::uint64_t* epi_done = o_done + 2;
+    std::uint64_t* p_half = s_full + L::kS;
+    std::uint64_t* p_ready = p_half + L::kS;
+    std::uint64_t* o_done = p_ready + L::kS;
+    std::uint64_t* epi_done = o_done + L::kS;
     std::uint64_t* drained = epi_done + 2;
     std::uint64_t* item_full = drained + 1;
     std::uint64_t* item_empty = item_full + kItems;
@@ -295,13 +299,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&v_empty[s], 1 + kCleanWarps);  // the last P V, and warps 10 and 11 keep step
             mbar_init(&v_clean[s], kCleanWarps);
         }
-        for (int s = 0; s < 2; ++s) {
+        for (int s = 0; s < L::kS; ++s) {
             mbar_init(&s_full[s], 1);
-            mbar_init(&p_ready[s], 4);
             mbar_init(&p_half[s], 4);
+            mbar_init(&p_ready[s], 4);
             mbar_init(&o_done[s], 1);
-            mbar_init(&epi_done[s], 4);
         }
+        mbar_init(&epi_done[0], 4);
+        mbar_init(&epi_done[1], 4);
         for (int s = 0; s < kItems; ++s) {
             mbar_init(&item_full[s], 1);
             mbar_init(&item_empty[s], 11);  // every warp but the producer
@@ -425,9 +430,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             // uniform registers (moving each to one cost 100 cycles an MMA).
             const std::uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
             std::uint32_t c = 0, n = 0, clean = 0;
-            // per query tile: P V issued, items with any, and whether the last
-            // one's epilogue has yet to be waited for
-            std::uint32_t done[2] = {0, 0}, outs[2] = {0, 0};
+            // per query tile: items with any tiles, and whether the last one's
+            // epilogue has yet to be waited for; and the passes so far
+            std::uint32_t outs[2] = {0, 0}, passed = 0;
             bool unread[2] = {false, false};
             const auto wait = [&](std::uint64_t* bar, std::uint32_t parity) {
                 return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag)) != 0;
@@ -441,9 +446,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const std::uint32_t masked = __reduce_max_sync(0xffffffffu, it.masked);
                 const std::uint32_t tiles = max(n0, n1);
                 if (tiles == 0) continue;
-                // S_m on K tile j of the item, then what its last use frees
-                const auto issue_s = [&](int m, std::uint32_t j) {
-                    const std::uint32_t s = (c + j) % kKV;
+                // The item's passes in order: pass x is tile j of query tile m, tile 0
+                // of both, tile 1 of both, and so on (query tile 1 attends as many
+                // tiles as 0 or more, or none).  Its S is in buffer (passed + x) % kS.
+                const std::uint32_t passes = n0 + n1, both = 2 * min(n0, n1);
+                const auto m_of = [&](std::uint32_t x) { return x < both ? static_cast<int>(x & 1) : n1 > n0; };
+                const auto j_of = [&](std::uint32_t x) { return x < both ? x / 2 : x - both / 2; };
+                const auto wait_k = [&](std::uint32_t j) {
+                    const std::uint32_t t = c + j;
+                    return wait(&k_full[t % kKV], (t / kKV) & 1u);
+                };
+                const auto issue_s = [&](std::uint32_t x) {  // then what its last use frees
+                    const int m = m_of(x);
+                    const std::uint32_t j = j_of(x), s = (c + j) % kKV, buf = (passed + x) % L::kS;
                     const std::uint64_t ad = gemm::smem_desc_sw128(base + L::kQ + m * L::kTile);
                     const std::uint64_t bd = gemm::smem_desc_sw128(base + L::kK + s * L::kTile);
                     const bool last = m == 1 || j >= n1;
@@ -452,76 +467,73 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int k = 0; k < HD / 16; ++k) {
                             constexpr std::uint32_t kStep = 32 >> 4, kNext = L::kHalf >> 4;
                             const std::uint32_t at = k / 4 * kNext + k % 4 * kStep;
-                            umma_f16_ss(tm + 128u * m, ad + at, bd + at, kIdescS, k != 0 ? 1u : 0u);
+                            umma_f16_ss(tm + 128u * buf, ad + at, bd + at, kIdescS, k != 0 ? 1u : 0u);
                         }
-                        gemm::umma_commit(smem_u32(&s_full[m]));
+                        gemm::umma_commit(smem_u32(&s_full[buf]));
                         if (last) gemm::umma_commit(smem_u32(&k_empty[s]));
-                        if (last && j + 1 == tiles) gemm::umma_commit(smem_u32(q_empty));
+                        if (x + 1 == passes) gemm::umma_commit(smem_u32(q_empty));
                     }
                     __syncwarp();
                 };
-                const auto wait_k = [&](std::uint32_t j) {
-                    const std::uint32_t t = c + j;
-                    return wait(&k_full[t % kKV], (t / kKV) & 1u);
-                };
-                ok = wait(q_full, n & 1u) && wait_k(0);
-                if (ok) {
+                ok = wait(q_full, n & 1u);
+                for (std::uint32_t x = 0; ok && x < L::kS && x < passes; ++x) {
+                    ok = wait_k(j_of(x));
                     gemm::tc_fence_after();
-                    if (n0 > 0) issue_s(0, 0);
-                    if (n1 > 0) issue_s(1, 0);
+                    if (ok) issue_s(x);
                 }
-                for (std::uint32_t j = 0; ok && j < tiles; ++j) {
-                    const std::uint32_t t = c + j, s = t % kKV;
-                    // V tile j has landed, and is looked through where rows see it in part
-                    // (its barriers go round with the tiles that are)
-                    ok = wait(&v_full[s], (t / kKV) & 1u);
-                    if (ok && j >= masked) {
-                        ok = wait(&v_clean[clean % kKV], (clean / kKV) & 1u);
-                        ++clean;
-                    }
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        // the last O is read (of both query tiles, so that neither
-                        // softmax group falls behind by more than an item)
-                        if (ok && unread[m] && j == 0) {
-                            ok = wait(&epi_done[m], (outs[m] - 1) & 1u);
-                            unread[m] = false;
-                        }
-                        if (!ok || j >= (m ? n1 : n0)) continue;
-                        ok = wait(&p_half[m], done[m] & 1u);
-                        if (!ok) continue;
-                        gemm::tc_fence_after();
-                        const std::uint64_t vd = v_desc<HD>(base + L::kV + s * L::kTile);
-                        const bool last = m == 1 || j >= n1;
-                        if (elect_one()) {
-#pragma unroll
-                            for (int k = 0; k < kBN / 32; ++k)
-                                gemm::umma_f16_ta(tm + kColO + 128u * m, tm + 128u * m + k * 8,
-                                                  vd + k * (2048 >> 4), kIdescPV, (j | k) != 0 ? 1u : 0u);
-                        }
-                        __syncwarp();
-                        ok = wait(&p_ready[m], done[m] & 1u);
-                        if (!ok) continue;
-                        gemm::tc_fence_after();
-                        if (elect_one()) {
-#pragma unroll
-                            for (int k = kBN / 32; k < kBN / 16; ++k)
-                                gemm::umma_f16_ta(tm + kColO + 128u * m, tm + 128u * m + k * 8,
-                                                  vd + k * (2048 >> 4), kIdescPV, (j | k) != 0 ? 1u : 0u);
-                            gemm::umma_commit(smem_u32(&o_done[m]));
-                            if (last) gemm::umma_commit(smem_u32(&v_empty[s]));
-                        }
-                        __syncwarp();
-                        ++done[m];
-                        if (j == 0) ++outs[m], unread[m] = true;
-                        if (j + 1 < (m ? n1 : n0)) {
-                            ok = wait_k(j + 1);
-                            if (!ok) continue;
-                            gemm::tc_fence_after();
-                            issue_s(m, j + 1);
+                for (std::uint32_t x = 0; ok && x < passes; ++x) {
+                    const int m = m_of(x);
+                    const std::uint32_t j = j_of(x), t = c + j, s = t % kKV;
+                    const std::uint32_t buf = (passed + x) % L::kS, phase = ((passed + x) / L::kS) & 1u;
+                    if (m == 0 || j >= n0) {
+                        // V tile j has landed, and is looked through where rows see it in
+                        // part (its barriers go round with the tiles that are)
+                        ok = wait(&v_full[s], (t / kKV) & 1u);
+                        if (ok && j >= masked) {
+                            ok = wait(&v_clean[clean % kKV], (clean / kKV) & 1u);
+                            ++clean;
                         }
                     }
+                    // the last O is read (of both query tiles, so that neither
+                    // softmax group falls behind by more than an item)
+                    if (x == 0) {
+#pragma unroll
+                        for (int y = 0; y < 2; ++y)
+                            if (ok && unread[y]) {
+                                ok = wait(&epi_done[y], (outs[y] - 1) & 1u);
+                                unread[y] = false;
+                            }
+                    }
+                    if (!ok) break;
+                    const std::uint64_t vd = v_desc<HD>(base + L::kV + s * L::kTile);
+                    const std::uint32_t p_col = tm + 128u * buf, o_col = tm + L::kColO + HD * m;
+                    const bool last = m == 1 || j >= n1;
+                    // P V in halves, the first while the second half of P is computed
+#pragma unroll
+                    for (int half = 0; half < 2 && ok; ++half) {
+                        ok = wait(half ? &p_ready[buf] : &p_half[buf], phase);
+                        gemm::tc_fence_after();
+                        if (ok && elect_one()) {
+#pragma unroll
+                            for (int k = half * kBN / 32; k < (half + 1) * kBN / 32; ++k)
+                                gemm::umma_f16_ta(o_col, p_col + k * 8, vd + k * (2048 >> 4), kIdescPV,
+                                                  (j | k) != 0 ? 1u : 0u);
+                            if (half) {
+                                gemm::umma_commit(smem_u32(&o_done[buf]));
+                                if (last) gemm::umma_commit(smem_u32(&v_empty[s]));
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    if (ok && x + L::kS < passes) {  // into the buffer that this P leaves
+                        ok = wait_k(j_of(x + L::kS));
+                        gemm::tc_fence_after();
+                        if (ok) issue_s(x + L::kS);
+                    }
                 }
+                if (n0 > 0) ++outs[0], unread[0] = true;
+                if (n1 > 0) ++outs[1], unread[1] = true;
+                passed += passes;
                 c += tiles;
                 ++n;
             }
@@ -591,10 +603,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int m = warp / 4;
         const int r = 32 * (warp % 4) + lane;
         const std::uint32_t row_tmem = tmem + (static_cast<std::uint32_t>(32 * (warp % 4)) << 16);
-        const std::uint32_t s_col = row_tmem + 128u * m, o_col = row_tmem + kColO + 128u * m;
+        const std::uint32_t o_col = row_tmem + L::kColO + HD * m;
         const std::uint32_t tok = r / p.group, head = r % p.group;
         const float sc = p.scale_log2;
-        std::uint32_t cnt = 0, n = 0;  // tiles of this query tile, items
+        std::uint32_t passed = 0, n = 0;  // softmax passes and items so far
         bool ok = true;
         for (std::uint32_t i = 0;; ++i) {
             const Item it = item_at(i);
@@ -607,8 +619,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 m * p.tile_tokens + 32u * (warp % 4) / p.group);
             const std::uint32_t tiles = m ? it.n[1] : it.n[0];
             float mx_ref = -INFINITY, l = 0.f;
-            for (std::uint32_t j = 0; j < tiles && ok; ++j, ++cnt) {
-                ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[m], cnt & 1u, abort_flag));
+            // tile j of this query tile is pass number pass_of(j), as the products are
+            // issued; a buffer's barriers count its passes, and none can be two
+            // phases behind, since S is issued on a buffer after its last P V
+            const auto pass_of = [&](std::uint32_t j) {
+                return passed + min(j, it.n[0]) + min(j, it.n[1]) + (m == 1 && j < it.n[0] ? 1u : 0u);
+            };
+            const auto wait_pass = [&](std::uint64_t* bar, std::uint32_t x) {
+                return __all_sync(0xffffffffu, wait_or_abort(bar + x % L::kS, (x / L::kS) & 1u, abort_flag)) != 0;
+            };
+            for (std::uint32_t j = 0; j < tiles && ok; ++j) {
+                const std::uint32_t x = pass_of(j), buf = x % L::kS, s_col = row_tmem + 128u * buf;
+                ok = wait_pass(s_full, x);
                 if (!ok) break;
                 gemm::tc_fence_after();
                 std::uint32_t v[4][32];
@@ -654,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (j > 0) {
                         // the previous P V is complete before O moves
-                        ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[m], (cnt - 1) & 1u, abort_flag));
+                        ok = wait_pass(o_done, pass_of(j - 1));
                         if (!ok) break;
                         gemm::tc_fence_after();
 #pragma unroll
@@ -691,23 +713,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_wait_st();
                         gemm::tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) arrive(&p_half[m]);
+                        if (lane == 0) arrive(&p_half[buf]);
                     }
                     tmem_st16(s_col + 16 * cc, pk);
                 }
                 tmem_wait_st();
                 gemm::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive(&p_ready[m]);
-                float x0, x1, y0, y1;
-                attnp::unpack_f32x2(acc2[0], x0, x1);
-                attnp::unpack_f32x2(acc2[1], y0, y1);
-                l += (x0 + x1) + (y0 + y1);
+                if (lane == 0) arrive(&p_ready[buf]);
+                float l0, l1, l2, l3;
+                attnp::unpack_f32x2(acc2[0], l0, l1);
+                attnp::unpack_f32x2(acc2[1], l2, l3);
+                l += (l0 + l1) + (l2 + l3);
             }
             // O / sum; rows before the first position have no sum and get zeros
             if (it.tiles() > 0) ++n;
-            if (tiles > 0 && ok)
-                ok = __all_sync(0xffffffffu, wait_or_abort(&o_done[m], (cnt - 1) & 1u, abort_flag));
+            if (tiles > 0 && ok) ok = wait_pass(o_done, pass_of(tiles - 1));
+            passed += it.n[0] + it.n[1];
             if (ok) {
                 gemm::tc_fence_after();
                 const bool some = tiles > 0 && limit >= 0;
