@@ -46,6 +46,7 @@ constexpr int kTile = 4096;   // bytes of K (and of V) in a unit: 4096 / head_di
 constexpr int kStages = 2;
 constexpr int kMaxCtas = 512;
 constexpr int kMinUnits = 2 * kWarps;  // rows of up to this many units are not split
+constexpr std::uint32_t kFew = 16;  // sequences up to which a warp finds its share alone (1 us less)
 constexpr int kRowCost = 14;  // what a row's end costs a CTA, in units (3 us of 0.2 us)
 
 struct Params {
@@ -396,107 +397,138 @@ __global__ void __launch_bounds__(kThreads, 1)
         return min(static_cast<std::uint32_t>(max(__ldg(p.seq_lens + b), 0)), cap);
     };
     const auto units = [&](std::uint32_t len) { return (len + kUnit - 1) / kUnit; };
-    const auto warp_sum = [](std::uint32_t x) {
-#pragma unroll
-        for (int d = 16; d > 0; d /= 2) x += __shfl_xor_sync(0xffffffffu, x, d);
-        return x;
-    };
-
-    // ---- the CTA's share (scratch: the flush area) -------------------------
-    volatile std::uint32_t* found = reinterpret_cast<std::uint32_t*>(flush);
-    volatile std::uint32_t* scan = found + 2 * kWarps + 4;
-    // all units, the longest row's, the sequences with any
-    std::uint32_t longest = 0;
-    std::uint32_t total = 0, filled = 0;
-    for (std::uint32_t b = threadIdx.x; b < batch; b += kThreads) {
-        const std::uint32_t n = units(length(b));
-        total += n;
-        filled += n > 0;
-        longest = max(longest, n);
-    }
-    longest = __reduce_max_sync(0xffffffffu, longest);
-    total = warp_sum(total);
-    filled = warp_sum(filled);
-    if (lane == 0) {
-        scan[warp] = longest;
-        found[2 * warp] = total;
-        found[2 * warp + 1] = filled;
-    }
-    __syncthreads();
-    total = 0, filled = 0, longest = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        longest = max(longest, scan[w]);
-        total += found[2 * w];
-        filled += found[2 * w + 1];
-    }
-    total *= rows;
-    filled *= rows;
-    __syncthreads();
-    // sequences without positions
-    for (std::uint32_t b = blockIdx.x; b < batch; b += gridDim.x)
-        if (length(b) == 0)
-            for (std::uint32_t i = threadIdx.x; i < p.q_heads * (HD / 8); i += kThreads)
-                reinterpret_cast<uint4*>(p.out + static_cast<std::uint64_t>(b) * p.q_heads * HD)[i] =
-                    make_uint4(0, 0, 0, 0);
-    if (total == 0) return;
+    // ---- the CTA's share --------------------------------------------------
     // Equal shares of the units, where a row's end counts as kRowCost units
     // more; or, where the rows are few, equal pieces of each row, one to a
-    // CTA, of the smallest size (in steps of 1 / kWarps) that needs no more
-    // CTAs than there are, unless shares are smaller by more than a row's end.
-    const std::uint32_t least = min(longest, static_cast<std::uint32_t>(kMinUnits));
-    std::uint32_t per = max((total + filled * kRowCost + gridDim.x - 1) / gridDim.x, least);
+    // CTA, of the smallest size (in small steps) that needs no more CTAs than
+    // there are, unless shares are smaller by more than a row's end.
+    std::uint32_t longest = 0, total = 0, filled = 0;  // units, sequences with any
+    std::uint32_t per = 0;                             // units of a CTA
     bool pieces = false;
-    if (filled <= gridDim.x) {
-        const std::uint32_t low = max((total + gridDim.x - 1) / gridDim.x, least);
-        const auto size = [&](int w) { return low + (low * w + kWarps - 1) / kWarps; };
-        std::uint32_t need = 0;
-        for (std::uint32_t b = lane; b < batch; b += 32)
-            need += (units(length(b)) + size(warp) - 1) / size(warp);
-        need = warp_sum(need) * rows;
-        if (lane == 0) scan[warp] = need <= gridDim.x;
-        __syncthreads();
-        int w = 0;
-        while (w < kWarps && !scan[w]) ++w;
-        pieces = w < kWarps && size(w) <= per + kRowCost;
-        if (pieces) per = size(w);
-        __syncthreads();
-    }
+    const auto least = [&] { return min(longest, static_cast<std::uint32_t>(kMinUnits)); };
+    const auto share = [&] { return max((total + filled * kRowCost + gridDim.x - 1) / gridDim.x, least()); };
+    const auto size = [&](std::uint32_t i, std::uint32_t steps) {  // pieces from the least on
+        const std::uint32_t low = max((total + gridDim.x - 1) / gridDim.x, least());
+        return low + (low * i + steps - 1) / steps;
+    };
     const auto extent = [&](std::uint32_t n) -> std::uint32_t {  // a row in virtual units
         return pieces ? (n + per - 1) / per * per : n == 0 ? 0 : n + kRowCost;
     };
-
-    // the row of virtual unit u0
-    const std::uint32_t u0 = per * blockIdx.x, u1 = u0 + per;
-    std::uint32_t before = 0;  // extents of the sequences before the chunk
-    if (threadIdx.x == 0) found[1] = 0;
-    for (std::uint32_t base = 0;; base += kThreads) {
-        const std::uint32_t b = base + threadIdx.x;
-        const std::uint32_t n = b < batch ? units(length(b)) : 0u;
-        const std::uint32_t mine = extent(n);
-        std::uint32_t incl = mine;
+    const auto clear_empty = [&] {  // sequences without positions
+        for (std::uint32_t b = blockIdx.x; b < batch; b += gridDim.x)
+            if (length(b) == 0)
+                for (std::uint32_t i = threadIdx.x; i < p.q_heads * (HD / 8); i += kThreads)
+                    reinterpret_cast<uint4*>(p.out + static_cast<std::uint64_t>(b) * p.q_heads * HD)[i] =
+                        make_uint4(0, 0, 0, 0);
+    };
+    const auto scan_up = [&](std::uint32_t x) {  // inclusive, over the warp
 #pragma unroll
         for (int d = 1; d < 32; d *= 2) {
-            const std::uint32_t y = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += y;
+            const std::uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += y;
         }
-        if (lane == 31) found[4 + warp] = incl;
+        return x;
+    };
+    std::uint32_t u0, at_b = 0, at_begin = 0;  // this CTA's first unit, its sequence and that one's
+    if (batch <= kFew) {
+        // every warp for itself, one sequence to a lane
+        const std::uint32_t n = static_cast<std::uint32_t>(lane) < batch ? units(length(lane)) : 0u;
+        longest = __reduce_max_sync(0xffffffffu, n);
+        total = __reduce_add_sync(0xffffffffu, n) * rows;
+        filled = __popc(__ballot_sync(0xffffffffu, n > 0)) * rows;
+        clear_empty();
+        if (total == 0) return;
+        per = share();
+        if (filled <= gridDim.x) {
+            const std::uint32_t mine = size(lane, 32);
+            std::uint32_t need = 0;
+            for (std::uint32_t b = 0; b < batch; ++b)
+                need += (__shfl_sync(0xffffffffu, n, b) + mine - 1) / mine;
+            const unsigned fits = __ballot_sync(0xffffffffu, need * rows <= gridDim.x);
+            const std::uint32_t best = __shfl_sync(0xffffffffu, mine, fits ? __ffs(fits) - 1 : 0);
+            pieces = fits != 0 && best <= per + kRowCost;
+            if (pieces) per = best;
+        }
+        u0 = per * blockIdx.x;
+        const std::uint32_t mine = extent(n), incl = scan_up(mine);
+        const std::uint32_t begin = (incl - mine) * rows;
+        const unsigned here = __ballot_sync(0xffffffffu, n > 0 && begin <= u0 && u0 < incl * rows);
+        if (here == 0) return;  // past the last unit
+        at_b = __ffs(here) - 1;
+        at_begin = __shfl_sync(0xffffffffu, begin, at_b);
+    } else {
+        // the CTA together (scratch: the flush area)
+        volatile std::uint32_t* found = reinterpret_cast<std::uint32_t*>(flush);
+        volatile std::uint32_t* scan = found + 2 * kWarps + 4;
+        for (std::uint32_t b = threadIdx.x; b < batch; b += kThreads) {
+            const std::uint32_t n = units(length(b));
+            total += n;
+            filled += n > 0;
+            longest = max(longest, n);
+        }
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        total = __reduce_add_sync(0xffffffffu, total);
+        filled = __reduce_add_sync(0xffffffffu, filled);
+        if (lane == 0) {
+            scan[warp] = longest;
+            found[2 * warp] = total;
+            found[2 * warp + 1] = filled;
+        }
         __syncthreads();
-        std::uint32_t lower = before;
+        total = 0, filled = 0, longest = 0;
+#pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) lower += found[4 + w];
-            before += found[4 + w];
+            longest = max(longest, scan[w]);
+            total += found[2 * w];
+            filled += found[2 * w + 1];
         }
-        const std::uint32_t end = (lower + incl) * rows, begin = (lower + incl - mine) * rows;
-        if (n > 0 && begin <= u0 && u0 < end) {
-            found[0] = begin;
-            found[1] = 1;
-            found[2] = b;
-        }
+        total *= rows;
+        filled *= rows;
         __syncthreads();
-        if (found[1] || base + kThreads >= batch) break;
+        clear_empty();
+        if (total == 0) return;
+        per = share();
+        if (filled <= gridDim.x) {
+            const std::uint32_t mine = size(warp, kWarps);
+            std::uint32_t need = 0;
+            for (std::uint32_t b = lane; b < batch; b += 32) need += (units(length(b)) + mine - 1) / mine;
+            need = __reduce_add_sync(0xffffffffu, need) * rows;
+            if (lane == 0) scan[warp] = need <= gridDim.x;
+            __syncthreads();
+            int w = 0;
+            while (w < kWarps && !scan[w]) ++w;
+            pieces = w < kWarps && size(w, kWarps) <= per + kRowCost;
+            if (pieces) per = size(w, kWarps);
+            __syncthreads();
+        }
+        u0 = per * blockIdx.x;
+        std::uint32_t before = 0;  // extents of the sequences before the chunk
+        if (threadIdx.x == 0) found[1] = 0;
+        for (std::uint32_t base = 0;; base += kThreads) {
+            const std::uint32_t b = base + threadIdx.x;
+            const std::uint32_t n = b < batch ? units(length(b)) : 0u;
+            const std::uint32_t mine = extent(n), incl = scan_up(mine);
+            if (lane == 31) found[4 + warp] = incl;
+            __syncthreads();
+            std::uint32_t lower = before;
+            for (int w = 0; w < kWarps; ++w) {
+                if (w < warp) lower += found[4 + w];
+                before += found[4 + w];
+            }
+            const std::uint32_t end = (lower + incl) * rows, begin = (lower + incl - mine) * rows;
+            if (n > 0 && begin <= u0 && u0 < end) {
+                found[0] = begin;
+                found[1] = 1;
+                found[2] = b;
+            }
+            __syncthreads();
+            if (found[1] || base + kThreads >= batch) break;
+        }
+        if (!found[1]) return;  // past the last unit
+        at_b = found[2], at_begin = found[0];
+        __syncthreads();  // the scratch is read
     }
-    if (!found[1]) return;  // past the last unit
+    const std::uint32_t u1 = u0 + per;
     const auto next = [&](Row& x) {  // the next row with positions, begin ~0 behind the last
         x.begin += extent(x.n);
         if (++x.r < rows) return;
@@ -518,12 +550,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         return min(u1 - x.begin, x.n);
     };
     Row row;
-    row.b = found[2];
+    row.b = at_b;
     row.len = length(row.b);
     row.n = units(row.len);
-    row.r = (u0 - found[0]) / extent(row.n);
-    row.begin = found[0] + row.r * extent(row.n);
-    __syncthreads();  // the scratch is read
+    row.r = (u0 - at_begin) / extent(row.n);
+    row.begin = at_begin + row.r * extent(row.n);
 
     // ---- the stream: each warp keeps its ring full, across rows -------------
     // the blocks of 32 / kSub units of this warp, from held_unit of sequence

@@ -779,13 +779,14 @@ def _operands(context: CudaContext, *operands) -> list[int]:
     pointers = []
     for tensor, name, dtype, shape in operands:
         desc = tensor.desc
-        if desc.encoding.plain is not dtype or desc.shape != shape:
+        if desc.dense_dtype is not dtype or desc.shape != shape:
             _plain(tensor, name, dtype)
             _rank(tensor, name, len(shape))
             _shape(tensor, name, shape)
+            continue
         storage = tensor.storage
         if (storage.__class__ is CudaStorage and storage.context is inner
-                and tensor.byte_offset == 0 and desc.is_contiguous):
+                and tensor.byte_offset == 0):
             pointers.append(storage.pointer)
     if len(pointers) != len(operands):  # let the context name what is wrong
         return [context.storage(operand[0]).pointer for operand in operands]

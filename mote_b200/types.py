@@ -137,6 +137,11 @@ class TensorDesc:
         return True
 
     @cached_property
+    def dense_dtype(self) -> DType | None:
+        """The dtype of a plain contiguous descriptor, else None."""
+        return self.encoding.plain if self.is_contiguous else None
+
+    @cached_property
     def required_span_bytes(self) -> int:
         """tensor_desc.rs:59-101: plain = span * size; quantized = rows * blocks * bytes."""
         if self.encoding.quantized is not None:
