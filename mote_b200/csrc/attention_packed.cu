@@ -104,9 +104,9 @@ struct Smem {
     static constexpr int kK = kQ + 2 * kTile;
     static constexpr int kV = kK + kKV * kTile;
     static constexpr int kBar = kV + kKV * kTile;
-    // q_full, q_empty, k_full, k_empty, v_full, v_empty, v_clean [kKV], s_full,
-    // p_half, p_ready, o_done [kS], epi_done[2], drained, item_full, item_empty [kItems]
-    static constexpr int kNumBars = 2 + 5 * kKV + 4 * kS + 2 + 1 + 2 * kItems;
+    // q_full, q_empty, k_full, k_empty, v_full, v_empty, v_clean [kKV],
+    // s_full, o_done [2][kS], p_half, p_ready [kS], epi_done[2], drained, item_full, item_empty [kItems]
+    static constexpr int kNumBars = 2 + 5 * kKV + 6 * kS + 2 + 1 + 2 * kItems;
     static constexpr int kTmemSlot = kBar + kNumBars * 8;
     static constexpr int kAbort = kTmemSlot + 4;
     static constexpr int kFlag = kAbort + 4;          // [kFlags][kCleanWarps]
@@ -275,10 +275,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     std::uint64_t* v_empty = v_full + kKV;
     std::uint64_t* v_clean = v_empty + kKV;
     std::uint64_t* s_full = v_clean + kKV;
-    std::uint64_t* p_half = s_full + L::kS;
+    std::uint64_t* p_half = s_full + 2 * L::kS;
     std::uint64_t* p_ready = p_half + L::kS;
     std::uint64_t* o_done = p_ready + L::kS;
-    std::uint64_t* epi_done = o_done + L::kS;
+    std::uint64_t* epi_done = o_done + 2 * L::kS;
     std::uint64_t* drained = epi_done + 2;
     std::uint64_t* item_full = drained + 1;
     std::uint64_t* item_empty = item_full + kItems;
@@ -301,9 +301,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int s = 0; s < L::kS; ++s) {
             mbar_init(&s_full[s], 1);
+            mbar_init(&s_full[L::kS + s], 1);
             mbar_init(&p_half[s], 4);
             mbar_init(&p_ready[s], 4);
             mbar_init(&o_done[s], 1);
+            mbar_init(&o_done[L::kS + s], 1);
         }
         mbar_init(&epi_done[0], 4);
         mbar_init(&epi_done[1], 4);
@@ -469,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const std::uint32_t at = k / 4 * kNext + k % 4 * kStep;
                             umma_f16_ss(tm + 128u * buf, ad + at, bd + at, kIdescS, k != 0 ? 1u : 0u);
                         }
-                        gemm::umma_commit(smem_u32(&s_full[buf]));
+                        gemm::umma_commit(smem_u32(&s_full[m * L::kS + buf]));
                         if (last) gemm::umma_commit(smem_u32(&k_empty[s]));
                         if (x + 1 == passes) gemm::umma_commit(smem_u32(q_empty));
                     }
@@ -519,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 gemm::umma_f16_ta(o_col, p_col + k * 8, vd + k * (2048 >> 4), kIdescPV,
                                                   (j | k) != 0 ? 1u : 0u);
                             if (half) {
-                                gemm::umma_commit(smem_u32(&o_done[buf]));
+                                gemm::umma_commit(smem_u32(&o_done[m * L::kS + buf]));
                                 if (last) gemm::umma_commit(smem_u32(&v_empty[s]));
                             }
                         }
@@ -606,7 +608,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const std::uint32_t o_col = row_tmem + L::kColO + HD * m;
         const std::uint32_t tok = r / p.group, head = r % p.group;
         const float sc = p.scale_log2;
-        std::uint32_t passed = 0, n = 0;  // softmax passes and items so far
+        std::uint32_t passed = 0, n = 0;  // softmax passes (of both query tiles) and items so far
+        std::uint32_t seen = 0;           // parity of this query tile's passes on each S buffer
         bool ok = true;
         for (std::uint32_t i = 0;; ++i) {
             const Item it = item_at(i);
@@ -620,17 +623,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             const std::uint32_t tiles = m ? it.n[1] : it.n[0];
             float mx_ref = -INFINITY, l = 0.f;
             // tile j of this query tile is pass number pass_of(j), as the products are
-            // issued; a buffer's barriers count its passes, and none can be two
-            // phases behind, since S is issued on a buffer after its last P V
+            // issued.  A buffer's S and O barriers are this query tile's own: their
+            // phases count its passes there, so a group that lags behind the other,
+            // or has no rows for some items, does not lose count.
             const auto pass_of = [&](std::uint32_t j) {
                 return passed + min(j, it.n[0]) + min(j, it.n[1]) + (m == 1 && j < it.n[0] ? 1u : 0u);
             };
-            const auto wait_pass = [&](std::uint64_t* bar, std::uint32_t x) {
-                return __all_sync(0xffffffffu, wait_or_abort(bar + x % L::kS, (x / L::kS) & 1u, abort_flag)) != 0;
+            const auto wait_own = [&](std::uint64_t* bar, std::uint32_t b, std::uint32_t parity) {
+                return __all_sync(0xffffffffu, wait_or_abort(bar + m * L::kS + b, parity, abort_flag)) != 0;
             };
+            std::uint32_t last_buf = 0, last_parity = 0;  // the last pass's
             for (std::uint32_t j = 0; j < tiles && ok; ++j) {
                 const std::uint32_t x = pass_of(j), buf = x % L::kS, s_col = row_tmem + 128u * buf;
-                ok = wait_pass(s_full, x);
+                const std::uint32_t parity = seen >> buf & 1u;
+                seen ^= 1u << buf;
+                ok = wait_own(s_full, buf, parity);
                 if (!ok) break;
                 gemm::tc_fence_after();
                 std::uint32_t v[4][32];
@@ -644,9 +651,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (kbase + kBN - 1 > least) {
 #pragma unroll
                     for (int cc = 0; cc < 4; ++cc) {
-                        const std::int32_t seen = limit - (kbase + 32 * cc) + 1;  // of these columns
+                        const std::int32_t cols = limit - (kbase + 32 * cc) + 1;  // attended of these
                         if (least - (kbase + 32 * cc) + 1 >= 32) continue;
-                        const std::uint32_t bits = seen >= 32 ? 0xffffffffu : seen <= 0 ? 0u : (1u << seen) - 1u;
+                        const std::uint32_t bits = cols >= 32 ? 0xffffffffu : cols <= 0 ? 0u : (1u << cols) - 1u;
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
                             if (!(bits >> e & 1u)) v[cc][e] = __float_as_uint(-INFINITY);
@@ -676,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (j > 0) {
                         // the previous P V is complete before O moves
-                        ok = wait_pass(o_done, pass_of(j - 1));
+                        ok = wait_own(o_done, last_buf, last_parity);
                         if (!ok) break;
                         gemm::tc_fence_after();
 #pragma unroll
@@ -725,10 +732,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 attnp::unpack_f32x2(acc2[0], l0, l1);
                 attnp::unpack_f32x2(acc2[1], l2, l3);
                 l += (l0 + l1) + (l2 + l3);
+                last_buf = buf, last_parity = parity;
             }
             // O / sum; rows before the first position have no sum and get zeros
             if (it.tiles() > 0) ++n;
-            if (tiles > 0 && ok) ok = wait_pass(o_done, pass_of(tiles - 1));
+            if (tiles > 0 && ok) ok = wait_own(o_done, last_buf, last_parity);
             passed += it.n[0] + it.n[1];
             if (ok) {
                 gemm::tc_fence_after();
@@ -740,6 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                        it.kvh * p.group + head) * HD;
 #pragma unroll 1
                 for (int cc = 0; cc < HD / 32; ++cc) {
+                    __syncwarp();
                     std::uint32_t o[32];
                     if (tiles > 0) {
                         tmem_ld32_nowait(o_col + 32 * cc, o);

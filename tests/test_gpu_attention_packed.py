@@ -199,3 +199,51 @@ def test_captured_and_replayed_with_other_lengths(ctx):
         check(got, q, k, v, s, s, rows=40)
     del graph
     assert ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("batch,qh,kvh,hd", [(31, 8, 2, 64), (200, 4, 1, 64), (256, 4, 2, 128),
+                                             (257, 2, 2, 64)])
+def test_ragged_batches_with_cached_positions(ctx, batch, qh, kvh, hd):
+    """Batches around the sizes where items are ranked another way: lengths
+    from nothing to hundreds, some over cached positions, some with fewer
+    positions than queries."""
+    r = np.random.default_rng(batch)
+    nq = r.integers(0, 60, batch)
+    nq[r.integers(0, batch, 4)] = 400
+    nk = np.maximum(0, nq + r.integers(-20, 200, batch))
+    qs, ks = starts_of(nq), starts_of(nk)
+    q, k, v = inputs(batch, qs[-1], ks[-1], qh, kvh, hd)
+    check(attend(ctx, q, k, v, qs, ks), q, k, v, qs, ks, rows=12)
+    assert ctx.device_status() == 0
+
+
+def test_through_the_registry(ctx):
+    from mote_b200 import kernel
+
+    s = [0, 40, 100]
+    q, k, v = inputs(12, 100, 100, 4, 2, 64)
+    want = attend(ctx, q, k, v, s, s)
+    runtime = kernel.Runtime()
+    kernel.register_cuda_kernels(runtime.kernels_mut())
+    entry = runtime.resolve(kernel.KernelKey("gqa_attention_packed", DType.F16), ctx.device)
+    t = [f16(ctx, a) for a in (q, k, v)] + [i32(ctx, s), i32(ctx, s), f16(ctx, np.zeros_like(q))]
+    entry.launch(ctx.device, kernel.KernelArgs((*(x.pointer for x in t), 100, 100, 2, 4, 2, 64,
+                                                kernel.f32_bits(0.125), ctx.stream)))
+    got = np.frombuffer(ctx.read_bytes(t[5]), np.float16).reshape(q.shape)
+    assert np.array_equal(got, want)
+
+
+def test_values_of_v_not_finite_before_a_long_prompt_end(ctx):
+    """Infinities in tiles that every row of a later item sees in full, and in
+    the rows behind a prompt whose length is a whole number of tiles."""
+    n, hd = 512, 128
+    q, k, v = inputs(13, n + 9, n + 9, 4, 2, hd)
+    v[n:] = np.nan
+    v[5, 1, 7] = -np.inf
+    got = attend(ctx, q, k, v, [0, n], [0, n])
+    assert (got[5:n, 2:, 7] == -np.inf).all() and np.isfinite(got[:n, :2]).all()
+    assert np.isfinite(got[:5]).all() and (got[n:] == 7).all()
+    ok = np.setdiff1d(np.arange(hd), [7])
+    want, mag = ref.attention(q[:n], k[:n], np.nan_to_num(v[:n].astype(np.float64), neginf=0),
+                              np.arange(n) + 1, ref.default_scale(hd))
+    ref.check_attention(got[:n][..., ok], want[..., ok], mag[..., ok])

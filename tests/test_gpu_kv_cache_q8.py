@@ -420,3 +420,94 @@ def test_two_contexts_at_once(ctx):
         for t in o:
             assert np.array_equal(np.frombuffer(c.ctx.read_bytes(t), np.float16).reshape(q.shape),
                                   want)
+
+
+@pytest.mark.parametrize("batch,kvh,top", [(16, 2, 300), (17, 2, 300), (1000, 1, 40), (400, 2, 90)])
+def test_decode_finds_its_share_of_any_batch(ctx, batch, kvh, top):
+    """Ragged batches around the sizes where the work is dealt another way,
+    empty sequences among them, and one that is much longer."""
+    r = np.random.default_rng(batch)
+    lens = r.integers(0, top, batch)
+    lens[r.integers(0, batch, batch // 5)] = 0
+    lens[batch // 2] = 1500
+    c = Cache(ctx, lens, kvh, 64, 32, seed=batch)
+    total = int(lens.sum())
+    c.append(keys(r, total, kvh, 64), keys(r, total, kvh, 64), lens, starts_of(lens))
+    c.check()
+    c.check_decode(r.normal(0, 1, (batch, 4 * kvh, 64)).astype(np.float16), lens)
+    assert ctx.device_status() == 0
+
+
+def test_graphs_that_share_the_workspace_take_turns(ctx):
+    """Two captured graphs of different shapes and an eager call use one
+    workspace one after another, in any order."""
+    import torch
+
+    r = np.random.default_rng(71)
+    runs = []
+    for hd, lens in ((128, [4000, 100]), (64, [900] * 30), (128, [20000])):
+        c = Cache(ctx, lens, 2, hd, 64, seed=hd + len(lens))
+        total = sum(lens)
+        c.append(keys(r, total, 2, hd), keys(r, total, 2, hd), lens, starts_of(lens))
+        q = r.normal(0, 1, (len(lens), 8, hd)).astype(np.float16)
+        runs.append((c, f16(ctx, q), i32(ctx, lens), f16(ctx, np.zeros_like(q)),
+                     c.check_decode(q, lens)))
+    stream = torch.cuda.ExternalStream(ctx.stream)
+
+    def call(run):
+        c, q, lens, out, _ = run
+        ops.gqa_attention_decode_q8(ctx, q, *c.tensors, lens, out)
+
+    graphs = []
+    for run in runs[:2]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            call(run)
+    for order in ([0, 1, 2], [2, 1, 0], [1, 1, 0, 0, 2]):
+        for t in runs:
+            ctx.upload_numpy(t[3], np.full(t[4].shape, np.nan, np.float16))
+        for i in order:
+            if i < 2:
+                with torch.cuda.stream(stream):
+                    graphs[i].replay()
+            else:
+                call(runs[2])
+        for run in runs:
+            got = np.frombuffer(ctx.read_bytes(run[3]), np.float16).reshape(run[4].shape)
+            assert np.array_equal(got, run[4])
+    del graphs
+    assert ctx.device_status() == 0
+
+
+def test_workspace_and_registry(ctx):
+    """The C entry refuses a missing, small or unaligned workspace; through
+    the kernel registry it takes the same words."""
+    import ctypes
+
+    from mote_b200 import kernel
+    from mote_b200._native import lib
+
+    r = np.random.default_rng(81)
+    c = Cache(ctx, [50, 700], 2, 128, 16, seed=81)
+    c.append(keys(r, 750, 2, 128), keys(r, 750, 2, 128), [50, 700], [0, 50, 750])
+    q = r.normal(0, 1, (2, 8, 128)).astype(np.float16)
+    want = c.check_decode(q, [50, 700])
+    need = ctypes.c_uint64(0)
+    assert lib().mote_cuda_gqa_attention_decode_q8_workspace_bytes(2, 8, 2, 128,
+                                                                   ctypes.byref(need)) == 0
+    ws = ctx.from_bytes(plain((need.value + 16,), DType.U8), np.zeros(need.value + 16, np.uint8))
+    tq, tl, to = f16(ctx, q), i32(ctx, [50, 700]), f16(ctx, np.zeros_like(q))
+    ptrs = [t.pointer for t in (tq, *c.tensors, tl, to)]
+    blocks, kvh, bt, hd = c.host["k"].shape
+    shape = (2, 8, kvh, hd, blocks, bt, c.table.shape[1])
+    scale = ref.default_scale(hd)
+    for pointer, size in ((None, 0), (ws.pointer, need.value - 1), (ws.pointer + 8, need.value)):
+        assert lib().mote_cuda_gqa_attention_decode_q8(*ptrs, *shape, scale, pointer, size,
+                                                       ctx.stream) == 1
+    runtime = kernel.Runtime()
+    kernel.register_cuda_kernels(runtime.kernels_mut())
+    k = runtime.resolve(kernel.KernelKey("gqa_attention_decode_q8", DType.F16), ctx.device)
+    k.launch(ctx.device, kernel.KernelArgs((*ptrs, *shape, kernel.f32_bits(scale), ws.pointer,
+                                            need.value, ctx.stream)))
+    got = np.frombuffer(ctx.read_bytes(to), np.float16).reshape(q.shape)
+    assert np.array_equal(got, want)
