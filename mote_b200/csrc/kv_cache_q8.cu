@@ -127,7 +127,18 @@ __device__ __forceinline__ std::uint32_t round_to_int8(float x, float m) {
     return static_cast<std::uint32_t>(__float_as_int(__fmaf_rn(x, m, 12582912.f))) & 0xffu;
 }
 
-// One CTA for each (work item, head, K or V).
+// Byte `sel & 3` of w (128 + value) as f32, exactly: as the low bits of 2^23 + u,
+// on the integer and FMA pipes (conversions run at a quarter of their rate).
+__device__ __forceinline__ float byte_value(std::uint32_t w, std::uint32_t sel) {
+    return __uint_as_float(prmt(w, 0x4b000000u, sel)) - 8388736.f;
+}
+
+// One CTA for each (work item, head, K or V).  Bound by HBM for large calls:
+// 16 prompts of 40 to 2048 rows (16.2 k rows of 8 x 128, 100 MB) take 21 us,
+// 0.75 of the copy bandwidth; 32 single rows 4 us, a chain of dependent loads
+// (offsets, length, table, rows).  Several heads to a CTA, the next one's rows
+// loading meanwhile, measured slower (58 against 44 us with the read back): it
+// leaves too few CTAs to balance.
 __global__ void __launch_bounds__(kThreads)
     append_kernel(const CacheShape c, const __half* k_new, const __half* v_new,
                   std::int8_t* k_cache, std::int8_t* v_cache, float* k_scales, float* v_scales,
@@ -220,7 +231,10 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // The first n_b = starts[b + 1] - starts[b] cached rows of every sequence in
-// f16 (fl32(q * scale), rounded once more), packed at row starts[b].
+// f16 (fl32(q * scale), rounded once more), packed at row starts[b].  8-byte
+// loads, so that a warp's 16-byte stores are whole lines (16-byte loads and
+// pairs of stores: 45 us): 31 k rows of 8 x 128, 193 MB, 35 us = 0.84 of the
+// copy bandwidth.
 __global__ void __launch_bounds__(kThreads)
     read_kernel(const CacheShape c, const std::int8_t* k_cache, const std::int8_t* v_cache,
                 const float* k_scales, const float* v_scales, const std::int32_t* tables,
@@ -254,9 +268,9 @@ __global__ void __launch_bounds__(kThreads)
             std::uint32_t o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const std::uint32_t y = (e < 2 ? held[k].x : held[k].y) >> (16 * (e & 1));
-                const float a = static_cast<float>(static_cast<std::int8_t>(y)) * scale;
-                const float b = static_cast<float>(static_cast<std::int8_t>(y >> 8)) * scale;
+                const std::uint32_t w = (e < 2 ? held[k].x : held[k].y) ^ 0x80808080u;
+                const float a = byte_value(w, 0x7440u + 2 * (e & 1)) * scale;
+                const float b = byte_value(w, 0x7441u + 2 * (e & 1)) * scale;
                 asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(o[e]) : "f"(b), "f"(a));
             }
             reinterpret_cast<uint4*>(dst + (i / vecs) * row_stride)[i % vecs] =
