@@ -446,7 +446,7 @@ int mote_cuda_gqa_attention_prefill_f16(const void* q, const void* k_cache, cons
  * head_dim 64 or 128; block_tokens a multiple of 16 from 16 to 256; caches and
  * f16 tensors 16-byte aligned, the others 4-byte; batch <= 2^20; null pointers
  * and other shapes -> 1.  A sequence whose offsets or lengths are out of range is skipped,
- * and so is a block whose number is; either sets *error_flag (uint32) to 1
+ * and so is a block whose number is or that lies past its table; either sets *error_flag (uint32) to 1
  * or, without one, bit 1 of the device status.  Caches need no
  * initialisation.  A block that is appended to belongs to one sequence; full
  * blocks may be shared.
@@ -483,8 +483,14 @@ int mote_cuda_kv_cache_read_q8(const void* k_cache, const void* v_cache, const v
  * most max_blocks * block_tokens; a sequence of length 0 gets zeros.  Positions
  * of a block outside [0, num_blocks) count as not there and set bit 1 of the
  * device status.  q_heads % kv_heads == 0, q_heads and batch <= 65535, scale
- * finite.  Workspace: mote_cuda_gqa_attention_decode_q8_workspace_bytes bytes
- * (0: none). */
+ * finite; batch * kv_heads * max_blocks * block_tokens * head_dim * (query
+ * heads to a KV head, in eights) below 2^42.  The work is dealt out on the
+ * device from seq_lens.  Workspace (16-byte aligned, zeroed once before first
+ * use): mote_cuda_gqa_attention_decode_q8_workspace_bytes bytes for the current
+ * device; its first 2 KiB are counters that every call leaves zero, the rest
+ * are partial results.  Calls that share a workspace must not overlap; in
+ * graphs too, where one workspace serves any number of graphs that are
+ * replayed one after another. */
 int mote_cuda_gqa_attention_decode_q8_workspace_bytes(uint64_t batch, uint64_t q_heads,
                                                       uint64_t kv_heads, uint64_t head_dim,
                                                       uint64_t* bytes);
@@ -502,7 +508,9 @@ int mote_cuda_gqa_attention_decode_q8(const void* q, const void* k_cache, const 
  * stands at position n_k - n_q + i:
  *   out[i, h] = softmax_{p <= n_k - n_q + i}(scale * q[i, h] . k[p, h / g]) . v[p, h / g]
  * A query before the first position gets zeros; rows of no sequence keep
- * their values; what k and v hold past a query's position does not reach it.
+ * their values; what k and v hold past a query's position does not reach it
+ * (infinities and NaN either).  Probabilities are rounded to f16 for the second
+ * product, sums are f32.
  * Offsets int32 [batch + 1] on the device, ascending; a sequence whose
  * offsets are out of range is skipped and sets bit 1 of the device status.
  * head_dim 64 or 128, q_heads a multiple of kv_heads and at most 128 times

