@@ -61,10 +61,10 @@ constexpr int kMmaWarp = 9;
 constexpr int kCleanWarps = 2;  // 10 and 11
 constexpr int kThreads = 12 * 32;
 // Register split (setmaxnreg, per warpgroup): launched at 168 a thread;
-// 384 x 168 = 256 x 216 + 128 x 72, and 32 x (216 + 216 + 72) <= 16384.
+// 384 x 168 = 256 x 224 + 128 x 56, and 32 x (224 + 224 + 56) <= 16384.
 constexpr int kLaunchRegs = 168;
-constexpr int kSoftmaxRegs = 216;
-constexpr int kOtherRegs = 72;
+constexpr int kSoftmaxRegs = 224;
+constexpr int kOtherRegs = 56;
 static_assert(kThreads * kLaunchRegs == 256 * kSoftmaxRegs + 128 * kOtherRegs, "register split");
 static_assert(32 * (2 * kSoftmaxRegs + kOtherRegs) <= 16384, "registers of a sub-partition");
 constexpr int kItems = 4;          // items that the producer may be ahead
