@@ -794,6 +794,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     gemm::tc_fence_after();
     if (warp == kMmaWarp) gemm::tmem_dealloc(tmem, kTmemCols);
+    if (*abort_flag) let_copies_land();
 }
 
 // [rows, heads, HD] f16 in boxes of `tokens` rows x `group` heads x 64; rows

@@ -814,6 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncthreads();  // the flush area is free again
     }
+    if (!waiting) let_copies_land();
 }
 
 inline int ctas(int& n) {

@@ -99,6 +99,14 @@ __device__ __forceinline__ bool mbar_wait_bounded(std::uint64_t* bar, std::uint3
     return true;
 }
 
+// After an expired wait: time (about a millisecond) for copies into shared
+// memory that are still in flight to land before the CTA gives it up.
+__device__ __forceinline__ void let_copies_land() {
+    const long long start = clock64();
+    while (clock64() - start < 2000000LL) {
+    }
+}
+
 // ---- bulk copy (TMA engine, untiled, no multicast) -------------------------
 // Copies `bytes` (multiple of 16) from 16-byte aligned global memory to
 // 16-byte aligned shared memory and signals completion on `bar` via
