@@ -51,7 +51,9 @@ class _ContextInner:
         self._lock = threading.Lock()
 
     def select(self) -> None:
-        errors.check(lib().mote_cuda_set_device(self.ordinal), "select device")
+        status = lib().mote_cuda_set_device(self.ordinal)
+        if status:
+            errors.check(status, "select device")
 
     def copy_channel(self) -> tuple[int, int]:
         """The copy stream and the event that orders it after the compute

@@ -32,7 +32,7 @@
 // the one issuing lane issues them.
 // Bound by the chain softmax -> P V -> S of a query tile (3700 cycles for two
 // tiles of 128 x 128 at head_dim 128, where the products take 2048 and the exp2
-// unit as many): 8192 tokens, 32/8 heads, head_dim 128: 557 us = 987 TFLOP/s;
+// unit as many): 8192 tokens, 32/8 heads, head_dim 128: 554 us = 992 TFLOP/s;
 // 12 prompts of 60 to 1000 tokens at head_dim 64: 50 us.
 // Every wait is bounded; an expired wait aborts the CTA, which waits for its
 // issued MMAs (bounded) and frees its tensor memory.  No load uses cluster

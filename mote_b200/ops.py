@@ -777,6 +777,7 @@ def _operands(context: CudaContext, *operands) -> list[int]:
     offset, layout), in one pass: calls of a few microseconds count here."""
     inner = getattr(context, "inner", None)
     pointers = []
+    add = pointers.append
     for tensor, name, dtype, shape in operands:
         desc = tensor.desc
         if desc.dense_dtype is not dtype or desc.shape != shape:
@@ -786,8 +787,8 @@ def _operands(context: CudaContext, *operands) -> list[int]:
             continue
         storage = tensor.storage
         if (storage.__class__ is CudaStorage and storage.context is inner
-                and tensor.byte_offset == 0):
-            pointers.append(storage.pointer)
+                and not tensor.byte_offset):
+            add(storage.pointer)
     if len(pointers) != len(operands):  # let the context name what is wrong
         return [context.storage(operand[0]).pointer for operand in operands]
     return pointers
