@@ -22,18 +22,22 @@
 //   in the order in which a thread's wide shared loads hold them without bank
 //   conflicts (the products do not depend on it); P^T gets from the
 //   accumulator layout to the operand's with movmatrix.
-// * scale * sk multiplies S in f32; sv multiplies P, relative to a power of
-//   two, before P is split into f16 high and low parts (two products, 22
-//   bits).  The running maximum moves only when a score passes it by more
-//   than 8 (log2 units), so a unit costs one vote instead of a reduction.
+// * scale * sk multiplies S in f32; sv multiplies P before it is split into f16
+//   high and low parts (two products).  For each head, O is held in a unit, a
+//   power of two, that keeps the products P * sv at hand within f16's range
+//   whatever the sizes of V and of the weights before; it moves both ways.
+//   The running maximum and the unit move only when a P passes 2^8 or a
+//   product leaves the range, so a step costs one vote instead of reductions.
 // * Rows that lie in several CTAs leave unnormalised parts in the workspace;
 //   the last CTA to finish joins them in order (a counter per row, left at
 //   zero), so results do not depend on timing.
 // Measured at 32 query / 8 KV heads: one sequence of 32768 (head_dim 128, 67 MB)
-// 20.1 us, of which the stream is 11 us (0.94 of the copy bandwidth); 16 x 4096
+// 20.2 us, of which the stream is 11 us (0.94 of the copy bandwidth); 16 x 4096
 // at head_dim 64 20.0 us (issue-bound: dequantizing takes 5 instructions for 4
 // bytes, 817 a warp for 32 positions at head_dim 128); 48 ragged up to 8192
-// at head_dim 128 (404 MB) 82 us, 0.75 of the copy bandwidth.
+// at head_dim 128 (404 MB) 85 us, 0.73 of the copy bandwidth (82 us with one
+// unit for all heads that followed V's scales alone, which lost the small V's
+// bits; the checks themselves measured nothing).
 // Every wait is bounded; one that expires is reported in the device status
 // and the CTA runs on without waiting.
 #include "mote_common.cuh"
@@ -160,6 +164,12 @@ __device__ __forceinline__ void mma_acc(float (&d)[4], std::uint32_t a0, std::ui
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ std::uint64_t mul_f32x2(std::uint64_t a, std::uint64_t b) {
+    std::uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // Where a tile of 16 positions lies in shared memory (the 128-byte swizzle: a
 // 16-byte chunk's place in its 128-byte line is exchanged by the line's number)
 // and which positions a thread's rows and columns of the products stand for.
@@ -205,13 +215,21 @@ struct Offsets {
 
 // One warp's state over its units of a row: O^T accumulators (dimension
 // HD / 8 * (lane / 4) + 2 i + e of heads 2 (lane % 4), + 1), this lane's part
-// of the sums, the reference maxima and V's reference scale.
+// of the sums, the reference maxima and the units in which O is held.
 template <int HD>
 struct State {
     float o[HD / 16][4];
     float m[2], l[2];
-    float wref;  // power of two: P is held times sv * wref; 0 until the first V scale
+    float w[2];  // powers of two: O is held times w
 };
+
+// P * sv * w is split into f16 high and low parts, off by 2^-25 at most (and by
+// 2^-22 of the value above 2^-3).  The largest of a lane's products of a step
+// stays in this range, so that is 2^-19 of the step's largest; a step whose two
+// tiles have scales further apart than kApart (a block of large values beside
+// one of small ones) is taken as two.
+constexpr float kMostProduct = 32768.f, kLeastProduct = 0x1p-6f, kApart = 64.f;
+constexpr int kProductExponent = 6;  // of the largest where a unit is chosen
 
 // 32 positions more, the first `live` of them attended, in two tiles of 16
 // whose scores are S times f0 and f1 and whose V scales are sv0 and sv1
@@ -262,9 +280,35 @@ __device__ __forceinline__ void attend32(State<HD>& s, const std::uint32_t (&qf)
         if (r + 8 >= n1) y[1][2] = y[1][3] = -INFINITY;
     };
     if (tail) mask(x);
-    const float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                            fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-    if (__any_sync(0xffffffffu, top > 8.f)) {
+    // P, its sums, and its products with V's scales (0 where there is no block)
+    const float v0 = tail && sv0 == -INFINITY ? 0.f : sv0, v1 = tail && sv1 == -INFINITY ? 0.f : sv1;
+    float a[2][4], sum[2];
+    const auto weigh = [&] {  // x becomes P (infinity before there is a maximum)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[k][i] = ex2(x[k][i]);
+        const auto pair = [&](int k, int i) { return attnp::pack_f32x2(x[k][i], x[k][i + 1]); };
+        attnp::unpack_f32x2(attnp::add_f32x2(attnp::add_f32x2(pair(0, 0), pair(0, 2)),
+                                             attnp::add_f32x2(pair(1, 0), pair(1, 2))),
+                            sum[0], sum[1]);
+    };
+    const auto scale = [&] {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const float v = k ? v1 : v0;
+                const std::uint64_t unit = mul_f32x2(attnp::pack_f32x2(v, v), attnp::pack_f32x2(s.w[0], s.w[1]));
+                attnp::unpack_f32x2(mul_f32x2(attnp::pack_f32x2(x[k][i], x[k][i + 1]), unit), a[k][i], a[k][i + 1]);
+            }
+    };
+    weigh();
+    scale();
+    const float a0 = fmaxf(attnp::max3f(a[0][0], a[0][2], a[1][0]), a[1][2]);
+    const float a1 = fmaxf(attnp::max3f(a[0][1], a[0][3], a[1][1]), a[1][3]);
+    if (__any_sync(0xffffffffu, fmaxf(sum[0], sum[1]) > 256.f || fmaxf(a0, a1) > kMostProduct ||
+                                    !(fminf(a0, a1) >= kLeastProduct))) {
         float y[2][4];
 #pragma unroll
         for (int k = 0; k < 2; ++k)
@@ -276,10 +320,22 @@ __device__ __forceinline__ void attend32(State<HD>& s, const std::uint32_t (&qf)
             float m = fmaxf(fmaxf(y[0][h], y[0][2 + h]), fmaxf(y[1][h], y[1][2 + h]));
 #pragma unroll
             for (int d = 4; d < 32; d *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            const float here = m;
             m = fmaxf(m, s.m[h]);
-            const float f = s.m[h] == m ? 1.f : ex2(s.m[h] - m);  // 0 from -infinity
+            float f = s.m[h] == m ? 1.f : ex2(s.m[h] - m);  // 0 from -infinity
             s.m[h] = m;
             s.l[h] *= f;
+            // another unit where the step's largest product is not near the middle
+            // of the range.  Up to 2^64, so that O stays finite (V and P below 2^17
+            // and 2^8, 2^31 positions): products that are below the range even
+            // then add less than 2^-60 to outputs that end in f16
+            const float c = ex2(here - m) * fmaxf(v0, v1);
+            if (c > 0.f && !(c * s.w[h] >= 1.f && c * s.w[h] <= 4096.f)) {  // (not where NaN)
+                const int e = kProductExponent + 127 - (__float_as_int(c) >> 23);
+                const float w = __int_as_float((min(max(e, -60), 64) + 127) << 23);
+                f *= w / s.w[h];
+                s.w[h] = w;
+            }
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) s.o[i][h] *= f, s.o[i][2 + h] *= f;
             // a maximum can still be -infinity only where no score is a number
@@ -287,39 +343,19 @@ __device__ __forceinline__ void attend32(State<HD>& s, const std::uint32_t (&qf)
             for (int k = 0; k < 2; ++k) x[k][h] = y[k][h] - m, x[k][2 + h] = y[k][2 + h] - m;
         }
         if (tail) mask(x);
+        weigh();
+        scale();
     }
-    // V's scales relative to the reference: sv * wref in [2^5, 2^6) where the
-    // reference was set, at most 2^7, so P (up to 2^8) times it fits f16 and
-    // keeps 22 bits down to 2^-14 of the row's largest
-    float w0 = sv0 * s.wref, w1 = sv1 * s.wref;
-    if (!(fmaxf(w0, w1) <= 128.f) || s.wref == 0.f || tail) {
-        const float sv = !(sv0 == sv0) || !(sv1 == sv1) ? NAN : fmaxf(fmaxf(sv0, sv1), 0.f);
-        if (sv != 0.f && (s.wref == 0.f || !(sv * s.wref <= 128.f))) {
-            const int e = min(max((__float_as_int(sv) >> 23 & 255) - 127, -100), 100);
-            const float ref = __int_as_float((5 - e + 127) << 23);
-            const float r = s.wref == 0.f ? 1.f : ref / s.wref;
-            s.wref = ref;
-#pragma unroll
-            for (int i = 0; i < HD / 16; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s.o[i][k] *= r;
-        }
-        // P is 0 where there is no block
-        w0 = sv0 == -INFINITY ? 0.f : sv0 * s.wref, w1 = sv1 == -INFINITY ? 0.f : sv1 * s.wref;
-    }
+    s.l[0] += sum[0], s.l[1] += sum[1];
     std::uint32_t hi[2][2], lo[2][2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[k][i] = ex2(x[k][i]);
-        s.l[0] += x[k][0] + x[k][2], s.l[1] += x[k][1] + x[k][3];
-        const float w = k ? w1 : w0;
-#pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const float a = x[k][2 * i] * w, b = x[k][2 * i + 1] * w;
-            hi[k][i] = half2_of(a, b);
-            lo[k][i] = half2_of(a - half_bits_to_float(hi[k][i] & 0xffffu),
-                                b - half_bits_to_float(hi[k][i] >> 16));
+            const float b0 = a[k][2 * i], b1 = a[k][2 * i + 1];
+            hi[k][i] = half2_of(b0, b1);
+            lo[k][i] = half2_of(b0 - half_bits_to_float(hi[k][i] & 0xffffu),
+                                b1 - half_bits_to_float(hi[k][i] >> 16));
             hi[k][i] = transpose8x8(hi[k][i]);
             lo[k][i] = transpose8x8(lo[k][i]);
         }
@@ -644,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < 4; ++k) s.o[i][k] = 0.f;
         s.m[0] = s.m[1] = -INFINITY;
         s.l[0] = s.l[1] = 0.f;
-        s.wref = 0.f;
+        s.w[0] = s.w[1] = 1.f;
 
         for (std::uint32_t v = v0 + warp; v < v1; v += kWarps) {
             if (waiting) waiting = mbar_wait_bounded(&full[stage], parity, &g_device_status);
@@ -656,9 +692,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < kSub / 2; ++k) {
                 if (k > 0 && live <= 32 * k) break;
                 const uint4 sc = lds128(scl + stage * 32 + k * 16);
-                attend32<HD>(s, qf, off, kt + k * 32 * HD, kt + kTile + k * 32 * HD,
-                             __uint_as_float(sc.x) * p.scale_log2, __uint_as_float(sc.z) * p.scale_log2,
-                             __uint_as_float(sc.y), __uint_as_float(sc.w), live - 32 * k);
+                const float sv0 = __uint_as_float(sc.y), sv1 = __uint_as_float(sc.w);
+                bool apart = fmaxf(sv0, sv1) > kApart * fminf(sv0, sv1) && fminf(sv0, sv1) >= 0.f;
+                bool second = false;
+#pragma unroll 1
+                for (;;) {
+                    attend32<HD>(s, qf, off, kt + k * 32 * HD, kt + kTile + k * 32 * HD,
+                                 __uint_as_float(sc.x) * p.scale_log2, __uint_as_float(sc.z) * p.scale_log2,
+                                 second ? -INFINITY : sv0, apart ? -INFINITY : sv1, live - 32 * k);
+                    if (!apart) break;
+                    apart = false, second = true;
+                }
             }
             if (++stage == kStages) stage = 0, parity ^= 1;
         }
@@ -678,7 +722,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             s.l[0] += __shfl_xor_sync(0xffffffffu, s.l[0], d);
             s.l[1] += __shfl_xor_sync(0xffffffffu, s.l[1], d);
         }
-        const float unref = s.wref == 0.f ? 0.f : 1.f / s.wref;
+        const float unit[2] = {1.f / s.w[0], 1.f / s.w[1]};
         float* part = p.parts + static_cast<std::uint64_t>(2 * blockIdx.x + (v0 == 0 ? 1 : 0)) * kPart;
         for (std::uint32_t quad = 0; quad * 4 < heads; ++quad) {
             // [head][pair of dimensions i][g]; the second two heads with i's
@@ -690,7 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
                         *reinterpret_cast<float2*>(mine + e * HD + 16 * (i ^ (t & 1))) =
-                            make_float2(s.o[i][e] * unref, s.o[i][2 + e] * unref);
+                            make_float2(s.o[i][e] * unit[e], s.o[i][2 + e] * unit[e]);
                 if (g == 0)
                     *reinterpret_cast<float4*>(ml + (warp * 4 + 2 * (t & 1)) * 2) =
                         make_float4(s.m[0], s.l[0], s.m[1], s.l[1]);

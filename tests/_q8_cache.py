@@ -67,14 +67,16 @@ def attention(q, k, v, reach, scale):
     return out, mag
 
 
-def check_attention(got, ref, mag):
+def check_attention(got, ref, mag, held=2.0 ** -11, lost=0.0):
     """f16 outputs against 64 bits.  Half a step of the output's own rounding
     (2^-11 of the value, 2^-25 below the normal range), half a step of each
-    probability held in f16 (2^-11 of the weighted mean of |v|), and 2^-13 of
-    it for the f32 steps: scores up to about 30 summed over 128 products are
-    off by at most 128 * 2^-24 * 30 = 2^-12.1 if every step rounds the same
-    way and below 2^-14 as roundings fall, exp2's approximation by 2^-22."""
-    bound = np.abs(ref) * 2.0 ** -11 + mag * (2.0 ** -11 + 2.0 ** -13) + 2.0 ** -25
+    probability held in f16 (2^-11 of the weighted mean of |v|; `held` is 0
+    for an operator that holds them in more), and 2^-13 of it for the f32
+    steps: scores up to about 30 summed over 128 products are off by at most
+    128 * 2^-24 * 30 = 2^-12.1 if every step rounds the same way and below
+    2^-14 as roundings fall, exp2's approximation by 2^-22.  `lost` is what
+    probabilities below the type's range may take from each output."""
+    bound = np.abs(ref) * 2.0 ** -11 + mag * (held + 2.0 ** -13) + 2.0 ** -25 + lost
     off = np.abs(np.asarray(got, np.float64) - ref)
     assert np.isfinite(got).all()
     assert (off <= bound).all(), (off / bound).max()
