@@ -510,7 +510,8 @@ int mote_cuda_gqa_attention_decode_q8(const void* q, const void* k_cache, const 
  * A query before the first position gets zeros; rows of no sequence keep
  * their values; what k and v hold past a query's position does not reach it
  * (infinities and NaN either).  Probabilities are rounded to f16 for the second
- * product, sums are f32.
+ * product: to 11 bits down to 2^-21 of the row's largest, to 2^-32 of it below;
+ * sums are f32.
  * Offsets int32 [batch + 1] on the device, ascending; a sequence whose
  * offsets are out of range is skipped and sets bit 1 of the device status.
  * head_dim 64 or 128, q_heads a multiple of kv_heads and at most 128 times

@@ -23,7 +23,8 @@
 //   at head_dim 64 a third S buffer keeps the next S ready for each;
 // * warps 0-3 and 4-7 run the softmax of query tiles 0 and 1, one thread per
 //   row: the maximum moves (and O_i is rescaled) only when a score passes it
-//   by more than 8 in log2 units;
+//   by more than 8 in log2 units.  P is rounded to f16, the operand's type: a
+//   second product for its low bits would add a third to the tensor work;
 // * warps 10 and 11 look through the V tiles that some row sees in part (the
 //   last of each item) before they are used: 0 times an infinity or NaN of a
 //   masked position would be NaN, so such values are taken out, and the
@@ -68,6 +69,11 @@ constexpr int kOtherRegs = 56;
 static_assert(kThreads * kLaunchRegs == 256 * kSoftmaxRegs + 128 * kOtherRegs, "register split");
 static_assert(32 * (2 * kSoftmaxRegs + kOtherRegs) <= 16384, "registers of a sub-partition");
 constexpr int kItems = 4;          // items that the producer may be ahead
+// P is held as 2^kShift times the probability relative to the reference, which
+// the row's maximum passes by 2^8 at most: up to 2^15 in f16, with its 11 bits
+// down to 2^-21 of the reference and steps of 2^-31 below (without the shift
+// 2^-14 and 2^-24, where a large V of little weight lost its bits).
+constexpr float kShift = 7.f;
 constexpr std::uint32_t kSorted = 256;  // sequences up to which items are sorted
 constexpr int kFlags = 8;  // items whose "V holds something not finite" flags are kept; a
                            // flag is used again when the item 6 before is long written
@@ -676,8 +682,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                  __uint_as_float(v[cc][e + 1]));
                 const float mx = max3f(max3f(mx8[0], mx8[1], mx8[2]), max3f(mx8[3], mx8[4], mx8[5]),
                                        fmaxf(mx8[6], mx8[7]));
-                // the reference moves only when a score passes it by more than 8
-                // (P stays below 2^8); -infinity while the row has seen nothing
+                // the reference moves only when a score passes it by more than 8;
+                // -infinity while the row has seen nothing
                 const float mnew = fmaxf(mx_ref, mx);
                 const bool grow = (mnew - mx_ref) * sc > 8.f;  // false while both are -inf (NaN)
                 if (__any_sync(0xffffffffu, grow)) {
@@ -703,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                const float neg = mx_ref == -INFINITY ? 0.f : -mx_ref * sc;
+                const float neg = mx_ref == -INFINITY ? 0.f : fmaf(-mx_ref, sc, kShift);
                 const std::uint64_t sc2 = attnp::pack_f32x2(sc, sc), neg2 = attnp::pack_f32x2(neg, neg);
                 std::uint64_t acc2[2] = {0, 0};
                 // P of 32 columns at a time; the first P V steps start on the first

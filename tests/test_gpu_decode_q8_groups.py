@@ -65,3 +65,23 @@ def test_ragged_batch_of_split_rows(ctx, hd, qh, kvh):
     (21, 3, 128, 64, [200, 7]), (16, 1, 128, 256, [700]), (40, 2, 128, 32, [77])])
 def test_short_rows(ctx, qh, kvh, hd, bt, lens):
     run(ctx, lens, qh, kvh, hd, bt, seed=hd + qh)
+
+
+@pytest.mark.parametrize("hd,qh,kvh", [(64, 8, 2), (128, 5, 1)])
+@pytest.mark.parametrize("n", [1, 2, 17, 48, 100])
+def test_outputs_are_rounded_once(ctx, hd, qh, kvh, n):
+    """Queries of zeros: every weight is 1 and every f32 step but the scales'
+    products is exact or below 2^-18 of the sum (100 additions of 2^-24, a
+    reciprocal and a product), so an output is the mean of V within half a
+    step of f16 and 2^-17.  The rows of a block share their product, so a
+    product held in 11 bits would be off by up to 2^-12 in all of them."""
+    r = np.random.default_rng(n + hd)
+    c = Cache(ctx, [n], kvh, hd, 16, seed=n)
+    v = r.uniform(0.5, 1.0, (n, kvh, hd)).astype(np.float16)
+    c.append(keys(r, n, kvh, hd), v, [n], [0, n])
+    q = np.zeros((1, qh, hd), np.float16)
+    got = c.decode(q, [n]).astype(np.float64)
+    k, v = (ref.rows(c.host[m], c.scale[m], c.table[0], n) for m in "kv")
+    want, mag = ref.attention(q, k, v, [n], 1.0)
+    half = np.spacing(np.abs(want).astype(np.float16)).astype(np.float64) / 2
+    assert (np.abs(got - want) <= half + mag * 2.0 ** -17).all()
