@@ -74,6 +74,10 @@ constexpr int kItems = 4;          // items that the producer may be ahead
 // down to 2^-21 of the reference and steps of 2^-31 below (without the shift
 // 2^-14 and 2^-24, where a large V of little weight lost its bits).
 constexpr float kShift = 7.f;
+// score * scale - reference * scale is one fma, whose rounded second product
+// leaves up to 2^-25 of it; references beyond this (log2 units) are subtracted
+// from the scores instead, so that the largest of any size weighs 1.
+constexpr float kVast = 65536.f;
 constexpr std::uint32_t kSorted = 256;  // sequences up to which items are sorted
 constexpr int kFlags = 8;  // items whose "V holds something not finite" flags are kept; a
                            // flag is used again when the item 6 before is long written
@@ -634,6 +638,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 m * p.tile_tokens + 32u * (warp % 4) / p.group);
             const std::uint32_t tiles = m ? it.n[1] : it.n[0];
             float mx_ref = -INFINITY, l = 0.f;
+            float neg = 0.f;    // what the scaled scores get added
+            bool vast = false;  // the reference is subtracted from the scores
             // tile j of this query tile is pass number pass_of(j), as the products are
             // issued.  A buffer's S and O barriers are this query tile's own: their
             // phases count its passes there, so a group that lags behind the other,
@@ -686,12 +692,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // -infinity while the row has seen nothing
                 const float mnew = fmaxf(mx_ref, mx);
                 const bool grow = (mnew - mx_ref) * sc > 8.f;  // false while both are -inf (NaN)
-                if (__any_sync(0xffffffffu, grow)) {
+                if (__any_sync(0xffffffffu, grow || vast)) {
                     float alpha = 1.f;
                     if (grow) {
                         alpha = ex2f((mx_ref - mnew) * sc);  // 0 from -infinity
                         mx_ref = mnew;
                         l *= alpha;
+                        vast = fabsf(mx_ref) * sc > kVast;
+                        neg = vast ? kShift : fmaf(-mx_ref, sc, kShift);
+                    }
+                    // (a row's own arithmetic, whatever the others of its warp hold)
+                    if (__any_sync(0xffffffffu, vast)) {
+                        const float from = vast ? mx_ref : 0.f;
+#pragma unroll
+                        for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[cc][e] = __float_as_uint(__uint_as_float(v[cc][e]) - from);
                     }
                     if (j > 0) {
                         // the previous P V is complete before O moves
@@ -709,7 +725,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                const float neg = mx_ref == -INFINITY ? 0.f : fmaf(-mx_ref, sc, kShift);
                 const std::uint64_t sc2 = attnp::pack_f32x2(sc, sc), neg2 = attnp::pack_f32x2(neg, neg);
                 std::uint64_t acc2[2] = {0, 0};
                 // P of 32 columns at a time; the first P V steps start on the first
