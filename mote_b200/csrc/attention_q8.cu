@@ -223,6 +223,12 @@ struct State {
     float w[2];  // powers of two: O is held times w
 };
 
+// A score less the reference is one fma of the unscaled score, whose rounded
+// reference leaves up to 2^-25 of it; beyond this (log2 units) the score is
+// rounded alike before it is subtracted, so that equal scores of any size weigh
+// the same.
+constexpr float kVast = 65536.f;
+
 // P * sv * w is split into f16 high and low parts, off by 2^-25 at most (and by
 // 2^-22 of the value above 2^-3).  The largest of a lane's products of a step
 // stays in this range, so that is 2^-19 of the step's largest; a step whose two
@@ -308,7 +314,8 @@ __device__ __forceinline__ void attend32(State<HD>& s, const std::uint32_t (&qf)
     const float a0 = fmaxf(attnp::max3f(a[0][0], a[0][2], a[1][0]), a[1][2]);
     const float a1 = fmaxf(attnp::max3f(a[0][1], a[0][3], a[1][1]), a[1][3]);
     if (__any_sync(0xffffffffu, fmaxf(sum[0], sum[1]) > 256.f || fmaxf(a0, a1) > kMostProduct ||
-                                    !(fminf(a0, a1) >= kLeastProduct))) {
+                                    !(fminf(a0, a1) >= kLeastProduct) ||
+                                    fmaxf(fabsf(s.m[0]), fabsf(s.m[1])) > kVast)) {
         float y[2][4];
 #pragma unroll
         for (int k = 0; k < 2; ++k)
