@@ -55,8 +55,15 @@ constexpr int kTile = 4096;   // bytes of K (and of V) in a unit: 4096 / head_di
 constexpr int kStages = 2;
 constexpr int kMaxCtas = 512;
 constexpr int kMinUnits = 2 * kWarps;  // rows of up to this many units are not split
-constexpr std::uint32_t kFew = 16;  // sequences up to which a warp finds its share alone (1 us less)
-constexpr int kRowCost = 14;  // what a row's end costs a CTA, in units (3 us of 0.2 us)
+// Sequences up to which every warp finds the CTA's share alone, one sequence to
+// a lane: 4 sequences of 2000 take 12.0 us against 12.9 by the CTA together, 16
+// ragged ones 20.6 against 21.3, 32 36.2 against 37.0.
+constexpr std::uint32_t kFew = 32;
+// What a row's end costs a CTA, in units: 14 against 8 and 20 measured 52.6
+// against 55.3 and 53.7 us (48 ragged sequences up to 8192, head_dim 64), 82.5
+// against 89.6 and 79.0 (the same at 128), 43.3 against 48.4 and 44.3 (100 up to
+// 2000, 64), 42.8 against 45.7 and 43.5 (128 of 100 to 600, 128).
+constexpr int kRowCost = 14;
 
 struct Params {
     const __half* q;

@@ -85,3 +85,17 @@ def test_outputs_are_rounded_once(ctx, hd, qh, kvh, n):
     want, mag = ref.attention(q, k, v, [n], 1.0)
     half = np.spacing(np.abs(want).astype(np.float16)).astype(np.float64) / 2
     assert (np.abs(got - want) <= half + mag * 2.0 ** -17).all()
+
+
+@pytest.mark.parametrize("batch", [31, 32, 33])
+@pytest.mark.parametrize("top", [90, 2500])
+def test_shares_found_by_warps_and_by_the_cta(ctx, batch, top):
+    """Around the number of sequences up to which a warp finds its share alone,
+    with short rows and with split ones, empty sequences at both ends."""
+    r = np.random.default_rng(batch)
+    lens = r.integers(0, top, batch)
+    lens[[0, 5, batch - 1]] = 0
+    lens[batch - 2] = 2 * top
+    run(ctx, lens.tolist(), 4, 2, 64, 32, seed=batch)
+    lens[batch - 1] = 7
+    run(ctx, lens.tolist(), 8, 1, 128, 16, seed=batch)
