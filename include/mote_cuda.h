@@ -445,10 +445,10 @@ int mote_cuda_gqa_attention_prefill_f16(const void* q, const void* k_cache, cons
  *                      row p % block_tokens of block block_tables[b][p / block_tokens]
  * head_dim 64 or 128; block_tokens a multiple of 16 from 16 to 256; caches and
  * f16 tensors 16-byte aligned, the others 4-byte; batch <= 2^20; null pointers
- * and other shapes -> 1.  A sequence whose offsets or lengths are out of range is skipped,
- * and so is a block whose number is or that lies past its table; either sets *error_flag (uint32) to 1
- * or, without one, bit 1 of the device status.  Caches need no
- * initialisation.  A block that is appended to belongs to one sequence; full
+ * and other shapes -> 1.  Append and read skip a sequence whose offsets or
+ * lengths are out of range, and a block whose number is or that lies past its
+ * table; either sets *error_flag (uint32) to 1 or, without one, bit 1 of the
+ * device status.  Caches need no initialisation.  A block that is appended to belongs to one sequence; full
  * blocks may be shared.
  *
  * Append: the rows seq_starts[b] .. seq_starts[b + 1] - 1 of k_new / v_new
@@ -479,12 +479,17 @@ int mote_cuda_kv_cache_read_q8(const void* k_cache, const void* v_cache, const v
                                void* stream);
 /* Decode attention over that cache, one query token per sequence:
  *   out[b, h] = softmax(scale * q[b, h] . K_b[:len_b, h / (q_heads / kv_heads)]) . V_b
- * q / out [batch, q_heads, head_dim] f16; seq_lens int32 [batch], len_b at
- * most max_blocks * block_tokens; a sequence of length 0 gets zeros.  Positions
- * of a block outside [0, num_blocks) count as not there and set bit 1 of the
- * device status.  q_heads % kv_heads == 0, q_heads and batch <= 65535, scale
- * finite; batch * kv_heads * max_blocks * block_tokens * head_dim * (query
- * heads to a KV head, in eights) below 2^42.  The work is dealt out on the
+ * q / out [batch, q_heads, head_dim] f16; seq_lens int32 [batch]; a sequence
+ * of length 0 gets zeros.  A length below 0 counts as 0 and one above the
+ * table's positions as those, unreported (as max_len cuts lengths in
+ * mote_cuda_gqa_attention_decode_f16).  Positions of a block outside
+ * [0, num_blocks) count as not there and set bit 1 of the device status.
+ * q_heads % kv_heads == 0, q_heads and batch <= 65535, scale finite; the work
+ * list, batch * kv_heads * ceil(q_heads / kv_heads / 8) rows times
+ * (max_blocks * block_tokens * head_dim / 4096 + 15), below 2^31; others -> 1.
+ * Weights times V's scales are held to 2^-19 of the largest at hand (32
+ * positions, or 16 of one block where V's scales differ much), whatever the
+ * sizes of V and of the scores; sums are f32.  The work is dealt out on the
  * device from seq_lens.  Workspace (16-byte aligned, zeroed once before first
  * use): mote_cuda_gqa_attention_decode_q8_workspace_bytes bytes for the current
  * device; its first 2 KiB are counters that every call leaves zero, the rest

@@ -905,8 +905,9 @@ def gqa_attention_decode_q8(context: CudaContext, q: Tensor, k_cache: Tensor, v_
     :func:`kv_cache_append_q8` (grouped-query): ``output[b, h] =
     softmax(scale * q[b, h] . K_b[:seq_lens[b], h // g]) . V_b`` with ``g =
     q_heads // kv_heads``; q and output [batch, q_heads, head_dim] f16.  A
-    sequence of length 0 gets zeros; blocks out of range count as not there
-    and set the device status.  ``scale`` defaults to ``1 / sqrt(head_dim)``.
+    sequence of length 0 gets zeros, a length below 0 counts as 0 and one above
+    the table's positions as those (neither is reported); blocks out of range
+    count as not there and set the device status.  ``scale`` defaults to ``1 / sqrt(head_dim)``.
     The parts of long rows meet in a workspace of the context, so calls of
     one context (replays of its captured graphs among them) must not overlap;
     the first call of a head_dim comes before any graph capture."""
