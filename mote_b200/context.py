@@ -289,22 +289,22 @@ class CudaContext:
 
     def decode_q8_workspace_bytes(self, batch: int, q_heads: int, kv_heads: int,
                                   head_dim: int) -> int:
-        """mote_cuda_gqa_attention_decode_q8_workspace_bytes, memoised (it
-        depends only on the shape and this context's device)."""
-        key = (batch, q_heads, kv_heads, head_dim)
+        """mote_cuda_gqa_attention_decode_q8_workspace_bytes of a call that has
+        work, memoised by what it depends on (head_dim and this context's
+        device)."""
         try:
-            return self._q8_need[key]
+            return self._q8_need[head_dim]
         except AttributeError:
             self._q8_need = {}
         except KeyError:
             pass
-        if key not in self._q8_need:
-            out = ctypes.c_uint64(0)
-            self.inner.select()
-            errors.check(lib().mote_cuda_gqa_attention_decode_q8_workspace_bytes(
-                *key, ctypes.byref(out)), "query 8-bit attention workspace")
-            self._q8_need[key] = out.value
-        return self._q8_need[key]
+        out = ctypes.c_uint64(0)
+        self.inner.select()
+        errors.check(lib().mote_cuda_gqa_attention_decode_q8_workspace_bytes(
+            1, 1, 1, head_dim, ctypes.byref(out)), "query 8-bit attention workspace")
+        if out.value:  # 0: a head_dim that the call refuses
+            self._q8_need[head_dim] = out.value
+        return out.value
 
     def decode_q8_workspace(self, nbytes: int) -> tuple[int, int]:
         """A zeroed device workspace of at least ``nbytes`` for the 8-bit

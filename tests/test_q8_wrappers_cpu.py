@@ -1,13 +1,13 @@
 """CPU tests of the 8-bit cache's and the packed attention's wrappers: every
-pair of tensors that must not share storage, and the largest work list of a
-decode call."""
+pair of tensors that must not share storage, the memo of the workspace's size
+and the largest work list of a decode call."""
 from __future__ import annotations
 
 import ctypes
 
 import pytest
 
-from mote_b200 import _native, errors, ops
+from mote_b200 import _native, context, errors, ops
 from mote_b200.types import DType
 from tests.test_q8_cache_cpu import _Context, _Tensor, decode, tensors
 
@@ -37,6 +37,35 @@ def test_cache_outputs_share_no_storage(op, names, pairs):
         t[a].storage = t[b].storage
         with pytest.raises(errors.AliasedStorage):
             op(_Context(), *(t[n] for n in names))
+
+
+def test_workspace_size_is_kept_by_head_dim(monkeypatch):
+    """Not by batch, and a call without work or of another head_dim leaves
+    nothing behind that a later call would take."""
+    asked = []
+
+    class _Lib:
+        @staticmethod
+        def mote_cuda_gqa_attention_decode_q8_workspace_bytes(b, qh, kvh, hd, out):
+            asked.append(hd)
+            found = hd in (64, 128) and b and qh and kvh
+            ctypes.cast(out, ctypes.POINTER(ctypes.c_uint64))[0] = 1000 * hd if found else 0
+            return 0
+
+    monkeypatch.setattr(context, "lib", lambda: _Lib)
+
+    class _Inner:
+        def select(self):
+            pass
+
+    c = context.CudaContext.__new__(context.CudaContext)
+    c.inner = _Inner()
+    assert c.decode_q8_workspace_bytes(0, 0, 0, 64) == 64000
+    assert c.decode_q8_workspace_bytes(1, 8, 2, 96) == 0
+    for batch in range(1, 500):
+        assert c.decode_q8_workspace_bytes(batch, 8 * batch, batch, 128) == 128000
+        assert c.decode_q8_workspace_bytes(batch, 8, 2, 64) == 64000
+    assert asked == [64, 96, 128] and len(c._q8_need) == 2
 
 
 def test_largest_work_list():
