@@ -488,8 +488,9 @@ int mote_cuda_kv_cache_read_q8(const void* k_cache, const void* v_cache, const v
  * list, batch * kv_heads * ceil(q_heads / kv_heads / 8) rows times
  * (max_blocks * block_tokens * head_dim / 4096 + 15), below 2^31; others -> 1.
  * Weights times V's scales are held to 2^-19 of the largest at hand (32
- * positions, or 16 of one block where V's scales differ much), whatever the
- * sizes of V and of the scores; sums are f32.  The work is dealt out on the
+ * positions, or 16 of one block where V's scales differ much), or weights to
+ * 2^-27 of the row's largest where |v| is below 127, whatever the sizes of V and
+ * of the scores were before; sums are f32.  The work is dealt out on the
  * device from seq_lens.  Workspace (16-byte aligned, zeroed once before first
  * use): mote_cuda_gqa_attention_decode_q8_workspace_bytes bytes for the current
  * device; its first 2 KiB are counters that every call leaves zero, the rest

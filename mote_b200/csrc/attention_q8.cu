@@ -4,14 +4,13 @@
 // with K = qk * sk, V = qv * sv (8-bit integers times the scale of their block
 // and head).
 //
-// HBM-bound: K and V of the attended positions are read once; 8 query heads
-// share each read.  Everything else is arranged so that the stream never
-// waits:
-// * The work is cut in units of 4096 / head_dim positions of one (sequence, KV head, up to
-//   8 query heads) "row".  One CTA per
-//   SM takes an equal share of consecutive units, found from the lengths on
-//   the device, so ragged batches balance and the host needs no bound on the
-//   lengths.  The 12 warps of a CTA take a row's units in turn, each through a
+// HBM-bound: K and V of the attended positions are read once for up to 8 query
+// heads of a KV head, which share the read (a larger group reads them once for
+// each eight).  Everything else is arranged so that the stream never waits:
+// * The work is cut in units of 4096 / head_dim positions of one (sequence, KV
+//   head, up to 8 query heads) "row".  One CTA per SM takes an equal share of
+//   consecutive units, found from the lengths on the device, so ragged batches
+//   balance and the host needs no bound on the lengths.  The 12 warps of a CTA take a row's units in turn, each through a
 //   ring of 16 KB that runs ahead across rows; the lane that holds a block's
 //   number issues its TMA loads (128-byte swizzle) and its scales.
 // * The 8-bit values become f16 exactly (the byte as the low bits of
@@ -26,18 +25,20 @@
 //   high and low parts (two products).  For each head, O is held in a unit, a
 //   power of two, that keeps the products P * sv at hand within f16's range
 //   whatever the sizes of V and of the weights before; it moves both ways.
-//   The running maximum and the unit move only when a P passes 2^8 or a
-//   product leaves the range, so a step costs one vote instead of reductions.
+//   The running maximum and the unit move only when a P passes 2^8 or the
+//   products leave the range, so a step costs one vote instead of reductions.
 // * Rows that lie in several CTAs leave unnormalised parts in the workspace;
 //   the last CTA to finish joins them in order (a counter per row, left at
 //   zero), so results do not depend on timing.
 // Measured at 32 query / 8 KV heads: one sequence of 32768 (head_dim 128, 67 MB)
-// 20.2 us, of which the stream is 11 us (0.94 of the copy bandwidth); 16 x 4096
-// at head_dim 64 20.0 us (issue-bound: dequantizing takes 5 instructions for 4
-// bytes, 817 a warp for 32 positions at head_dim 128); 48 ragged up to 8192
-// at head_dim 128 (404 MB) 85 us, 0.73 of the copy bandwidth (82 us with one
-// unit for all heads that followed V's scales alone, which lost the small V's
-// bits; the checks themselves measured nothing).
+// 20.4 us, of which the stream is 11 us (0.94 of the copy bandwidth); 16 x 4096
+// at head_dim 64 20.3 us; 48 ragged up to 8192 at head_dim 128 (404 MB) 84 us,
+// 0.73 of the copy bandwidth (82 us with one unit for all heads that followed
+// V's scales alone, which lost the small V's bits).  head_dim 64 is bound by
+// the dependent steps between the 8-bit values and the products at three warps
+// a scheduler (0.46 issues a cycle, 1048 instructions a warp for 64 positions;
+// stalls on fixed latencies 1.7 an issue, on loads 0.9, on a busy pipe 0.6):
+// dequantizing takes 5 instructions for 4 bytes.
 // Every wait is bounded; one that expires is reported in the device status
 // and the CTA runs on without waiting.
 #include "mote_common.cuh"
@@ -238,10 +239,14 @@ constexpr float kVast = 65536.f;
 
 // P * sv * w is split into f16 high and low parts, off by 2^-25 at most (and by
 // 2^-22 of the value above 2^-3).  The largest of a lane's products of a step
-// stays in this range, so that is 2^-19 of the step's largest; a step whose two
-// tiles have scales further apart than kApart (a block of large values beside
-// one of small ones) is taken as two.
-constexpr float kMostProduct = 32768.f, kLeastProduct = 0x1p-6f, kApart = 64.f;
+// stays in this range, so that is 2^-19 of the step's largest.  Steps of less
+// are left in the unit where V is of ordinary size (scales up to kOrdinary, |v|
+// up to 127) and a weight of 1 makes a product of kLeastOne or more: weights are
+// then off by 2^-27 of the row's largest, and scores that spread widely do not
+// move the unit up and down.  A step whose two tiles have scales further apart
+// than kApart (a block of large values beside one of small ones) is taken as two.
+constexpr float kMostProduct = 32768.f, kLeastProduct = 0x1p-6f, kLeastOne = 4.f;
+constexpr float kOrdinary = 1.f, kApart = 64.f;
 constexpr int kProductExponent = 6;  // of the largest where a unit is chosen
 
 // 32 positions more, the first `live` of them attended, in two tiles of 16
@@ -320,8 +325,11 @@ __device__ __forceinline__ void attend32(State<HD>& s, const std::uint32_t (&qf)
     scale();
     const float a0 = fmaxf(attnp::max3f(a[0][0], a[0][2], a[1][0]), a[1][2]);
     const float a1 = fmaxf(attnp::max3f(a[0][1], a[0][3], a[1][1]), a[1][3]);
+    // ordinary V: fine enough where a weight of 1 is well inside the range
+    const float u = fmaxf(v0, v1) <= kOrdinary ? fminf(v0, v1) * (kLeastProduct / kLeastOne) : 0.f;
+    const float b0 = fmaxf(a0, s.w[0] * u), b1 = fmaxf(a1, s.w[1] * u);
     if (__any_sync(0xffffffffu, fmaxf(sum[0], sum[1]) > 256.f || fmaxf(a0, a1) > kMostProduct ||
-                                    !(fminf(a0, a1) >= kLeastProduct) ||
+                                    !(fminf(b0, b1) >= kLeastProduct) ||
                                     fmaxf(fabsf(s.m[0]), fabsf(s.m[1])) > kVast)) {
         float y[2][4];
 #pragma unroll
@@ -344,7 +352,8 @@ __device__ __forceinline__ void attend32(State<HD>& s, const std::uint32_t (&qf)
             // and 2^8, 2^31 positions): products that are below the range even
             // then add less than 2^-60 to outputs that end in f16
             const float c = ex2(here - m) * fmaxf(v0, v1);
-            if (c > 0.f && !(c * s.w[h] >= 1.f && c * s.w[h] <= 4096.f)) {  // (not where NaN)
+            const bool fine = (c * s.w[h] >= 1.f || s.w[h] * u >= kLeastProduct) && c * s.w[h] <= 4096.f;
+            if (c > 0.f && !fine) {  // (not where NaN)
                 const int e = kProductExponent + 127 - (__float_as_int(c) >> 23);
                 const float w = __int_as_float((min(max(e, -60), 64) + 127) << 23);
                 f *= w / s.w[h];

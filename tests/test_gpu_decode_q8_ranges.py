@@ -55,3 +55,25 @@ def test_v_of_different_sizes(ctx, hd, n, big, small, order):
         check(c, got, q, [n], math.log(2.0))
         assert np.array_equal(got, c.decode(q, [n], math.log(2.0)))
     assert ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("hd,n", [(64, 1536), (128, 3000)])
+@pytest.mark.parametrize("spread", [5.0, 13.0, 40.0])
+@pytest.mark.parametrize("sizes", [(0, 0), (-4, 0), (-14, 7), (5, 12)])
+def test_scores_that_spread_widely(ctx, hd, n, spread, sizes):
+    """Every step's largest weight is another power of two away, with V of
+    ordinary sizes, of sizes that change from block to block, and of scales on
+    both sides of 1.  Scores are one product, below 200 log2 units."""
+    r = np.random.default_rng(n + int(spread))
+    kvh, qh, bt = 2, 8, 16
+    k = r.normal(0, 0.2, (n, kvh, hd))
+    k[:, :, 0] = r.normal(0, spread, (n, kvh))
+    size = 2.0 ** r.uniform(*sizes, -(-n // bt)).repeat(bt)[:n]
+    v = r.uniform(0.5, 1.0, (n, kvh, hd)) * size[:, None, None]
+    q = np.zeros((1, qh, hd))
+    q[0, :, 0] = np.arange(qh) % 4 / 4 + 0.25
+    q = q.astype(np.float16)
+    c = Cache(ctx, [n], kvh, hd, bt, seed=n)
+    c.append(k.astype(np.float16), v.astype(np.float16), [n], [0, n])
+    check(c, c.decode(q, [n], math.log(2.0)), q, [n], math.log(2.0))
+    assert ctx.device_status() == 0
