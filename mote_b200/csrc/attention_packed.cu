@@ -24,7 +24,7 @@
 // * warps 0-3 and 4-7 run the softmax of query tiles 0 and 1, one thread per
 //   row: the maximum moves (and O_i is rescaled) only when a score passes it
 //   by more than 8 in log2 units.  P is rounded to f16, the operand's type: a
-//   second product for its low bits would add a third to the tensor work;
+//   second product for its low bits would add half to the tensor work;
 // * warps 10 and 11 look through the V tiles that some row sees in part (the
 //   last of each item) before they are used: 0 times an infinity or NaN of a
 //   masked position would be NaN, so such values are taken out, and the
@@ -33,8 +33,8 @@
 // the one issuing lane issues them.
 // Bound by the chain softmax -> P V -> S of a query tile (3700 cycles for two
 // tiles of 128 x 128 at head_dim 128, where the products take 2048 and the exp2
-// unit as many): 8192 tokens, 32/8 heads, head_dim 128: 554 us = 992 TFLOP/s;
-// 12 prompts of 60 to 1000 tokens at head_dim 64: 50 us.
+// unit as many): 8192 tokens, 32/8 heads, head_dim 128: 565 us = 974 TFLOP/s;
+// 12 prompts of 60 to 1000 tokens at head_dim 64: 50.5 us.
 // Every wait is bounded; an expired wait aborts the CTA, which waits for its
 // issued MMAs (bounded) and frees its tensor memory.  No load uses cluster
 // multicast.
@@ -78,9 +78,16 @@ constexpr float kShift = 7.f;
 // leaves up to 2^-25 of it; references beyond this (log2 units) are subtracted
 // from the scores instead, so that the largest of any size weighs 1.
 constexpr float kVast = 65536.f;
-constexpr std::uint32_t kSorted = 256;  // sequences up to which items are sorted
-constexpr int kFlags = 8;  // items whose "V holds something not finite" flags are kept; a
-                           // flag is used again when the item 6 before is long written
+// Sequences up to which items are ranked by size: 8 to a lane of the producer
+// warp, in registers.  Ranked against in the order of the sequences: 12 prompts
+// of 60 to 1000 57 against 62 us, 64 of 50 to 100 over 2000 cached 108 against
+// 142, 256 of up to 300 209 against 210 (head_dim 64); 310 against 326 (128).
+constexpr std::uint32_t kSorted = 256;
+// Items whose "V holds something not finite" flags are kept.  A row's thread
+// takes an item from the ring when it is done with the one before, so warps 10
+// and 11 are at most kItems items past the one whose flag a row still reads.
+constexpr int kFlags = 8;
+static_assert(kFlags > kItems, "a flag in use is not written");
 
 // TMEM columns: S buffers of 128, then O_0 and O_1; P over the first 64 of its S.
 constexpr std::uint32_t kTmemCols = 512;

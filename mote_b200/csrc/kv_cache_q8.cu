@@ -20,9 +20,14 @@
 // x has 11 bits, q 8 and inv 24, so both products are rounded once, to the
 // integer itself: fma(x, inv, 1.5 * 2^23) leaves the integer in the low bits
 // of the sum (ties to even).  The result does not depend on the order of
-// anything.  Rows behind the new ones keep their bytes.  A row with an
-// infinity or a NaN makes the block's scale NaN (every row of the block then
-// reads as NaN for this head) until the block is written from its first row.
+// anything.  A block that is written at once is off by half a step of its scale
+// at most, 0.289 rms; rows appended one by one are rounded again whenever the
+// scale grows: normal rows end at 0.36 to 0.38 steps rms (0.84 -> 1.05 % of the
+// rows' rms with 16 tokens to a block, 0.97 -> 1.29 % with 256), rows that grow
+// sevenfold along a block at 0.48 to 0.79.  Rows behind the new ones keep their
+// bytes.  A row with an infinity or a NaN makes the block's scale NaN (every row
+// of the block then reads as NaN for this head) until the block is written from
+// its first row.
 #include "mote_common.cuh"
 
 namespace mote {
