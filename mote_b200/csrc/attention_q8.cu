@@ -40,7 +40,7 @@
 // stalls on fixed latencies 1.7 an issue, on loads 0.9, on a busy pipe 0.6):
 // dequantizing takes 5 instructions for 4 bytes.
 // Every wait is bounded; one that expires is reported in the device status
-// and the CTA runs on without waiting.
+// and the lane runs on without waiting and without further copies.
 #include "mote_common.cuh"
 
 #include <cuda.h>
@@ -708,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (std::uint32_t v = v0 + warp; v < v1; v += kWarps) {
             if (waiting) waiting = mbar_wait_bounded(&full[stage], parity, &g_device_status);
             __syncwarp();  // the unit has landed; the stage before it is read by all lanes
-            issue();
+            if (waiting) issue();  // (a stage whose copies are late gets no more)
             const std::uint32_t kt = ring + stage * 2 * kTile;
             const std::int32_t live = static_cast<std::int32_t>(row.len - v * kUnit);
 #pragma unroll
