@@ -529,6 +529,74 @@ int mote_cuda_gqa_attention_packed_f16(const void* q, const void* k, const void*
                                        uint64_t q_heads, uint64_t kv_heads, uint64_t head_dim,
                                        float scale, void* stream);
 
+/* ---- paged KV cache held in f16 --------------------------------------------
+ * No reference counterpart (KV-cache operations and attention are planned
+ * primitives, docs/roadmap.md:58-60; the reference takes cos/sin tables as
+ * inputs, crates/mote-backend-hip/src/rope.rs:66-82).  The layout of the 8-bit
+ * cache, without scales:
+ *   k_cache, v_cache   f16 [num_blocks, kv_heads, block_tokens, head_dim]
+ *   block_tables       int32 [batch, max_blocks]: position p of sequence b is
+ *                      row p % block_tokens of block block_tables[b][p / block_tokens]
+ * head_dim 64 or 128; block_tokens a multiple of 16 from 16 to 256; caches and
+ * f16 tensors 16-byte aligned, the others 4-byte; batch <= 2^20; null pointers
+ * and other shapes -> 1.  Caches need no initialisation.  A block that is
+ * appended to belongs to one sequence; full blocks may be shared.
+ *
+ * cos/sin tables [tokens, pairs] f32 of positions int32 [axes, tokens] with 1
+ * to 4 axes (time, height, width), pairs = section0 + .. + section3 <= 128 (0
+ * past the axes): angle(t, j) = positions[axis(j)][t] * theta^-e(j).  order 0:
+ * axis a has the next section_a pairs, e(j) = j / pairs; order 1: axis j % axes
+ * while j / axes < its section, axis 0 otherwise, e(j) = j / pairs (sections
+ * that do not find their pairs so -> 1); order 2: the pairs of order 0, e = (the
+ * pair's number within its axis) / section_a.  Angles are taken in 64 bits.
+ * theta finite and at least 1. */
+int mote_cuda_rope_cos_sin_axes_f32(const void* positions, void* cos_out, void* sin_out,
+                                    uint64_t tokens, uint64_t axes, uint32_t section0,
+                                    uint32_t section1, uint32_t section2, uint32_t section3,
+                                    uint32_t order, double theta, void* stream);
+/* Rotation and append: qkv [tokens, q_heads + 2 kv_heads, head_dim] f16 (the
+ * rows of a fused QKV projection).  The q and k heads are rotated as by
+ * mote_cuda_rope_f16 (cos/sin f32 [tokens, pairs], rotary_dim = 2 pairs <=
+ * head_dim, layout 0 = half-split, 1 = interleaved; pairs 0: no rotation, the
+ * tables may be null); q goes to q_out [tokens, q_heads, head_dim], k and v of
+ * the rows seq_starts[b] .. seq_starts[b + 1] - 1 (int32 [batch + 1],
+ * ascending) to the last positions of sequence b, whose length with them is
+ * seq_lens[b] (int32 [batch]).  Rows of no sequence, and those of a sequence
+ * whose offsets or length are out of range, are left out (q too); k and v of a
+ * block outside [0, num_blocks) are.  What is out of range sets *error_flag
+ * (uint32) to 1 or, without one, bit 1 of the device status.  q_heads <= 65535;
+ * q_out must not overlap qkv.  tokens == 0 returns 0. */
+int mote_cuda_rope_kv_cache_append_paged_f16(
+    const void* qkv, const void* cos, const void* sin, void* q_out, void* k_cache, void* v_cache,
+    const void* block_tables, const void* seq_starts, const void* seq_lens, uint64_t tokens,
+    uint64_t batch, uint64_t q_heads, uint64_t kv_heads, uint64_t head_dim, uint64_t pairs,
+    uint64_t num_blocks, uint64_t block_tokens, uint64_t max_blocks, uint32_t layout,
+    void* error_flag, void* stream);
+/* Causal attention of new tokens over that cache: sequence b has the queries
+ * q_starts[b] .. q_starts[b + 1] - 1 of q / out [tokens, q_heads, head_dim] f16
+ * (int32 [batch + 1], ascending), the last of its seq_lens[b] cached positions
+ * (int32 [batch]; their K and V already appended); with n of them, query i
+ * stands at position seq_lens[b] - n + i:
+ *   out[i, h] = softmax_{p <= len - n + i}(scale * q[i, h] . K[p, h / g]) . V[p, h / g]
+ * One token of a running sequence, a few drafted ones and chunks of prompts may
+ * be mixed.  max_new: the most tokens that any sequence has.  A query before the
+ * first position gets zeros; rows of no sequence keep their values; what the
+ * cache holds past a query's position does not reach it (infinities and NaN
+ * either).  A sequence whose offsets or length are out of range, or that has
+ * more than max_new tokens, is skipped; a block outside [0, num_blocks) reads
+ * as zeros; both set bit 1 of the device status.  q_heads a multiple of
+ * kv_heads and at most 128 times it, q_heads <= 65535, scale > 0; tokens == 0
+ * returns 0. */
+int mote_cuda_gqa_attention_paged_f16_workspace_bytes(uint64_t q_heads, uint64_t kv_heads,
+                                                      uint64_t head_dim, uint64_t max_new,
+                                                      uint64_t* bytes);
+int mote_cuda_gqa_attention_paged_f16(
+    const void* q, const void* k_cache, const void* v_cache, const void* block_tables,
+    const void* q_starts, const void* seq_lens, void* out, uint64_t tokens, uint64_t batch,
+    uint64_t q_heads, uint64_t kv_heads, uint64_t head_dim, uint64_t num_blocks,
+    uint64_t block_tokens, uint64_t max_blocks, uint64_t max_new, float scale, void* workspace,
+    uint64_t workspace_bytes, void* stream);
+
 /* ---- multi-GPU exchange for column-sharded linears ----------------------
  * The reference is single-device (crates/mote-backend-hip/src/context.rs:13-80
  * holds one device and one stream); these entry points are new.  Each rank

@@ -102,6 +102,10 @@ unsafe extern "C" {
     pub fn mote_cuda_gqa_attention_decode_q8_workspace_bytes(batch: u64, q_heads: u64, kv_heads: u64, head_dim: u64, bytes: *mut u64) -> i32;
     pub fn mote_cuda_gqa_attention_decode_q8(q: *const c_void, k_cache: *const c_void, v_cache: *const c_void, k_scales: *const c_void, v_scales: *const c_void, block_tables: *const c_void, seq_lens: *const c_void, out: *mut c_void, batch: u64, q_heads: u64, kv_heads: u64, head_dim: u64, num_blocks: u64, block_tokens: u64, max_blocks: u64, scale: f32, workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> i32;
     pub fn mote_cuda_gqa_attention_packed_f16(q: *const c_void, k: *const c_void, v: *const c_void, q_starts: *const c_void, kv_starts: *const c_void, out: *mut c_void, tokens: u64, kv_tokens: u64, batch: u64, q_heads: u64, kv_heads: u64, head_dim: u64, scale: f32, stream: *mut c_void) -> i32;
+    pub fn mote_cuda_rope_cos_sin_axes_f32(positions: *const c_void, cos_out: *mut c_void, sin_out: *mut c_void, tokens: u64, axes: u64, section0: u32, section1: u32, section2: u32, section3: u32, order: u32, theta: f64, stream: *mut c_void) -> i32;
+    pub fn mote_cuda_rope_kv_cache_append_paged_f16(qkv: *const c_void, cos: *const c_void, sin: *const c_void, q_out: *mut c_void, k_cache: *mut c_void, v_cache: *mut c_void, block_tables: *const c_void, seq_starts: *const c_void, seq_lens: *const c_void, tokens: u64, batch: u64, q_heads: u64, kv_heads: u64, head_dim: u64, pairs: u64, num_blocks: u64, block_tokens: u64, max_blocks: u64, layout: u32, error_flag: *mut c_void, stream: *mut c_void) -> i32;
+    pub fn mote_cuda_gqa_attention_paged_f16_workspace_bytes(q_heads: u64, kv_heads: u64, head_dim: u64, max_new: u64, bytes: *mut u64) -> i32;
+    pub fn mote_cuda_gqa_attention_paged_f16(q: *const c_void, k_cache: *const c_void, v_cache: *const c_void, block_tables: *const c_void, q_starts: *const c_void, seq_lens: *const c_void, out: *mut c_void, tokens: u64, batch: u64, q_heads: u64, kv_heads: u64, head_dim: u64, num_blocks: u64, block_tokens: u64, max_blocks: u64, max_new: u64, scale: f32, workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> i32;
     pub fn mote_cuda_comm_unique_id(id_out: *mut c_void) -> i32;
     pub fn mote_cuda_comm_init(comm: *mut *mut c_void, nranks: i32, id: *const c_void, rank: i32) -> i32;
     pub fn mote_cuda_comm_init_timeout(comm: *mut *mut c_void, nranks: i32, id: *const c_void, rank: i32, timeout_ms: u64) -> i32;

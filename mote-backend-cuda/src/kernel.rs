@@ -52,6 +52,9 @@ const KERNELS: &[(&str, DType, &str, usize, Call)] = &[
     ("kv_cache_read_q8", DType::F16, "mote_cuda_kv_cache_read_q8", 17, call_kv_cache_read_q8),
     ("gqa_attention_decode_q8", DType::F16, "mote_cuda_gqa_attention_decode_q8", 19, call_gqa_attention_decode_q8),
     ("gqa_attention_packed", DType::F16, "mote_cuda_gqa_attention_packed_f16", 14, call_gqa_attention_packed_f16),
+    ("rope_cos_sin_axes", DType::F32, "mote_cuda_rope_cos_sin_axes_f32", 12, call_rope_cos_sin_axes_f32),
+    ("rope_kv_cache_append_paged", DType::F16, "mote_cuda_rope_kv_cache_append_paged_f16", 21, call_rope_kv_cache_append_paged_f16),
+    ("gqa_attention_paged", DType::F16, "mote_cuda_gqa_attention_paged_f16", 20, call_gqa_attention_paged_f16),
     ("decoder_stack_q4_0", DType::F16, "mote_cuda_q4_0_decoder_stack_f16", 12, call_q4_0_decoder_stack_f16),
 ];
 
@@ -231,6 +234,18 @@ fn call_gqa_attention_decode_q8(w: &[usize]) -> i32 {
 fn call_gqa_attention_packed_f16(w: &[usize]) -> i32 {
     // SAFETY: the caller's words follow the entry point's argument list.
     unsafe { ffi::mote_cuda_gqa_attention_packed_f16(w[0] as *const c_void, w[1] as *const c_void, w[2] as *const c_void, w[3] as *const c_void, w[4] as *const c_void, w[5] as *mut c_void, w[6] as u64, w[7] as u64, w[8] as u64, w[9] as u64, w[10] as u64, w[11] as u64, f32::from_bits(w[12] as u32), w[13] as *mut c_void) }
+}
+fn call_rope_cos_sin_axes_f32(w: &[usize]) -> i32 {
+    // SAFETY: the caller's words follow the entry point's argument list.
+    unsafe { ffi::mote_cuda_rope_cos_sin_axes_f32(w[0] as *const c_void, w[1] as *mut c_void, w[2] as *mut c_void, w[3] as u64, w[4] as u64, w[5] as u32, w[6] as u32, w[7] as u32, w[8] as u32, w[9] as u32, f64::from_bits(w[10] as u64), w[11] as *mut c_void) }
+}
+fn call_rope_kv_cache_append_paged_f16(w: &[usize]) -> i32 {
+    // SAFETY: the caller's words follow the entry point's argument list.
+    unsafe { ffi::mote_cuda_rope_kv_cache_append_paged_f16(w[0] as *const c_void, w[1] as *const c_void, w[2] as *const c_void, w[3] as *mut c_void, w[4] as *mut c_void, w[5] as *mut c_void, w[6] as *const c_void, w[7] as *const c_void, w[8] as *const c_void, w[9] as u64, w[10] as u64, w[11] as u64, w[12] as u64, w[13] as u64, w[14] as u64, w[15] as u64, w[16] as u64, w[17] as u64, w[18] as u32, w[19] as *mut c_void, w[20] as *mut c_void) }
+}
+fn call_gqa_attention_paged_f16(w: &[usize]) -> i32 {
+    // SAFETY: the caller's words follow the entry point's argument list.
+    unsafe { ffi::mote_cuda_gqa_attention_paged_f16(w[0] as *const c_void, w[1] as *const c_void, w[2] as *const c_void, w[3] as *const c_void, w[4] as *const c_void, w[5] as *const c_void, w[6] as *mut c_void, w[7] as u64, w[8] as u64, w[9] as u64, w[10] as u64, w[11] as u64, w[12] as u64, w[13] as u64, w[14] as u64, w[15] as u64, f32::from_bits(w[16] as u32), w[17] as *mut c_void, w[18] as u64, w[19] as *mut c_void) }
 }
 fn call_q4_0_decoder_stack_f16(w: &[usize]) -> i32 {
     // SAFETY: the caller's words follow the entry point's argument list.

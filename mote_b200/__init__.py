@@ -12,7 +12,8 @@ this package is the host-side mirror of the reference's Rust wrappers:
 
 There is no CPU fallback: without the built library every op raises.
 """
-from .types import DType, Encoding, Layout, QuantFormat, RopeLayout, TensorDesc, plain, quantized
+from .types import (DType, Encoding, Layout, QuantFormat, RopeAxes, RopeLayout, TensorDesc, plain,
+                    quantized)
 
-__all__ = ["DType", "Encoding", "Layout", "QuantFormat", "RopeLayout", "TensorDesc", "plain",
-           "quantized"]
+__all__ = ["DType", "Encoding", "Layout", "QuantFormat", "RopeAxes", "RopeLayout", "TensorDesc",
+           "plain", "quantized"]

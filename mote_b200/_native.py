@@ -102,6 +102,10 @@ SIGNATURES: dict[str, tuple] = {
     "mote_cuda_q4_0_decoder_stack_workspace_bytes": (I, [U64, ctypes.POINTER(U64)]),
     "mote_cuda_q4_0_decoder_stack_f16": (I, [P, U32, P, U64, U64, U64, U64, U64, ctypes.c_float,
                                              P, U64, P]),
+    "mote_cuda_rope_cos_sin_axes_f32": (I, [P, P, P, U64, U64, U32, U32, U32, U32, U32, D, P]),
+    "mote_cuda_rope_kv_cache_append_paged_f16": (I, [P] * 9 + [U64] * 9 + [U32, P, P]),
+    "mote_cuda_gqa_attention_paged_f16_workspace_bytes": (I, [U64] * 4 + [ctypes.POINTER(U64)]),
+    "mote_cuda_gqa_attention_paged_f16": (I, [P] * 7 + [U64] * 9 + [F, P, U64, P]),
     "mote_cuda_comm_unique_id": (I, [P]),
     "mote_cuda_comm_init": (I, [ctypes.POINTER(P), I, P, I]),
     "mote_cuda_comm_init_timeout": (I, [ctypes.POINTER(P), I, P, I, U64]),

@@ -318,6 +318,27 @@ class CudaContext:
             held.append(CudaStorage(self.inner, size, np.zeros(size, np.uint8)))
         return held[-1].pointer, held[-1].size_bytes
 
+    def paged_workspace_bytes(self, q_heads: int, kv_heads: int, head_dim: int,
+                              max_new: int) -> int:
+        """mote_cuda_gqa_attention_paged_f16_workspace_bytes on this context's
+        device."""
+        out = ctypes.c_uint64(0)
+        self.inner.select()
+        errors.check(lib().mote_cuda_gqa_attention_paged_f16_workspace_bytes(
+            q_heads, kv_heads, head_dim, max_new, ctypes.byref(out)),
+            "query paged attention workspace")
+        return out.value
+
+    def paged_workspace(self, nbytes: int) -> tuple[int, int]:
+        """A zeroed device workspace of at least ``nbytes`` for the paged
+        attention; grown and kept as :meth:`decode_q8_workspace`."""
+        held = self.__dict__.setdefault("_paged_workspaces", [])
+        if not held or held[-1].size_bytes < nbytes:
+            self.sync()
+            size = max(int(nbytes), 1 << 20)
+            held.append(CudaStorage(self.inner, size, np.zeros(size, np.uint8)))
+        return held[-1].pointer, held[-1].size_bytes
+
     def read_bytes(self, tensor: Tensor) -> bytes:
         storage = self.storage(tensor)
         return storage.read_bytes()[: tensor.desc.required_span_bytes]

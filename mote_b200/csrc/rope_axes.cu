@@ -1,0 +1,136 @@
+// cos/sin tables of rotary positions with several axes (time, height, width
+// of an image or a video), the f32 [tokens, pairs] tables that every rotation
+// of this library takes:
+//   angle(t, j) = positions[axis(j)][t] * theta^-e(j),   j < pairs
+// order 0, sections: axis a has the next sections[a] pairs, e(j) = j / pairs;
+// order 1, interleaved: axis j % axes while j / axes < sections[j % axes], axis
+//   0 otherwise, e(j) = j / pairs;
+// order 2, own: the pairs of order 0, e = (the pair's number within its axis) /
+//   sections[a], so that every axis has a whole series of frequencies.
+//
+// No reference counterpart (the reference takes such tables as inputs,
+// crates/mote-backend-hip/src/rope.rs:66-82).
+//
+// An angle of a far position needs more than 32 bits before it is reduced to a
+// turn: position * frequency is taken in 64, in quarter turns, the nearest
+// whole number subtracted (exactly), and what is left, at most half a quarter
+// turn, goes to f32 for the sine and cosine.  Results are within 2^-23 of the
+// angle's own up to positions of 2^26 or so (the product is off by 2^-53 of it).
+#include "mote_common.cuh"
+
+#include <cmath>
+
+namespace mote {
+namespace ropeaxes {
+
+constexpr std::uint32_t kMaxAxes = 4;
+constexpr std::uint32_t kMaxPairs = 128;
+constexpr int kThreads = 256;
+
+struct Params {
+    const std::int32_t* positions;  // [axes, tokens]
+    float* cos;
+    float* sin;
+    std::uint64_t tokens;
+    std::uint32_t pairs;
+    double quarters[kMaxPairs];      // quarter turns of a position
+    std::uint8_t axis[kMaxPairs];
+};
+
+__device__ __forceinline__ void angle(std::int32_t position, double quarters, float& c, float& s) {
+    const double q = static_cast<double>(position) * quarters;
+    constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are the integer
+    const double n = q + kWhole;
+    const float r = static_cast<float>(q - (n - kWhole));
+    const int k = __double2loint(n);
+    float sr, cr;
+    sincospif(0.5f * r, &sr, &cr);
+    const float a = k & 1 ? sr : cr, b = k & 1 ? cr : sr;
+    c = (k + 1) & 2 ? -a : a;
+    s = k & 2 ? -b : b;
+}
+
+// A thread keeps VEC neighbouring pairs and goes through tokens.
+template <int VEC>
+__global__ void __launch_bounds__(kThreads) table_kernel(const __grid_constant__ Params p) {
+    pdl_launch_dependents();
+    const std::uint32_t cols = p.pairs / VEC, rows = blockDim.x / cols;
+    const std::uint32_t j = threadIdx.x % cols * VEC, r = threadIdx.x / cols;
+    double quarters[VEC];
+    const std::int32_t* position[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        quarters[e] = p.quarters[j + e];
+        position[e] = p.positions + p.axis[j + e] * p.tokens;
+    }
+    pdl_wait();
+    for (std::uint64_t t = static_cast<std::uint64_t>(blockIdx.x) * rows + r; t < p.tokens;
+         t += static_cast<std::uint64_t>(gridDim.x) * rows) {
+        float c[VEC], s[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) angle(__ldg(position[e] + t), quarters[e], c[e], s[e]);
+        float* const co = p.cos + t * p.pairs + j;
+        float* const so = p.sin + t * p.pairs + j;
+        if constexpr (VEC == 4) {
+            *reinterpret_cast<float4*>(co) = make_float4(c[0], c[1], c[2], c[3]);
+            *reinterpret_cast<float4*>(so) = make_float4(s[0], s[1], s[2], s[3]);
+        } else {
+            *co = c[0];
+            *so = s[0];
+        }
+    }
+}
+
+}  // namespace ropeaxes
+}  // namespace mote
+
+extern "C" int mote_cuda_rope_cos_sin_axes_f32(const void* positions, void* cos_out, void* sin_out,
+                                               uint64_t tokens, uint64_t axes, uint32_t section0,
+                                               uint32_t section1, uint32_t section2,
+                                               uint32_t section3, uint32_t order, double theta,
+                                               void* stream) {
+    using namespace mote;
+    using namespace mote::ropeaxes;
+    if (positions == nullptr || cos_out == nullptr || sin_out == nullptr || stream == nullptr)
+        return kInvalidValue;
+    if (axes == 0 || axes > kMaxAxes || order > 2 || !std::isfinite(theta) || theta < 1.0 ||
+        tokens > 0x7fffffffull || !kvq8::aligned4({positions, cos_out, sin_out}))
+        return kInvalidValue;
+    const std::uint32_t sections[kMaxAxes] = {section0, section1, section2, section3};
+    std::uint64_t pairs = 0;
+    for (std::uint32_t a = 0; a < kMaxAxes; ++a) {
+        if (a >= axes && sections[a] != 0) return kInvalidValue;
+        pairs += sections[a];
+    }
+    if (pairs > kMaxPairs) return kInvalidValue;
+    if (order == 1)  // every axis finds its pairs
+        for (std::uint32_t a = 1; a < axes; ++a)
+            if (sections[a] != 0 && a + axes * (sections[a] - 1ull) >= pairs) return kInvalidValue;
+    if (tokens == 0 || pairs == 0) return kSuccess;
+    Params p{};
+    p.positions = static_cast<const std::int32_t*>(positions);
+    p.cos = static_cast<float*>(cos_out);
+    p.sin = static_cast<float*>(sin_out);
+    p.tokens = tokens;
+    p.pairs = static_cast<std::uint32_t>(pairs);
+    const double log2_theta = std::log2(theta);
+    std::uint32_t axis = 0, first = 0;
+    for (std::uint32_t j = 0; j < pairs; ++j) {
+        while (j - first >= sections[axis]) first += sections[axis++];
+        double e = static_cast<double>(j) / static_cast<double>(pairs);
+        p.axis[j] = static_cast<std::uint8_t>(axis);
+        if (order == 1) {
+            const std::uint32_t a = j % static_cast<std::uint32_t>(axes);
+            p.axis[j] = static_cast<std::uint8_t>(j / axes < sections[a] ? a : 0);
+        } else if (order == 2) {
+            e = static_cast<double>(j - first) / sections[axis];
+        }
+        p.quarters[j] = std::exp2(-e * log2_theta) * 0.63661977236758134308;  // 2 / pi
+    }
+    const bool vec = pairs % 4 == 0 && kvq8::aligned16({cos_out, sin_out});
+    const std::uint32_t cols = p.pairs / (vec ? 4 : 1), rows = kThreads / cols;
+    const std::uint64_t blocks = (tokens + rows - 1) / rows;
+    const dim3 grid(static_cast<unsigned>(blocks < 148 * 8 ? blocks : 148 * 8));
+    return launch_pdl(vec ? table_kernel<4> : table_kernel<1>, grid, dim3(cols * rows),
+                      static_cast<cudaStream_t>(stream), p);
+}

@@ -129,6 +129,9 @@ _ARG_KINDS = {
     "mote_cuda_kv_cache_read_q8": "ppppppppuuuuuuupp",
     "mote_cuda_gqa_attention_decode_q8": "ppppppppuuuuuuufpup",
     "mote_cuda_gqa_attention_packed_f16": "ppppppuuuuuufp",
+    "mote_cuda_rope_cos_sin_axes_f32": "pppuuwwwwwdp",
+    "mote_cuda_rope_kv_cache_append_paged_f16": "pppppppppuuuuuuuuuwpp",
+    "mote_cuda_gqa_attention_paged_f16": "pppppppuuuuuuuuufpup",
     "mote_cuda_q4_0_decoder_stack_f16": "pwpuuuuufpup",
 }
 
@@ -165,6 +168,9 @@ CUDA_KERNELS = {
     ("kv_cache_read_q8", DType.F16): "mote_cuda_kv_cache_read_q8",
     ("gqa_attention_decode_q8", DType.F16): "mote_cuda_gqa_attention_decode_q8",
     ("gqa_attention_packed", DType.F16): "mote_cuda_gqa_attention_packed_f16",
+    ("rope_cos_sin_axes", DType.F32): "mote_cuda_rope_cos_sin_axes_f32",
+    ("rope_kv_cache_append_paged", DType.F16): "mote_cuda_rope_kv_cache_append_paged_f16",
+    ("gqa_attention_paged", DType.F16): "mote_cuda_gqa_attention_paged_f16",
     ("decoder_stack_q4_0", DType.F16): "mote_cuda_q4_0_decoder_stack_f16",
 }
 

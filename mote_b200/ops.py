@@ -22,7 +22,7 @@ import math
 from . import errors
 from ._native import lib
 from .context import CudaContext, CudaStorage, Tensor
-from .types import DType, QuantFormat, RopeLayout, TensorDesc
+from .types import DType, QuantFormat, RopeAxes, RopeLayout, TensorDesc
 
 U32_MAX = 0xFFFFFFFF
 
@@ -595,6 +595,33 @@ def rope_cos_sin_f32(context: CudaContext, positions: Tensor, cos: Tensor, sin: 
                  "launch RoPE table kernel")
 
 
+def rope_cos_sin_axes_f32(context: CudaContext, positions: Tensor, cos: Tensor, sin: Tensor,
+                          sections, theta: float = 10000.0,
+                          order: RopeAxes = RopeAxes.Sections) -> None:
+    """Fills ``cos``/``sin`` [tokens, pairs] for int32 ``positions`` [axes,
+    tokens] with several axes (time, height, width): ``sections[a]`` of the
+    pairs turn with axis ``a``, dealt out as ``order`` says.  Up to four axes
+    and 128 pairs, ``theta`` at least 1.  The tables serve :func:`rope_f16`
+    and :func:`rope_kv_cache_append_paged_f16` (rotary_dim = 2 * pairs)."""
+    axes, tokens = _dims(positions, "positions", 2)
+    sections = tuple(int(n) for n in sections)
+    if len(sections) != axes or axes > 4 or min(sections, default=0) < 0:
+        raise errors.ShapeMismatch(tensor="positions", expected=(len(sections), tokens),
+                                   actual=(axes, tokens))
+    table = (tokens, sum(sections))
+    _not_aliased(cos, "cos", sin, "sin")
+    f32 = DType.F32
+    ptrs = _operands(context, (positions, "positions", DType.I32, (axes, tokens)),
+                     (cos, "cos", f32, table), (sin, "sin", f32, table))
+    inner = context.inner
+    inner.select()
+    st = lib().mote_cuda_rope_cos_sin_axes_f32(*ptrs, tokens, axes,
+                                               *(sections + (0, 0, 0, 0))[:4], order.value,
+                                               theta, inner.stream)
+    if st:
+        errors.check(st, "launch RoPE table kernel")
+
+
 # ---------------------------------------------------------- SwiGLU, gather --
 def swiglu_f16(context: CudaContext, gate: Tensor, up: Tensor, output: Tensor) -> None:
     """``output = silu(gate) * up`` elementwise (f16, f32 math)."""
@@ -970,3 +997,101 @@ def gqa_attention_packed_f16(context: CudaContext, q: Tensor, k: Tensor, v: Tens
                                                   scale, inner.stream)
     if st:
         errors.check(st, "launch packed GQA attention kernel")
+
+
+# ---------------------------------------------- paged KV cache held in f16 --
+def rope_kv_cache_append_paged_f16(context: CudaContext, qkv: Tensor, cos: Tensor, sin: Tensor,
+                                   q_out: Tensor, k_cache: Tensor, v_cache: Tensor,
+                                   block_tables: Tensor, seq_starts: Tensor, seq_lens: Tensor,
+                                   layout: RopeLayout = RopeLayout.HalfSplit,
+                                   check: bool = True) -> None:
+    """Rotates the rows of a fused QKV projection on their way into a paged
+    KV cache held in f16.
+
+    ``qkv`` [tokens, q_heads + 2 * kv_heads, head_dim]; the q and k heads
+    are rotated as by :func:`rope_f16` with ``cos``/``sin`` [tokens, pairs]
+    (rotary_dim = 2 * pairs).  q goes to ``q_out`` [tokens, q_heads,
+    head_dim].  Caches f16 [num_blocks, kv_heads, block_tokens, head_dim],
+    ``block_tables`` int32 [batch, max_blocks]: position ``p`` of sequence
+    ``b`` is row ``p % block_tokens`` of block ``block_tables[b, p //
+    block_tokens]``; the k and v of rows ``seq_starts[b] .. seq_starts[b + 1]
+    - 1`` become the last positions of sequence ``b``, whose length with them
+    is ``seq_lens[b]``.  Rows of no sequence, or of one whose offsets or
+    length are out of range, are left out (q too), as are k and v of a block
+    out of range.  With ``check`` the call synchronizes and raises
+    :class:`errors.IndexOutOfRange` for what is out of range; without it the
+    device status is set."""
+    blocks, kvh, bt, hd = cache = _dims(k_cache, "k_cache", 4)
+    batch, width = tables = _dims(block_tables, "block_tables", 2)
+    tokens, qh, _ = rows = _dims(q_out, "q_out", 3)
+    pairs = _dims(cos, "cos", 2)[1]
+    if 2 * pairs > hd:
+        raise errors.InvalidRotaryDim(rotary_dim=2 * pairs, head_dim=hd)
+    outs = ((q_out, "q_out"), (k_cache, "k_cache"), (v_cache, "v_cache"))
+    for i, (out, name) in enumerate(outs):
+        for other, other_name in outs[:i] + ((qkv, "qkv"),):
+            _not_aliased(out, name, other, other_name)
+    f16, f32, i32 = DType.F16, DType.F32, DType.I32
+    ptrs = _operands(context, (qkv, "qkv", f16, (tokens, qh + 2 * kvh, hd)),
+                     (cos, "cos", f32, (tokens, pairs)), (sin, "sin", f32, (tokens, pairs)),
+                     (q_out, "q_out", f16, (tokens, qh, hd)), (k_cache, "k_cache", f16, cache),
+                     (v_cache, "v_cache", f16, cache), (block_tables, "block_tables", i32, tables),
+                     (seq_starts, "seq_starts", i32, (batch + 1,)),
+                     (seq_lens, "seq_lens", i32, (batch,)))
+    if tokens == 0:
+        return
+    flag = _error_flag(context, "_append_paged_flag") if check else None
+    inner = context.inner
+    inner.select()
+    st = lib().mote_cuda_rope_kv_cache_append_paged_f16(*ptrs, tokens, batch, qh, kvh, hd, pairs,
+                                                        blocks, bt, width, layout.value, flag,
+                                                        inner.stream)
+    if st:
+        errors.check(st, "launch paged KV-cache append kernel")
+    if check:
+        _raise_flagged(context, "_append_paged_flag", blocks)
+
+
+def gqa_attention_paged_f16(context: CudaContext, q: Tensor, k_cache: Tensor, v_cache: Tensor,
+                            block_tables: Tensor, q_starts: Tensor, seq_lens: Tensor,
+                            output: Tensor, max_new: int, scale: float | None = None) -> None:
+    """Causal attention of new tokens over the paged cache of
+    :func:`rope_kv_cache_append_paged_f16` (grouped-query): sequence ``b``
+    has rows ``q_starts[b] .. q_starts[b + 1] - 1`` of ``q``/``output``
+    [tokens, q_heads, head_dim] f16, the last of its ``seq_lens[b]`` cached
+    positions (their K and V already appended).  One token of a running
+    sequence, a few drafted ones and chunks of prompts may be mixed;
+    ``max_new`` is the most that any sequence has.  A query before the first
+    position gets zeros; rows of no sequence keep their values.  A sequence
+    whose offsets or length are out of range, or with more than ``max_new``
+    tokens, is skipped, and a block out of range reads as zeros; both set the
+    device status.  ``scale`` defaults to ``1 / sqrt(head_dim)``.  The parts
+    of long rows meet in a workspace of the context, so calls of one context
+    (replays of its captured graphs among them) must not overlap; the first
+    call that needs a larger workspace comes before any graph capture."""
+    blocks, kvh, bt, hd = cache = _dims(k_cache, "k_cache", 4)
+    batch, width = tables = _dims(block_tables, "block_tables", 2)
+    tokens, qh, _ = _dims(q, "q", 3)
+    rows = (tokens, qh, hd)
+    if max_new < 0:
+        raise errors.ShapeMismatch(tensor="q", expected=(max_new, qh, hd), actual=rows)
+    _not_aliased(output, "output", q, "q")
+    _not_aliased(output, "output", k_cache, "k_cache")
+    _not_aliased(output, "output", v_cache, "v_cache")
+    f16, i32 = DType.F16, DType.I32
+    ptrs = _operands(context, (q, "q", f16, rows), (k_cache, "k_cache", f16, cache),
+                     (v_cache, "v_cache", f16, cache), (block_tables, "block_tables", i32, tables),
+                     (q_starts, "q_starts", i32, (batch + 1,)),
+                     (seq_lens, "seq_lens", i32, (batch,)), (output, "output", f16, rows))
+    if tokens == 0 or qh == 0 or batch == 0:
+        return
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    need = context.paged_workspace_bytes(qh, kvh, hd, max_new)
+    ws_ptr, ws_bytes = context.paged_workspace(need) if need else (None, 0)
+    inner = context.inner
+    inner.select()
+    st = lib().mote_cuda_gqa_attention_paged_f16(*ptrs, tokens, batch, qh, kvh, hd, blocks, bt,
+                                                 width, max_new, scale, ws_ptr, ws_bytes,
+                                                 inner.stream)
+    if st:
+        errors.check(st, "launch paged GQA attention kernel")

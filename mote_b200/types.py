@@ -79,6 +79,15 @@ class RopeLayout(enum.Enum):
     Interleaved = 1
 
 
+class RopeAxes(enum.Enum):
+    """How rotary pairs are dealt to the axes of a position; values are the
+    ABI selectors (no reference counterpart)."""
+
+    Sections = 0     # the next sections[a] pairs to axis a, one series of frequencies
+    Interleaved = 1  # pair j to axis j % axes while that axis has pairs left, else to axis 0
+    Own = 2          # as Sections, with a whole series of frequencies for each axis
+
+
 class TensorDescError(ValueError):
     pass
 
