@@ -142,14 +142,14 @@ constexpr float kMostSum = 32768.f;
 // subtracted, so that equal scores of any size weigh the same.
 constexpr float kVast = 1024.f;
 
-// One unit more.  `limit` holds how many of the unit's positions each of the
+// One unit more, for SETS of the MOST sets.  `limit` holds how many of the unit's positions each of the
 // lane's columns attends, where `masked` (some column does not attend all); `live`
 // how many there are.  Returns whether V held something that is not finite.
-template <int HD, int SETS>
-__device__ __forceinline__ bool attend(State<HD, SETS>& s, const std::uint32_t (&qf)[HD / 16][SETS][2],
-                                       std::uint32_t sets, std::uint32_t stage, std::uint32_t koff,
+template <int HD, int SETS, int MOST>
+__device__ __forceinline__ bool attend(State<HD, MOST>& s, const std::uint32_t (&qf)[HD / 16][MOST][2],
+                                       std::uint32_t stage, std::uint32_t koff,
                                        std::uint32_t voff, float sc, bool masked, std::int32_t live,
-                                       const std::int32_t (&limit)[SETS][2]) {
+                                       const std::int32_t (&limit)[MOST][2]) {
     constexpr int T = 128 / HD;  // tiles of 16 positions
     const std::uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     float x[T][SETS][4];
@@ -166,7 +166,7 @@ __device__ __forceinline__ bool attend(State<HD, SETS>& s, const std::uint32_t (
             ldsm_x4(stage + (HD == 128 ? d / 4 : k) * kBox + (koff ^ (d % 4 << 5)), a);
 #pragma unroll
             for (int c = 0; c < SETS; ++c)
-                if (c == 0 || c < sets) attn8::mma_acc(x[k][c], a[0], a[1], a[2], a[3], qf[d][c][0], qf[d][c][1]);
+                attn8::mma_acc(x[k][c], a[0], a[1], a[2], a[3], qf[d][c][0], qf[d][c][1]);
         }
     }
     // positions g, g + 8 of each tile, columns 2 t, 2 t + 1
@@ -269,7 +269,7 @@ __device__ __forceinline__ bool attend(State<HD, SETS>& s, const std::uint32_t (
             }
 #pragma unroll
             for (int c = 0; c < SETS; ++c)
-                if (c == 0 || c < sets) attn8::mma_acc(s.o[d][c], a[0], a[1], a[2], a[3], pt[k][c][0], pt[k][c][1]);
+                attn8::mma_acc(s.o[d][c], a[0], a[1], a[2], a[3], pt[k][c][0], pt[k][c][1]);
         }
     return bad;
 }
@@ -595,8 +595,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < SETS; ++c)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) here[c][h] = limit[c][h] - from;
-            bad |= attend<HD, SETS>(s, qf, sets, ring + stage * kStage, koff, voff, p.scale_log2, masked,
-                                    static_cast<std::int32_t>(seq.len) - from, here);
+            const auto run = [&](auto n) {
+                return attend<HD, decltype(n)::value, SETS>(s, qf, ring + stage * kStage, koff, voff, p.scale_log2,
+                                                            masked, static_cast<std::int32_t>(seq.len) - from, here);
+            };
+            if (SETS == 1 || sets == 1) bad |= run(std::integral_constant<int, 1>{});
+            else if (SETS == 2 || sets == 2) bad |= run(std::integral_constant<int, SETS < 2 ? 1 : 2>{});
+            else bad |= run(std::integral_constant<int, SETS>{});
             if (++stage == kStages) stage = 0, parity ^= 1;
         }
 

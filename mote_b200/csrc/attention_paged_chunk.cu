@@ -820,77 +820,47 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 
-// Adds up the parts of the pairs that lie in several CTAs, in order: a task is 32
-// rows of a pair and 32 of the HD dimensions.
+// Adds up the parts of the pairs that lie in several CTAs, in order: a CTA takes 32
+// rows and 64 dimensions of one pair, or returns where there is none.
 template <int HD>
-__global__ void __launch_bounds__(256) join_kernel(const ChunkParams c, const std::uint32_t ctas) {
-    __shared__ std::uint32_t list[kMaxCtas];
-    __shared__ std::uint32_t counts[8];
-    __shared__ float wts[kMaxCtas][32];
-    __shared__ float invs[32];
+__global__ void __launch_bounds__(256) join_kernel(const ChunkParams c) {
     const Params& p = c.p;
-    const std::uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const std::uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x;
     pdl_launch_dependents();
     pdl_wait();
-    // the pairs that there are
-    const bool has = threadIdx.x < ctas && __ldcg(&c.joins[threadIdx.x].count) != 0;
-    const unsigned mask = __ballot_sync(0xffffffffu, has);
-    if (lane == 0) counts[warp] = __popc(mask);
-    __syncthreads();
-    std::uint32_t lower = 0, all = 0;
+    const Join j = c.joins[cta];
+    const std::uint32_t row = blockIdx.y * 32 + lane, m = row / kBM, tok = row % kBM / p.group, head = row % kBM % p.group;
+    const std::uint32_t token = m * c.tile_tokens + tok, d = blockIdx.z * 16 + warp;
+    if (j.count == 0 || tok >= c.tile_tokens || token >= j.left) return;
+    const auto part_of = [&](std::uint32_t k) {
+        return c.parts + static_cast<std::uint64_t>(2 * (cta + k) + (k == 0 ? 1 : 0)) * kPart<HD>;
+    };
+    const auto ml_of = [&](std::uint32_t k) {
+        return __ldcg(reinterpret_cast<const float2*>(part_of(k) + 256 * HD) + row);
+    };
+    float mt = -INFINITY, lt = 0.f;
+#pragma unroll 8
+    for (std::uint32_t k = 0; k < j.count; ++k) mt = fmaxf(mt, ml_of(k).x);
+    float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll 8
+    for (std::uint32_t k = 0; k < j.count; ++k) {
+        const float4* part = reinterpret_cast<const float4*>(part_of(k)) + row;
+        const float4 y0 = __ldcg(part + 256 * d), y1 = __ldcg(part + 256 * (d + 8));
+        const float2 a = ml_of(k);
+        if (a.x == -INFINITY && a.y == 0.f) continue;  // no position of its own there
+        const float w = a.y != a.y || a.x == mt ? 1.f : ex2f((a.x - mt) * p.scale_log2);
+        lt = fmaf(a.y, w, lt);
+        o[0].x = fmaf(y0.x, w, o[0].x), o[0].y = fmaf(y0.y, w, o[0].y);
+        o[0].z = fmaf(y0.z, w, o[0].z), o[0].w = fmaf(y0.w, w, o[0].w);
+        o[1].x = fmaf(y1.x, w, o[1].x), o[1].y = fmaf(y1.y, w, o[1].y);
+        o[1].z = fmaf(y1.z, w, o[1].z), o[1].w = fmaf(y1.w, w, o[1].w);
+    }
+    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    __half* dst = p.out + (static_cast<std::uint64_t>(j.q0 + token) * p.q_heads + j.kvh * p.group + head) * HD;
 #pragma unroll
-    for (std::uint32_t w = 0; w < 8; ++w) {
-        if (w < warp) lower += counts[w];
-        all += counts[w];
-    }
-    if (has) list[lower + __popc(mask & ((1u << lane) - 1u))] = threadIdx.x;
-    __syncthreads();
-    constexpr std::uint32_t kTasks = 8 * HD / 32;
-    for (std::uint32_t task = blockIdx.x; task < all * kTasks; task += gridDim.x) {
-        const std::uint32_t cta = list[task / kTasks], r0 = task % kTasks / (HD / 32) * 32, d0 = task % (HD / 32) * 8;
-        const Join j = c.joins[cta];
-        const auto part_of = [&](std::uint32_t k) {
-            return c.parts + static_cast<std::uint64_t>(2 * (cta + k) + (k == 0 ? 1 : 0)) * kPart<HD>;
-        };
-        const std::uint32_t row = r0 + lane, m = row / kBM, tok = row % kBM / p.group, head = row % kBM % p.group;
-        const std::uint32_t token = m * c.tile_tokens + tok;
-        const bool mine = tok < c.tile_tokens && token < j.left;
-        if (__syncthreads_or(mine) == 0) continue;
-        // every warp the weights of every eighth part
-        const auto ml_of = [&](std::uint32_t k) {
-            return __ldcg(reinterpret_cast<const float2*>(part_of(k) + 256 * HD) + row);
-        };
-        float mt = -INFINITY;
-        for (std::uint32_t k = 0; k < j.count; ++k) mt = fmaxf(mt, ml_of(k).x);
-        float lt = 0.f;
-        for (std::uint32_t k = warp; k < j.count; k += 8) {
-            const float2 a = ml_of(k);
-            const float w = a.y != a.y || a.x == mt ? 1.f : ex2f((a.x - mt) * p.scale_log2);
-            wts[k][lane] = w;
-        }
-        __syncthreads();
-        if (warp == 0) {
-            for (std::uint32_t k = 0; k < j.count; ++k) lt += ml_of(k).y * wts[k][lane];
-            invs[lane] = lt == 0.f ? 0.f : 1.f / lt;
-        }
-        __syncthreads();
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (mine) {
-#pragma unroll 4
-            for (std::uint32_t k = 0; k < j.count; ++k) {
-                const float4 y = __ldcg(reinterpret_cast<const float4*>(part_of(k)) + 256 * (d0 + warp) + row);
-                const float2 a = ml_of(k);
-                const float w = wts[k][lane];
-                if (a.x == -INFINITY && a.y == 0.f) continue;  // no position of its own there
-                o.x = fmaf(y.x, w, o.x), o.y = fmaf(y.y, w, o.y);
-                o.z = fmaf(y.z, w, o.z), o.w = fmaf(y.w, w, o.w);
-            }
-            const float inv = invs[lane];
-            __half* dst = p.out + (static_cast<std::uint64_t>(j.q0 + token) * p.q_heads + j.kvh * p.group + head) * HD + 4 * (d0 + warp);
-            *reinterpret_cast<uint2*>(dst) = make_uint2(attn8::half2_of(o.x * inv, o.y * inv), attn8::half2_of(o.z * inv, o.w * inv));
-        }
-        __syncthreads();  // the scratch is read
-    }
+    for (int k = 0; k < 2; ++k)
+        *reinterpret_cast<uint2*>(dst + 4 * (d + 8 * k)) =
+            make_uint2(attn8::half2_of(o[k].x * inv, o[k].y * inv), attn8::half2_of(o[k].z * inv, o[k].w * inv));
 }
 
 template <int HD>
@@ -917,8 +887,7 @@ int launch(const ChunkParams& c, const void* q, const void* k_cache, int ctas, c
     st = launch_pdl_smem(chunk_kernel<HD>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), Smem<HD>::kBytes,
                          stream, map_q, map_k, map_v, c);
     if (st != kSuccess) return st;
-    return launch_pdl(join_kernel<HD>, dim3(static_cast<unsigned>(2 * ctas)), dim3(256), stream, c,
-                      static_cast<std::uint32_t>(ctas));
+    return launch_pdl(join_kernel<HD>, dim3(static_cast<unsigned>(ctas), 8, HD / 64), dim3(256), stream, c);
 }
 
 // Bytes of the workspace: counters and parts of the few-row kernel, then parts and

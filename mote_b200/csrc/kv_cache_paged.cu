@@ -35,43 +35,77 @@ struct Params {
 
 constexpr int kThreads = 128;
 
-// One CTA for each token.
-__global__ void __launch_bounds__(kThreads) append_kernel(const Params p) {
+// Where token t's k and v go: rows of the first KV head, a head `head_stride`
+// further (k null: nowhere), and whether its row belongs to a sequence at all.
+struct Place {
+    __half* k;
+    __half* v;
+    bool any;
+};
+
+// By a whole warp.
+__device__ __forceinline__ Place place_of(const Params& p, std::uint32_t t) {
+    Place x{nullptr, nullptr, false};
+    const std::uint32_t lane = threadIdx.x & 31;
+    std::uint32_t b;
+    std::int32_t s0, s1, length;
+    if (p.c.batch <= 32) {  // one sequence to a lane: one round of loads
+        const bool here = lane < p.c.batch;
+        const std::int32_t a0 = here ? __ldg(p.starts + lane) : 0, a1 = here ? __ldg(p.starts + lane + 1) : 0;
+        const std::int32_t al = here ? __ldg(p.lens + lane) : 0;
+        const unsigned below = __ballot_sync(0xffffffffu, here && static_cast<std::uint32_t>(max(a0, 0)) <= t);
+        const unsigned run = below == 0xffffffffu ? 32u : __ffs(~below) - 1u;  // as warp_search counts
+        b = run == 0 ? 0 : run - 1;
+        s0 = __shfl_sync(0xffffffffu, a0, b), s1 = __shfl_sync(0xffffffffu, a1, b);
+        length = __shfl_sync(0xffffffffu, al, b);
+    } else {
+        b = kvq8::warp_search(p.c.batch, t, [&](std::uint32_t i) {
+            return static_cast<std::uint32_t>(max(__ldg(p.starts + i), 0));
+        });
+        s0 = __ldg(p.starts + b), s1 = __ldg(p.starts + b + 1), length = __ldg(p.lens + b);
+    }
+    if (s0 < 0 || s1 < s0 || static_cast<std::uint32_t>(s1) > p.tokens ||
+        t < static_cast<std::uint32_t>(s0) || t >= static_cast<std::uint32_t>(s1))
+        return x;
+    const std::int64_t len = length, pos = len - s1 + t;
+    if (len < s1 - s0 || len > static_cast<std::int64_t>(p.c.max_blocks) * p.c.block_tokens) {
+        if (lane == 0) kvq8::report(p.error_flag);
+        return x;
+    }
+    x.any = true;
+    const std::uint32_t i = static_cast<std::uint32_t>(pos) / p.c.block_tokens;
+    const std::int32_t block = __ldg(p.tables + static_cast<std::uint64_t>(b) * p.c.max_blocks + i);
+    if (block < 0 || static_cast<std::uint64_t>(block) >= p.c.num_blocks) {
+        if (lane == 0) kvq8::report(p.error_flag);
+        return x;
+    }
+    const std::uint64_t row = (static_cast<std::uint64_t>(block) * p.c.kv_heads * p.c.block_tokens +
+                               (static_cast<std::uint32_t>(pos) - i * p.c.block_tokens)) * p.c.head_dim;
+    x.k = p.k_cache + row;
+    x.v = p.v_cache + row;
+    return x;
+}
+
+// Pairs or head parts that are no whole 16-byte vectors, or tables that are not
+// aligned to them: one CTA for each token, element by element.
+__global__ void __launch_bounds__(kThreads) append_scalar_kernel(const Params p) {
     pdl_launch_dependents();
     pdl_wait();
     if (blockIdx.x == 0) kvq8::check_starts(p.c, p.starts, p.tokens, p.error_flag);
     const std::uint32_t t = blockIdx.x, hd = p.c.head_dim, kvh = p.c.kv_heads;
-    const std::uint32_t b = kvq8::warp_search(p.c.batch, t, [&](std::uint32_t i) {
-        return static_cast<std::uint32_t>(max(__ldg(p.starts + i), 0));
-    });
-    const std::int32_t s0 = __ldg(p.starts + b), s1 = __ldg(p.starts + b + 1);
-    if (s0 < 0 || s1 < s0 || static_cast<std::uint32_t>(s1) > p.tokens ||
-        t < static_cast<std::uint32_t>(s0) || t >= static_cast<std::uint32_t>(s1))
-        return;  // a row of no sequence
-    const std::int64_t len = __ldg(p.lens + b), pos = len - s1 + t;
-    if (len < s1 - s0 || len > static_cast<std::int64_t>(p.c.max_blocks) * p.c.block_tokens) {
-        if (threadIdx.x == 0) kvq8::report(p.error_flag);
-        return;
-    }
-    const std::int32_t block = __ldg(p.tables + static_cast<std::uint64_t>(b) * p.c.max_blocks + pos / p.c.block_tokens);
-    const bool there = block >= 0 && static_cast<std::uint64_t>(block) < p.c.num_blocks;
-    if (!there && threadIdx.x == 0) kvq8::report(p.error_flag);
-    const std::uint64_t tile = static_cast<std::uint64_t>(block) * kvh;
-    const std::uint32_t off = static_cast<std::uint32_t>(pos % p.c.block_tokens);
-    const __half* row = p.qkv + static_cast<std::uint64_t>(t) * (p.q_heads + 2 * kvh) * hd;
-    const auto dst_of = [&](std::uint32_t h) -> __half* {
-        if (h < p.q_heads) return p.q_out + (static_cast<std::uint64_t>(t) * p.q_heads + h) * hd;
-        if (!there) return nullptr;
-        const std::uint32_t k = h - p.q_heads;
-        return k < kvh ? p.k_cache + ((tile + k) * p.c.block_tokens + off) * hd
-                       : p.v_cache + ((tile + k - kvh) * p.c.block_tokens + off) * hd;
-    };
+    const Place place = place_of(p, t);
+    if (!place.any) return;
     const std::uint32_t heads = p.q_heads + 2 * kvh, rotated = p.q_heads + kvh;
+    const std::uint64_t stride = static_cast<std::uint64_t>(p.c.block_tokens) * hd;
+    const __half* row = p.qkv + static_cast<std::uint64_t>(t) * heads * hd;
     for (std::uint32_t i = threadIdx.x; i < heads * hd; i += kThreads) {
         const std::uint32_t h = i / hd, e = i - h * hd;
         const __half* src = row + h * hd;
-        __half* dst = dst_of(h);
-        if (dst == nullptr) continue;
+        __half* dst = p.q_out + (static_cast<std::uint64_t>(t) * p.q_heads + h) * hd;
+        if (h >= p.q_heads) {
+            if (place.k == nullptr) continue;
+            dst = h < rotated ? place.k + (h - p.q_heads) * stride : place.v + (h - rotated) * stride;
+        }
         if (h >= rotated || e >= 2 * p.pairs) {
             dst[e] = src[e];
             continue;
@@ -79,11 +113,115 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const Params p) {
         const std::uint32_t j = p.interleaved ? e / 2 : e % p.pairs;
         const bool second = p.interleaved ? e & 1 : e >= p.pairs;
         const float a = __half2float(src[p.interleaved ? 2 * j : j]);
-        const float bb = __half2float(src[p.interleaved ? 2 * j + 1 : j + p.pairs]);
+        const float b = __half2float(src[p.interleaved ? 2 * j + 1 : j + p.pairs]);
         float o1, o2;
-        rotate(a, bb, p.cos[static_cast<std::uint64_t>(t) * p.pairs + j],
+        rotate(a, b, p.cos[static_cast<std::uint64_t>(t) * p.pairs + j],
                p.sin[static_cast<std::uint64_t>(t) * p.pairs + j], o1, o2);
         dst[e] = __float2half_rn(second ? o2 : o1);
+    }
+}
+
+__device__ __forceinline__ float2 halves(std::uint32_t w) {
+    __half2 h;
+    memcpy(&h, &w, 4);
+    return __half22float2(h);
+}
+
+// HBM-bound: rows in 16-byte vectors, read and written once.  `per_token` threads
+// (32, 64 or 128) take a token.  Each keeps one place within a head (a vector and
+// its partner half a rotary width further, or one vector of interleaved pairs) with
+// the place's cosines and sines in registers, and goes through the heads; its first
+// kHeld of them, and the v heads, load while the token's sequence and page are found.
+constexpr int kHeld = 4;
+template <bool HALF>
+__global__ void __launch_bounds__(kThreads) append_kernel(const Params p, const std::uint32_t per_token) {
+    pdl_launch_dependents();
+    pdl_wait();
+    if (blockIdx.x == 0) kvq8::check_starts(p.c, p.starts, p.tokens, p.error_flag);
+    const std::uint32_t t = blockIdx.x * (kThreads / per_token) + threadIdx.x / per_token;
+    if (t >= p.tokens) return;  // (whole warps)
+    const std::uint32_t me = threadIdx.x % per_token;
+    const std::uint32_t hd = p.c.head_dim, kvh = p.c.kv_heads, vecs = hd / 8;
+    const std::uint32_t turned = HALF ? p.pairs / 8 : p.pairs / 4;     // places of a head that turn
+    const std::uint32_t places = HALF ? vecs - turned : vecs;
+    const std::uint32_t step = per_token / places;                     // heads at a time
+    const std::uint32_t u = me % places, h0 = me / places < step ? me / places : 0x7fffffffu;
+    const bool turns = u < turned;
+    const std::uint32_t at = HALF && !turns ? u + turned : u;          // vectors of the place
+    const std::uint32_t heads = p.q_heads + 2 * kvh, rotated = p.q_heads + kvh;
+    const uint4* row = reinterpret_cast<const uint4*>(p.qkv) + static_cast<std::uint64_t>(t) * heads * vecs;
+    uint4 x[kHeld][HALF ? 2 : 1], v = make_uint4(0, 0, 0, 0);
+    const auto load = [&](std::uint32_t base) {
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            const std::uint32_t h = base + k * step;
+            if (h >= rotated) break;
+            x[k][0] = __ldg(row + h * vecs + at);
+            if (HALF && turns) x[k][HALF ? 1 : 0] = __ldg(row + h * vecs + at + turned);
+        }
+    };
+    load(h0);
+    if (me < kvh * vecs) v = __ldg(row + rotated * vecs + me);
+    constexpr int N = HALF ? 8 : 4;  // pairs of a place
+    float c[N], s[N];
+    if (turns) {
+        const float4* cp = reinterpret_cast<const float4*>(p.cos + static_cast<std::uint64_t>(t) * p.pairs + N * u);
+        const float4* sp = reinterpret_cast<const float4*>(p.sin + static_cast<std::uint64_t>(t) * p.pairs + N * u);
+#pragma unroll
+        for (int k = 0; k < N / 4; ++k) {
+            const float4 a = __ldg(cp + k), b = __ldg(sp + k);
+            c[4 * k] = a.x, c[4 * k + 1] = a.y, c[4 * k + 2] = a.z, c[4 * k + 3] = a.w;
+            s[4 * k] = b.x, s[4 * k + 1] = b.y, s[4 * k + 2] = b.z, s[4 * k + 3] = b.w;
+        }
+    }
+    const Place place = place_of(p, t);
+    if (!place.any) return;
+    const std::uint64_t stride = static_cast<std::uint64_t>(p.c.block_tokens) * vecs;
+    uint4* const q_out = reinterpret_cast<uint4*>(p.q_out) + static_cast<std::uint64_t>(t) * p.q_heads * vecs;
+    uint4* const k_out = reinterpret_cast<uint4*>(place.k);
+    for (std::uint32_t base = h0; base < rotated; base += kHeld * step) {
+        if (base != h0) load(base);
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+            const std::uint32_t h = base + k * step;
+            if (h >= rotated) break;
+            uint4* const dst = h < p.q_heads ? q_out + h * vecs
+                                             : k_out == nullptr ? nullptr : k_out + (h - p.q_heads) * stride;
+            if (dst == nullptr) break;  // (the heads behind are k's too)
+            if (!turns) {
+                dst[at] = x[k][0];
+                continue;
+            }
+            const std::uint32_t a[4] = {x[k][0].x, x[k][0].y, x[k][0].z, x[k][0].w};
+            std::uint32_t o[4], o2[4];
+            if constexpr (HALF) {
+                const std::uint32_t b[4] = {x[k][1].x, x[k][1].y, x[k][1].z, x[k][1].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 y = halves(a[e]), z = halves(b[e]);
+                    float r0, r1, w0, w1;
+                    rotate(y.x, z.x, c[2 * e], s[2 * e], r0, w0);
+                    rotate(y.y, z.y, c[2 * e + 1], s[2 * e + 1], r1, w1);
+                    o[e] = attn8::half2_of(r0, r1), o2[e] = attn8::half2_of(w0, w1);
+                }
+                dst[at + turned] = make_uint4(o2[0], o2[1], o2[2], o2[3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 y = halves(a[e]);
+                    float r0, r1;
+                    rotate(y.x, y.y, c[e], s[e], r0, r1);
+                    o[e] = attn8::half2_of(r0, r1);
+                }
+            }
+            dst[at] = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+    if (place.v == nullptr) return;
+    uint4* const v_out = reinterpret_cast<uint4*>(place.v);
+    for (std::uint32_t i = me; i < kvh * vecs; i += per_token) {
+        if (i != me) v = __ldg(row + rotated * vecs + i);
+        v_out[i / vecs * stride + i % vecs] = v;
     }
 }
 
@@ -123,6 +261,13 @@ extern "C" int mote_cuda_rope_kv_cache_append_paged_f16(
     p.pairs = static_cast<std::uint32_t>(pairs);
     p.interleaved = layout == 1;
     p.error_flag = static_cast<unsigned*>(error_flag);
-    return launch_pdl(kvpaged::append_kernel, dim3(p.tokens), dim3(kvpaged::kThreads),
-                      static_cast<cudaStream_t>(stream), p);
+    const auto stream_ = static_cast<cudaStream_t>(stream);
+    if (p.pairs % (p.interleaved ? 4 : 8) != 0 || !kvq8::aligned16({cos, sin}))
+        return launch_pdl(kvpaged::append_scalar_kernel, dim3(p.tokens), dim3(kvpaged::kThreads), stream_, p);
+    // threads of a token: one for each place of kHeld heads, or so
+    const std::uint64_t vecs = head_dim / 8, work = (q_heads + kv_heads) * (p.interleaved ? vecs : vecs - pairs / 8);
+    const std::uint32_t per = work <= 32 * kvpaged::kHeld ? 32 : work <= 64 * kvpaged::kHeld ? 64 : 128;
+    const std::uint32_t each = kvpaged::kThreads / per;
+    return launch_pdl(p.interleaved ? kvpaged::append_kernel<false> : kvpaged::append_kernel<true>,
+                      dim3((p.tokens + each - 1) / each), dim3(kvpaged::kThreads), stream_, p, per);
 }

@@ -43,8 +43,11 @@ __device__ __forceinline__ void angle(std::int32_t position, double quarters, fl
     const double n = q + kWhole;
     const float r = static_cast<float>(q - (n - kWhole));
     const int k = __double2loint(n);
-    float sr, cr;
-    sincospif(0.5f * r, &sr, &cr);
+    // sine and cosine of x = pi r / 2, |x| <= pi / 4, by their Taylor series: what
+    // follows x^9 and x^10 is below 2^-28
+    const float x = r * 1.57079632679489662f, y = x * x;
+    const float sr = fmaf(x * y, fmaf(y, fmaf(y, fmaf(y, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), x);
+    const float cr = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
     const float a = k & 1 ? sr : cr, b = k & 1 ? cr : sr;
     c = (k + 1) & 2 ? -a : a;
     s = k & 2 ? -b : b;
