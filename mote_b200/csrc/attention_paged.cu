@@ -6,9 +6,10 @@
 // no sequence keep their values.
 //
 // Two kernels, each for its own sequences of a batch (the lengths are on the
-// device): this file's for sequences with up to 32 query rows (tokens times
-// grouped heads) of a KV head, whose cost is the stream of K and V;
-// attention_paged_chunk.cu's for more, on the tcgen05 tensor cores.
+// device): this file's for sequences with up to 16 query rows (tokens times grouped
+// heads of a KV head), whose cost is the stream of K and V;
+// attention_paged_chunk.cu's for more, on the tcgen05 tensor cores.  Where a batch may hold both, the kernels run at the same time, on SMs
+// that they divide by the work that each has (few_ctas).
 //
 // Few rows: HBM-bound, K and V of the attended positions are read once.
 // * The work is cut in units of 8 KB of K and V (16 positions at head_dim 128, 32
@@ -57,6 +58,9 @@ struct Params {
     std::uint32_t tokens, q_heads, group, max_new;
     std::uint32_t few;   // query rows of a KV head up to which a sequence is the first kernel's
     bool reports;        // this kernel tells of sequences that are skipped
+    bool shares;         // both kernels run, each on its part of the SMs
+    std::uint32_t tile_tokens;  // of a query tile of the chunk kernel: floor(128 / group)
+    std::uint32_t sub;   // loads of K in a unit of the few-row kernel
     float scale_log2;
     unsigned* counters;  // [kMaxCtas], zero between calls
     float* parts;
@@ -67,8 +71,13 @@ struct Seq {
     std::uint32_t q0, n, len;
     bool bad;
 };
+// Offsets, lengths and block numbers.  A kernel that runs beside the other one does
+// not wait for what is before both (that one has), so it reads past its L1.
+__device__ __forceinline__ std::int32_t fetch(const Params& p, const std::int32_t* x) {
+    return p.shares ? __ldcg(x) : __ldg(x);
+}
 __device__ __forceinline__ Seq sequence(const Params& p, std::uint32_t b) {
-    const std::int32_t s0 = __ldg(p.starts + b), s1 = __ldg(p.starts + b + 1), len = __ldg(p.lens + b);
+    const std::int32_t s0 = fetch(p, p.starts + b), s1 = fetch(p, p.starts + b + 1), len = fetch(p, p.lens + b);
     Seq s{static_cast<std::uint32_t>(s0), static_cast<std::uint32_t>(s1 - s0), static_cast<std::uint32_t>(len), false};
     s.bad = s0 < 0 || s1 < s0 || static_cast<std::uint32_t>(s1) > p.tokens ||
             (s1 > s0 && (len < 0 || static_cast<std::uint32_t>(len) > p.c.max_blocks * p.c.block_tokens || s.n > p.max_new));
@@ -80,12 +89,67 @@ __device__ __forceinline__ void report_bad(const Params& p, std::uint32_t first,
         if (sequence(p, b).bad) atomicOr(&g_device_status, kDevIndexOutOfRange);
 }
 
+// The chunk kernel's work, a line of positions: all pairs of query tiles of all its
+// sequences and KV heads, each as long as the positions that it attends and its end
+// (kEnd).  A pair whose second tile has no rows counts as much: it streams as much.
+constexpr std::uint32_t kEnd = 256;
+
+// A sequence's pairs on that line, for one KV head.
+struct Pairs {
+    Seq s;
+    std::uint32_t span;   // tokens of a pair
+    std::uint32_t count;  // pairs
+
+    __device__ __forceinline__ Pairs(const Params& p, const Seq& of) : s(of), span(2 * p.tile_tokens) {
+        if (static_cast<std::uint64_t>(s.n) * p.group <= p.few) s.n = 0;
+        count = (s.n + span - 1) / span;
+    }
+    // positions that pair i attends
+    __device__ __forceinline__ std::uint32_t reach(std::uint32_t i) const {
+        const std::uint32_t end = s.len + min((i + 1) * span, s.n);  // below 2^32
+        return end > s.n ? end - s.n : 0u;
+    }
+    __device__ __forceinline__ std::uint32_t extent(std::uint32_t i) const { return reach(i) + kEnd; }
+    // extents of the pairs before i (i <= count): a series, but for pairs that
+    // attend nothing and the last one
+    __device__ __forceinline__ std::uint64_t before(std::uint32_t i) const {
+        const std::uint32_t full = i < count ? i : count == 0 ? 0 : count - 1;
+        // reach(k) = len - n + (k + 1) span for k = none .. full - 1
+        const std::uint32_t none = s.n > s.len ? min((s.n - s.len) / span, full) : 0u, m = full - none;
+        const std::int64_t sum = static_cast<std::int64_t>(m) * (static_cast<std::int64_t>(s.len) - s.n) +
+                                 static_cast<std::int64_t>(static_cast<std::uint64_t>(span) * (static_cast<std::uint64_t>(m) * none + static_cast<std::uint64_t>(m) * (m + 1ull) / 2));
+        const std::uint64_t x = static_cast<std::uint64_t>(sum) + static_cast<std::uint64_t>(full) * kEnd;
+        return i < count || count == 0 ? x : x + extent(count - 1);
+    }
+    __device__ __forceinline__ std::uint64_t all() const { return before(count); }
+};
+
+// The chunk kernel's work of a sequence.
+__device__ __forceinline__ std::uint64_t line_of(const Params& p, const Seq& s) {
+    return Pairs(p, s).all() * p.c.kv_heads;
+}
+// SMs of `n` that the few-row kernel has where both run, from its work (units, row
+// ends counted) and the other's (positions): a unit takes an SM about as long as
+// kUnitCost positions of a pair.  In f32, of which both kernels make the same.
+constexpr float kUnitCost = 11.f;
+__device__ __forceinline__ std::uint32_t few_ctas(std::uint32_t n, std::uint64_t units, std::uint64_t line) {
+    if (line == 0) return n;
+    if (units == 0) return 0;
+    const float mine = __fmul_rn(__ull2float_rn(units), kUnitCost), all = __fadd_rn(mine, __ull2float_rn(line));
+    const std::uint32_t x = __float2uint_rn(__fmul_rn(__fdiv_rn(mine, all), static_cast<float>(n)));
+    return min(max(x, 1u), n - 1);
+}
+// A share of `total` over `ctas`, rounded up (by up to 2^-22 of it).
+__device__ __forceinline__ std::uint64_t share_of(std::uint64_t total, std::uint32_t ctas) {
+    return __float2ull_ru(__fmul_ru(__ull2float_ru(total), __frcp_ru(static_cast<float>(ctas)))) + 1;
+}
+
 namespace few {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kCols = 8;         // columns of a set: (token, query head) pairs
-constexpr int kMaxSets = 4;
+constexpr int kMaxSets = 2;
 constexpr int kBox = 2048;       // 16 rows of 128 bytes
 constexpr int kStage = 4 * kBox; // K and V of a unit
 constexpr int kStages = 3;
@@ -142,13 +206,13 @@ constexpr float kMostSum = 32768.f;
 // subtracted, so that equal scores of any size weigh the same.
 constexpr float kVast = 1024.f;
 
-// One unit more, for SETS of the MOST sets.  `limit` holds how many of the unit's positions each of the
-// lane's columns attends, where `masked` (some column does not attend all); `live`
-// how many there are.  Returns whether V held something that is not finite.
+// One unit more, for SETS of the MOST sets.  `limit` holds how many of the unit's
+// positions each of the lane's columns attends, where `masked` (some column does not
+// attend all).
 template <int HD, int SETS, int MOST>
-__device__ __forceinline__ bool attend(State<HD, MOST>& s, const std::uint32_t (&qf)[HD / 16][MOST][2],
+__device__ __forceinline__ void attend(State<HD, MOST>& s, const std::uint32_t (&qf)[HD / 16][MOST][2],
                                        std::uint32_t stage, std::uint32_t koff,
-                                       std::uint32_t voff, float sc, bool masked, std::int32_t live,
+                                       std::uint32_t voff, float sc, bool masked,
                                        const std::int32_t (&limit)[MOST][2]) {
     constexpr int T = 128 / HD;  // tiles of 16 positions
     const std::uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -250,28 +314,52 @@ __device__ __forceinline__ bool attend(State<HD, MOST>& s, const std::uint32_t (
             for (int i = 0; i < 2; ++i)
                 pt[k][c][i] = attn8::transpose8x8(attn8::half2_of(p[k][c][2 * i], p[k][c][2 * i + 1]));
     }
-    bool bad = false;
 #pragma unroll
     for (int k = 0; k < T; ++k)
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) {
             std::uint32_t a[4];
             ldsm_x4_trans(stage + 2 * kBox + (HD == 128 ? d / 4 : k) * kBox + (voff ^ (d % 4 << 5)), a);
-            if (masked) {
-                // positions 2 t, 2 t + 1 (a[0], a[1]) and 8 more (a[2], a[3])
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const std::int32_t left = live - static_cast<std::int32_t>(16 * k + 2 * t + 8 * (i >> 1));
-                    a[i] &= left >= 2 ? 0xffffffffu : left == 1 ? 0x0000ffffu : 0u;
-                    if ((a[i] & 0x7c00u) == 0x7c00u) a[i] &= 0xffff0000u, bad = true;
-                    if ((a[i] & 0x7c000000u) == 0x7c000000u) a[i] &= 0x0000ffffu, bad = true;
-                }
-            }
 #pragma unroll
             for (int c = 0; c < SETS; ++c)
                 attn8::mma_acc(s.o[d][c], a[0], a[1], a[2], a[3], pt[k][c][0], pt[k][c][1]);
         }
+}
+
+// Rows of a unit's V behind its first `live` positions become zeros, and values that
+// are not finite too; whether there were any among the positions.  By a warp.
+template <int HD>
+__device__ __forceinline__ bool clean(std::uint8_t* v, std::int32_t live) {
+    bool bad = false;
+
+    for (std::uint32_t x = threadIdx.x & 31; x < 2 * kBox / 16; x += 32) {
+        // 16-byte chunk x: row x / 8 of the two boxes (head_dim 128: of either)
+        const std::int32_t pos = static_cast<std::int32_t>(HD == 128 ? x / 8 % 16 : x / 8);
+        const uint4 y = reinterpret_cast<const uint4*>(v)[x];
+        std::uint32_t w[4] = {y.x, y.y, y.z, y.w};
+        bool any = pos >= live;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (pos >= live) w[e] = 0;
+            if ((w[e] & 0x7c00u) == 0x7c00u) w[e] &= 0xffff0000u, any = bad = true;
+            if ((w[e] & 0x7c000000u) == 0x7c000000u) w[e] &= 0x0000ffffu, any = bad = true;
+        }
+        if (any) reinterpret_cast<uint4*>(v)[x] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    fence_proxy_async_smem();  // before the next unit's load into the stage
+    __syncwarp();
     return bad;
+}
+
+// A sequence where it is this kernel's (n 0 otherwise), and its units.
+__device__ __forceinline__ Seq few_part(const Params& p, Seq s) {
+    if (static_cast<std::uint64_t>(s.n) * p.group > p.few) s.n = 0;
+    return s;
+}
+template <int HD>
+__device__ __forceinline__ std::uint32_t units_of(const Seq& s) {
+    constexpr std::uint32_t kUnit = 2048 / HD;
+    return s.n == 0 ? 0u : (s.len + kUnit - 1) / kUnit;
 }
 
 // A row of the work list: sequence b and KV head r, the units, and the virtual
@@ -287,8 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                const Params p) {
     using L = Smem<HD>;
-    constexpr int kSub = 128 / HD;      // tiles of 16 positions in a unit
-    constexpr int kUnit = 16 * kSub;
+    constexpr int kUnit = 2048 / HD;  // positions
     constexpr int kPart = kCols * SETS * (HD + 2);
     extern __shared__ std::uint8_t smem_raw[];
     const std::uint32_t raw = smem_u32(smem_raw);
@@ -302,25 +389,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     float* const ml = reinterpret_cast<float*>(smem + L::kMl);
     volatile std::uint32_t* bad_flags = reinterpret_cast<std::uint32_t*>(smem + L::kBad);
     volatile std::uint32_t* last_cta = reinterpret_cast<std::uint32_t*>(smem + L::kLast);
+    const std::uint32_t sub = p.sub;  // loads of K in a unit, each of kUnit / sub positions
     if (lane < kStages) {
-        mbar_init(&full[lane], kSub);
+        mbar_init(&full[lane], sub);
         fence_mbarrier_init();
     }
     if (threadIdx.x == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<std::uint64_t>(&map_k)) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<std::uint64_t>(&map_v)) : "memory");
     }
-    pdl_launch_dependents();
+    if (!p.shares) pdl_launch_dependents();
     pdl_wait();
+    // (the other kernel, which starts then, may rely on what is before this one)
+    if (p.shares) pdl_launch_dependents();
 
     const std::uint32_t batch = p.c.batch, bt = p.c.block_tokens, rows = p.c.kv_heads;
     // sequence b where it is this kernel's (n 0 otherwise)
-    const auto mine = [&](std::uint32_t b) {
-        Seq s = sequence(p, b);
-        if (static_cast<std::uint64_t>(s.n) * p.group > p.few) s.n = 0;
-        return s;
-    };
-    const auto units = [&](const Seq& s) { return s.n == 0 ? 0u : (s.len + kUnit - 1) / kUnit; };
+    const auto mine = [&](std::uint32_t b) { return few_part(p, sequence(p, b)); };
+    const auto units = [&](const Seq& s) { return units_of<HD>(s); };
     if (p.reports && blockIdx.x == gridDim.x - 1) report_bad(p, threadIdx.x, kThreads);
     // ---- the CTA's share --------------------------------------------------
     // Equal shares of the units, where a row's end counts as kRowCost units
@@ -328,16 +414,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     // CTA, of the smallest size (in small steps) that needs no more CTAs than
     // there are, unless shares are smaller by more than a row's end.
     std::uint32_t longest = 0, filled = 0;  // units, rows with any
-    std::uint64_t total = 0;
+    std::uint64_t total = 0, line = 0;      // units, and the other kernel's work
     std::uint32_t per = 0;  // units of a CTA
+    std::uint32_t ctas = gridDim.x;
     bool pieces = false;
     const auto least = [&] { return min(longest, static_cast<std::uint32_t>(kMinUnits)); };
     const auto share = [&] {
-        const std::uint64_t n = (total + static_cast<std::uint64_t>(filled) * kRowCost + gridDim.x - 1) / gridDim.x;
-        return max(static_cast<std::uint32_t>(n), least());
+        return max(static_cast<std::uint32_t>(share_of(total + static_cast<std::uint64_t>(filled) * kRowCost, ctas)), least());
     };
     const auto size = [&](std::uint32_t i, std::uint32_t steps) {  // pieces from the least on
-        const std::uint32_t low = max(static_cast<std::uint32_t>((total + gridDim.x - 1) / gridDim.x), least());
+        const std::uint32_t low = max(static_cast<std::uint32_t>(share_of(total, ctas)), least());
         return low + (low * i + steps - 1) / steps;
     };
     const auto extent = [&](std::uint32_t n) -> std::uint32_t {  // a row in virtual units
@@ -363,18 +449,26 @@ __global__ void __launch_bounds__(kThreads, 1)
     std::uint32_t at_b = 0;
     if (batch <= kFew) {
         // every warp for itself, one sequence to a lane
-        const std::uint32_t n = static_cast<std::uint32_t>(lane) < batch ? units(mine(lane)) : 0u;
+        std::uint32_t n = 0;
+        if (static_cast<std::uint32_t>(lane) < batch) {
+            const Seq s = sequence(p, lane);
+            n = units(few_part(p, s));
+            if (p.shares) line = line_of(p, s);
+        }
+        if (p.shares) line = __shfl_sync(0xffffffffu, scan_up(line), 31);
         longest = __reduce_max_sync(0xffffffffu, n);
         total = static_cast<std::uint64_t>(__reduce_add_sync(0xffffffffu, n)) * rows;
         filled = __popc(__ballot_sync(0xffffffffu, n > 0)) * rows;
-        if (total == 0) return;
+        if (p.shares) ctas = few_ctas(ctas, total + static_cast<std::uint64_t>(filled) * kRowCost, line);
+        if (total == 0 || blockIdx.x >= ctas) return;
         per = share();
-        if (filled <= gridDim.x) {
+        if (filled <= ctas) {
             const std::uint32_t step = size(lane, 32);
             std::uint32_t need = 0;
+
             for (std::uint32_t b = 0; b < batch; ++b)
                 need += (__shfl_sync(0xffffffffu, n, b) + step - 1) / step;
-            const unsigned fits = __ballot_sync(0xffffffffu, need * rows <= gridDim.x);
+            const unsigned fits = __ballot_sync(0xffffffffu, need * rows <= ctas);
             const std::uint32_t best = __shfl_sync(0xffffffffu, step, fits ? __ffs(fits) - 1 : 0);
             pieces = fits != 0 && best <= per + kRowCost;
             if (pieces) per = best;
@@ -390,8 +484,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         // the CTA together (scratch: the flush area)
         volatile std::uint64_t* found = reinterpret_cast<std::uint64_t*>(flush);  // [0..3], sums [4 + warp]
         volatile std::uint32_t* scan = reinterpret_cast<std::uint32_t*>(flush) + 64;  // [warp][2]
+
         for (std::uint32_t b = threadIdx.x; b < batch; b += kThreads) {
-            const std::uint32_t n = units(mine(b));
+            const Seq s = sequence(p, b);
+            const std::uint32_t n = units(few_part(p, s));
+            if (p.shares) line += line_of(p, s);
             total += n;
             filled += n > 0;
             longest = max(longest, n);
@@ -399,30 +496,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         longest = __reduce_max_sync(0xffffffffu, longest);
         filled = __reduce_add_sync(0xffffffffu, filled);
         total = __shfl_sync(0xffffffffu, scan_up(total), 31);
+        line = __shfl_sync(0xffffffffu, scan_up(line), 31);
         if (lane == 0) {
             found[4 + warp] = total;
+            found[4 + kWarps + warp] = line;
             scan[2 * warp] = longest;
             scan[2 * warp + 1] = filled;
         }
         __syncthreads();
-        total = 0, filled = 0, longest = 0;
+        total = 0, filled = 0, longest = 0, line = 0;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             longest = max(longest, scan[2 * w]);
             total += found[4 + w];
+            line += found[4 + kWarps + w];
             filled += scan[2 * w + 1];
         }
         total *= rows;
         filled *= rows;
         __syncthreads();
-        if (total == 0) return;
+        if (p.shares) ctas = few_ctas(ctas, total + static_cast<std::uint64_t>(filled) * kRowCost, line);
+        if (total == 0 || blockIdx.x >= ctas) return;
         per = share();
-        if (filled <= gridDim.x) {
+        if (filled <= ctas) {
             const std::uint32_t step = size(warp, kWarps);
             std::uint32_t need = 0;
+
             for (std::uint32_t b = lane; b < batch; b += 32) need += (units(mine(b)) + step - 1) / step;
             need = __reduce_add_sync(0xffffffffu, need) * rows;
-            if (lane == 0) scan[warp] = need <= gridDim.x;
+            if (lane == 0) scan[warp] = need <= ctas;
             __syncthreads();
             int w = 0;
             while (w < kWarps && !scan[w]) ++w;
@@ -433,6 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         u0 = static_cast<std::uint64_t>(per) * blockIdx.x;
         std::uint64_t before = 0;  // extents of the sequences before the chunk
         if (threadIdx.x == 0) found[1] = 0;
+
         for (std::uint32_t base = 0;; base += kThreads) {
             const std::uint32_t b = base + threadIdx.x;
             const std::uint32_t n = b < batch ? units(mine(b)) : 0u;
@@ -486,14 +589,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     row.begin = at_begin + static_cast<std::uint64_t>(row.r) * extent(row.n);
 
     // ---- the stream: each warp keeps its ring full, across rows -------------
-    // the blocks of 32 / kSub units of this warp, from held_unit of sequence
-    // held_b on: one lane for each 16 positions, as the row of its first head's
-    // tile in the cache
+    // the blocks of 32 / sub units of this warp, from held_unit of sequence held_b
+    // on: one lane for each load
     std::uint32_t a_unit = first_of(row) + warp, a_last = last_of(row), a_slot = 0, a_stage = 0;
     Row ahead = row;
     std::int32_t held_block = -1;
     std::uint32_t held_row = 0, held_b = ~0u, held_unit = 0;
     const auto issue = [&]() {
+
         while (a_unit >= a_last) {
             if (ahead.begin >= u1) return;
             next(ahead);
@@ -502,12 +605,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (a_slot == 0 && (held_b != ahead.b || held_unit != a_unit)) {
             held_b = ahead.b, held_unit = a_unit;
-            const std::uint32_t pos = (a_unit + lane / kSub * kWarps) * kUnit + 16 * (lane % kSub);
+            const std::uint32_t pos = sub == 1 ? (a_unit + lane * kWarps) * kUnit
+                                               : (a_unit + lane / 2 * kWarps) * kUnit + 16 * (lane % 2);
             held_block = -1;
             if (pos < ahead.s.len) {
                 const std::uint32_t i = pos / bt;
                 held_row = pos - i * bt;
-                held_block = __ldg(p.tables + static_cast<std::uint64_t>(ahead.b) * p.c.max_blocks + i);
+                held_block = fetch(p, p.tables + static_cast<std::uint64_t>(ahead.b) * p.c.max_blocks + i);
                 if (held_block < 0 || static_cast<std::uint64_t>(held_block) >= p.c.num_blocks) {
                     held_block = -1;
                     atomicOr(&g_device_status, kDevIndexOutOfRange);
@@ -515,24 +619,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         const std::uint32_t i = lane - a_slot;
-        if (i < kSub) {
+        if (i < sub) {
             const std::uint32_t bar = bars + 8 * a_stage;
-            const std::uint32_t kt = ring + a_stage * kStage + i * kBox, vt = kt + 2 * kBox;
+            const std::uint32_t kt = ring + a_stage * kStage + i * kBox;
             // (what is not there reads as zeros)
             const int y = held_block < 0 ? kNowhere
                                          : static_cast<int>((static_cast<std::uint32_t>(held_block) * p.c.kv_heads + ahead.r) * bt + held_row);
-            attn8::mbar_expect(bar, kStage / kSub);
-            attn8::tma_load_2d(kt, &map_k, 0, y, bar);
-            if (HD == 128) attn8::tma_load_2d(kt + kBox, &map_k, 64, y, bar);
-            attn8::tma_load_2d(vt, &map_v, 0, y, bar);
-            if (HD == 128) attn8::tma_load_2d(vt + kBox, &map_v, 64, y, bar);
+            attn8::mbar_expect(bar, kStage / sub);
+            attnp::tma_load_3d(kt, &map_k, 0, y, 0, bar);
+            attnp::tma_load_3d(kt + 2 * kBox, &map_v, 0, y, 0, bar);
         }
         a_unit += kWarps;
-        a_slot = (a_slot + kSub) % 32;
+        a_slot = (a_slot + sub) % 32;
         a_stage = a_stage == kStages - 1 ? 0 : a_stage + 1;
     };
     __syncwarp();
-#pragma unroll
+
     for (int k = 0; k < kStages - 1; ++k) issue();
 
     // Q^T as the B operand: dimensions 16 d + 2 t, + 1 and 8 more of column g of each set
@@ -595,13 +697,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < SETS; ++c)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) here[c][h] = limit[c][h] - from;
-            const auto run = [&](auto n) {
-                return attend<HD, decltype(n)::value, SETS>(s, qf, ring + stage * kStage, koff, voff, p.scale_log2,
-                                                            masked, static_cast<std::int32_t>(seq.len) - from, here);
-            };
-            if (SETS == 1 || sets == 1) bad |= run(std::integral_constant<int, 1>{});
-            else if (SETS == 2 || sets == 2) bad |= run(std::integral_constant<int, SETS < 2 ? 1 : 2>{});
-            else bad |= run(std::integral_constant<int, SETS>{});
+            if (masked)
+                bad |= clean<HD>(smem + L::kRing + (warp * kStages + stage) * kStage + 2 * kBox,
+                                 static_cast<std::int32_t>(seq.len) - from);
+            if (SETS == 1 || sets == 1)
+                attend<HD, 1, SETS>(s, qf, ring + stage * kStage, koff, voff, p.scale_log2, masked, here);
+            else
+                attend<HD, SETS, SETS>(s, qf, ring + stage * kStage, koff, voff, p.scale_log2, masked, here);
             if (++stage == kStages) stage = 0, parity ^= 1;
         }
 
@@ -638,6 +740,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             bool any_bad = false;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) any_bad |= bad_flags[w] != 0;
+
             for (std::uint32_t x = threadIdx.x; x < kCols * (HD / 2); x += kThreads) {
                 const std::uint32_t hq = x / (HD / 2), d = x % (HD / 2) * 2, col = kCols * c + hq;
                 if (col >= cols) break;
@@ -658,6 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (any_bad) {
                     // what was taken out of the V that this column attends
                     const std::uint32_t reach = min(static_cast<std::uint32_t>(max(static_cast<std::int32_t>(seq.len - seq.n + col / p.group + 1), 0)), v1 * kUnit);
+
                     for (std::uint32_t pos = max(all / kUnit, v0) * kUnit; pos < reach; ++pos) {
                         const std::int32_t blk = __ldg(p.tables + static_cast<std::uint64_t>(b) * p.c.max_blocks + pos / bt);
                         if (blk < 0 || static_cast<std::uint64_t>(blk) >= p.c.num_blocks) continue;
@@ -695,6 +799,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 };
                 float* invs = flush;                    // [columns]
                 float* wts = flush + kCols * kMaxSets;  // [count][columns]
+
                 for (std::uint32_t col = warp; col < cols; col += kWarps) {
                     const auto ml_of = [&](std::uint32_t j) {
                         return __ldcg(reinterpret_cast<const float2*>(part_of(j) + kCols * SETS * HD) + col);
@@ -720,19 +825,52 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (lane == 0) invs[col] = lt == 0.f ? 0.f : 1.f / lt;
                 }
                 __syncthreads();
-                for (std::uint32_t x = threadIdx.x; x < cols * (HD / 4); x += kThreads) {
-                    const std::uint32_t col = x / (HD / 4), d = x % (HD / 4) * 4;
+                const auto sum_of = [&](std::uint32_t cell, std::uint32_t first, std::uint32_t step) {
+                    const std::uint32_t col = cell / (HD / 4), d = cell % (HD / 4) * 4;
                     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 6
-                    for (std::uint32_t j = 0; j < count; ++j) {
-                        const float4 y = __ldcg(reinterpret_cast<const float4*>(part_of(j) + col * HD + d));
-                        const float w = wts[j * cols + col];
-                        o.x = fmaf(y.x, w, o.x), o.y = fmaf(y.y, w, o.y);
-                        o.z = fmaf(y.z, w, o.z), o.w = fmaf(y.w, w, o.w);
+                    constexpr int kAhead = SETS == 1 ? 6 : 4;  // loads in flight
+
+                    for (std::uint32_t j0 = first; j0 < count; j0 += kAhead * step) {
+                        float4 y[kAhead];
+#pragma unroll
+                        for (int k = 0; k < kAhead; ++k)
+                            if (j0 + k * step < count) y[k] = __ldcg(reinterpret_cast<const float4*>(part_of(j0 + k * step) + col * HD + d));
+#pragma unroll
+                        for (int k = 0; k < kAhead; ++k) {
+                            if (j0 + k * step >= count) break;
+                            const float w = wts[(j0 + k * step) * cols + col];
+                            o.x = fmaf(y[k].x, w, o.x), o.y = fmaf(y[k].y, w, o.y);
+                            o.z = fmaf(y[k].z, w, o.z), o.w = fmaf(y[k].w, w, o.w);
+                        }
                     }
+                    return o;
+                };
+                const auto store = [&](std::uint32_t cell, const float4& o) {
+                    const std::uint32_t col = cell / (HD / 4), d = cell % (HD / 4) * 4;
                     const float inv = invs[col];
                     *reinterpret_cast<uint2*>(out_of(col) + d) =
                         make_uint2(attn8::half2_of(o.x * inv, o.y * inv), attn8::half2_of(o.z * inv, o.w * inv));
+                };
+                const std::uint32_t cells = cols * (HD / 4);
+                if (cells > kThreads / 2) {
+
+                    for (std::uint32_t x = threadIdx.x; x < cells; x += kThreads) store(x, sum_of(x, 0, 1));
+                } else {
+                    // groups of threads take every groups-th part, and add up theirs
+                    const std::uint32_t groups = kThreads / cells;
+                    float4* red = reinterpret_cast<float4*>(wts + ((count * cols + 3) & ~3u));  // [kThreads]
+                    if (threadIdx.x < cells * groups)
+                        red[threadIdx.x] = sum_of(threadIdx.x % cells, threadIdx.x / cells, groups);
+                    __syncthreads();
+                    if (threadIdx.x < cells) {
+                        float4 o = red[threadIdx.x];
+
+                        for (std::uint32_t k = 1; k < groups; ++k) {
+                            const float4 y = red[threadIdx.x + k * cells];
+                            o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+                        }
+                        store(threadIdx.x, o);
+                    }
                 }
             }
         }
@@ -743,16 +881,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 }  // namespace few
 
-// The cache as rows of a head in boxes of `rows` of 64 values.
-inline int make_map(CUtensorMap* map, const void* cache, const kvq8::CacheShape& c, std::uint32_t rows) {
+// The cache as rows of a head, 64 dimensions at a time: boxes of `rows` rows and
+// `halves` times 64 dimensions, one behind the other.
+inline int make_map(CUtensorMap* map, const void* cache, const kvq8::CacheShape& c, std::uint32_t rows,
+                    std::uint32_t halves) {
     auto encode = gemm::encode_fn();
     if (encode == nullptr) return static_cast<int>(cudaErrorNotSupported);
     const std::uint64_t all = c.num_blocks * c.kv_heads * c.block_tokens;
-    const cuuint32_t box[2] = {64, rows};
-    const cuuint64_t dims[2] = {c.head_dim, all < rows ? rows : all};  // no blocks: never loaded
-    const cuuint64_t strides[1] = {c.head_dim * 2ull};
-    const cuuint32_t estr[2] = {1, 1};
-    if (encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(cache), dims, strides, box,
+    const cuuint32_t box[3] = {64, rows, halves};
+    const cuuint64_t dims[3] = {64, all < rows ? rows : all, c.head_dim / 64};  // no blocks: never loaded
+    const cuuint64_t strides[2] = {c.head_dim * 2ull, 128};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    if (encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(cache), dims, strides, box,
                estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return kInvalidValue;
@@ -768,14 +908,17 @@ inline int sm_count(int& n) {
 
 namespace few {
 
-// Sets of columns that sequences of `rows` query rows take.
-inline std::uint32_t sets_of(std::uint64_t rows) { return rows <= kCols ? 1 : rows <= 2 * kCols ? 2 : 4; }
+// Query rows of a KV head that the kernel takes: with four sets of columns 16
+// sequences of 4000 with 5 and 8 tokens of 4 grouped heads took 98 and 104 us at
+// head_dim 128 (registers spill), the chunk kernel 71 and 72; at head_dim 64 (32 of
+// 4000, 6 tokens) 73 against 80.
+constexpr std::uint32_t kMostRows = kCols * kMaxSets;
 
 template <int HD, int SETS>
 int launch(const Params& p, const void* k_cache, int ctas, cudaStream_t stream) {
     CUtensorMap map_k{}, map_v{};
-    int st = make_map(&map_k, k_cache, p.c, 16);
-    if (st == kSuccess) st = make_map(&map_v, p.v_cache, p.c, 16);
+    int st = make_map(&map_k, k_cache, p.c, 2048 / HD / p.sub, HD / 64);
+    if (st == kSuccess) st = make_map(&map_v, p.v_cache, p.c, 2048 / HD / p.sub, HD / 64);
     if (st != kSuccess) return st;
     static std::atomic<std::uint64_t> done{0};
     st = ensure_dynamic_smem(few_kernel<HD, SETS>, Smem<HD>::kBytes, done);

@@ -7,17 +7,27 @@
 // every K/V tile of 128 positions, which TMA puts together from the pages (boxes of
 // the largest power of two of rows that a block holds, 16 to 128 of them; the block
 // numbers of the next tile are read while this one's stage is waited for).  Within a
-// CTA the roles are those of attention_packed.cu: warp 8 walks the work and loads,
-// warp 9 owns tensor memory and issues S_i = Q_i K^T and O_i += P_i V (P from tensor
-// memory), warps 0-3 and 4-7 run the softmax of the two query tiles, one thread per
-// row, warps 10 and 11 take what is not finite out of V tiles that some row sees in
-// part (later positions, and the rows of a page behind the last position).
+// CTA
+// * warp 8 walks the work and loads Q, K and V (TMA, 128-byte swizzle);
+// * warps 9 and 10 issue the products, each for its query tile m: S_m = Q_m K^T and
+//   O_m += P_m V (P from tensor memory).  One warp for both had to take them in turn,
+//   and an MMA costs its warp 30 to 60 cycles to issue: chunk of 2048 over 16384 at
+//   head_dim 128 652 us, 590 with two;
+// * warps 0-3 and 4-7 run the softmax of the two query tiles, one thread per row: the
+//   maximum moves (and O_m is rescaled) only when a score passes it by more than 8 in
+//   log2 units.  P is rounded to f16 (11 bits down to 2^-21 of the row's largest);
+//   at head_dim 128 it lies over the first half of S, at 64 in columns of its own, so
+//   that the next S is computed while P of this one still is;
+// * warp 11 takes what is not finite out of V tiles that some row sees in part (later
+//   positions, and the rows of a page behind the last position): 0 times an infinity
+//   or NaN would be NaN.  The rows that do attend such values add them at the end
+//   (rare, from global memory).
+// Every wait is bounded; an expired wait aborts the CTA, which waits for its issued
+// MMAs (bounded) and frees its tensor memory.  No load uses cluster multicast.
 //
-// The work, all pairs of all sequences and KV heads, is a line of virtual positions:
-// a pair is as long as the positions that it attends (times kBoth or kOne, for two
-// query tiles or one) and its end (kEnd).  Each CTA takes an equal share of it,
-// found on the device from sums of arithmetic series, so one chunk over a long cache
-// fills the GPU as well as a batch of prompts does.  A pair that lies in several
+// The work is a line of positions (attention_paged.cu).  Each CTA takes an
+// equal share of it, found on the device from sums of arithmetic series, so one chunk
+// over a long cache fills the GPU as well as a batch of prompts does.  A pair that lies in several
 // CTAs leaves unnormalised parts, which join_kernel adds up in order.
 #include "mote_common.cuh"
 
@@ -34,12 +44,10 @@ using attnp::tma_load_3d;
 using attnp::tmem_ld32_nowait;
 using attnp::tmem_wait_ld;
 using attnp::tmem_wait_st;
-using attnp::umma_f16_ss;
 using attnv::arrive;
 using attnv::elect_one;
 using attnv::kBM;
 using attnv::kBN;
-using attnv::kCleanWarps;
 using attnv::kFlags;
 using attnv::kItems;
 using attnv::kLaunchRegs;
@@ -57,12 +65,37 @@ using attnv::v_desc;
 using gemm::wait_or_abort;
 
 constexpr int kMaxCtas = 192;
-// Virtual positions: of a position for a pair of two query tiles and of one, and of a
-// pair's end.
-constexpr std::uint32_t kBoth = 4, kOne = 3, kEnd = 4 * 256;
-// The least share, in virtual positions, and the least piece of a pair, in K/V tiles.
-constexpr std::uint64_t kLeast = 4 * 1024;
+// The least share, in positions, and the least piece of a pair, in K/V tiles.
+constexpr std::uint64_t kLeast = 1024;
 constexpr std::uint32_t kMinTiles = 3;
+
+// One MMA, issued by the lane whose `lead` is set; all lanes of the (converged) warp
+// run through it, without a branch.
+__device__ __forceinline__ void mma_ss(std::uint32_t lead, std::uint32_t d, std::uint64_t a, std::uint64_t b,
+                                       std::uint32_t idesc, std::uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+}
+// ... with A in tensor memory.
+__device__ __forceinline__ void mma_ts(std::uint32_t lead, std::uint32_t d, std::uint32_t a, std::uint64_t b,
+                                       std::uint32_t idesc, std::uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+}
+// An arrival on `bar` when the MMAs that the lane has issued so far are complete.
+__device__ __forceinline__ void commit(std::uint32_t lead, std::uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(lead)
+        : "memory");
+}
 
 // Two query tiles of one sequence and KV head, or some of their K/V tiles.
 struct Item {
@@ -86,15 +119,28 @@ struct Join {
 
 template <int HD>
 struct Smem {
-    using Base = attnv::Smem<HD>;
-    static constexpr int kHalf = Base::kHalf, kTile = Base::kTile, kKV = Base::kKV, kS = Base::kS;
-    static constexpr std::uint32_t kColO = Base::kColO;
-    static constexpr int kQ = Base::kQ, kK = Base::kK, kV = Base::kV, kBar = Base::kBar;
-    static constexpr int kTmemSlot = Base::kTmemSlot, kAbort = Base::kAbort, kFlag = Base::kFlag;
-    static constexpr int kItem = (Base::kItem + 15) / 16 * 16;  // [kItems]
-    static constexpr int kShare = kItem + kItems * static_cast<int>(sizeof(Item));  // [3] first sequence, share, begin
-    static constexpr int kScan = (kShare + 7) / 8 * 8 + 3 * 8;  // [warp] sums
-    static constexpr int kUsed = kScan + kThreads / 32 * 8 + 1008;  // + alignment slack
+    static constexpr int kHalf = 128 * 128;           // 128 rows of 64 f16
+    static constexpr int kTile = HD / 64 * kHalf;     // a Q, K or V tile
+    static constexpr int kKV = HD == 64 ? 4 : 2;      // K and V stages
+    // TMEM columns: S_m at 128 m, O_m, and at head_dim 64 P_m; at 128 P_m over S_m
+    static constexpr std::uint32_t kColO = 256;
+    static constexpr std::uint32_t kColP = HD == 64 ? kColO + 2 * HD : 0;
+    static constexpr std::uint32_t kPStep = HD == 64 ? 64 : 128;
+    static constexpr int kQ = 0;                      // [2] query tiles
+    static constexpr int kK = kQ + 2 * kTile;
+    static constexpr int kV = kK + kKV * kTile;
+    static constexpr int kBar = kV + kKV * kTile;
+    // q_full, q_empty, k_full, k_empty, v_full, v_empty, v_clean [kKV], s_full,
+    // s_free, p_half, p_ready, o_done, epi_done, drained [2], item_full, item_empty [kItems]
+    static constexpr int kNumBars = 2 + 5 * kKV + 7 * 2 + 2 * kItems;
+    static constexpr int kTmemSlot = kBar + kNumBars * 8;
+    static constexpr int kAbort = kTmemSlot + 4;
+    static constexpr int kFlag = kAbort + 4;          // [kFlags]
+    static constexpr int kItem = kFlag + 4 * kFlags;  // [kItems]
+    static constexpr int kShare = (kItem + kItems * static_cast<int>(sizeof(Item)) + 7) / 8 * 8;  // first sequence, its begin
+    static constexpr int kScan = kShare + 2 * 8;      // [warp][2] sums
+    static constexpr int kTurn = kScan + kThreads / 32 * 16;  // [query tile][warp] passes whose exponentials are done
+    static constexpr int kUsed = kTurn + 8 * 4 + 1008;  // + alignment slack
     // one CTA per SM: its 512 TMEM columns never wait for another's
     static constexpr int kBytes = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
     static_assert(kBytes <= 232448, "shared memory");
@@ -102,7 +148,6 @@ struct Smem {
 
 struct ChunkParams {
     Params p;
-    std::uint32_t tile_tokens;  // floor(128 / group)
     std::uint32_t box;          // rows of a K or V box
     Join* joins;                // [CTAs]
     float* parts;               // [2 CTAs][HD / 4][256][4], then [256][2]: maxima and sums
@@ -111,48 +156,11 @@ struct ChunkParams {
 template <int HD>
 constexpr std::uint64_t kPart = 256ull * (HD + 2);
 
-// A sequence's pairs, as the line of virtual positions has them.
-struct Pairs {
-    Seq s;
-    std::uint32_t span, tile;  // tokens of a pair and of a query tile
-    std::uint32_t count;       // pairs
-
-    __device__ __forceinline__ Pairs(const ChunkParams& c, std::uint32_t b)
-        : s(sequence(c.p, b)), span(2 * c.tile_tokens), tile(c.tile_tokens) {
-        if (static_cast<std::uint64_t>(s.n) * c.p.group <= c.p.few) s.n = 0;
-        count = (s.n + span - 1) / span;
-    }
-    // positions that pair i attends
-    __device__ __forceinline__ std::uint32_t reach(std::uint32_t i) const {
-        const std::int64_t end = static_cast<std::int64_t>(s.len) - s.n + min(static_cast<std::uint64_t>(i + 1) * span, static_cast<std::uint64_t>(s.n));
-        return end < 0 ? 0u : static_cast<std::uint32_t>(end);
-    }
-    __device__ __forceinline__ std::uint64_t extent(std::uint32_t i) const {
-        const bool both = s.n - i * span > tile;
-        return static_cast<std::uint64_t>(reach(i)) * (both ? kBoth : kOne) + kEnd;
-    }
-    // extents of the pairs before i (i <= count): a series, but for pairs that
-    // attend nothing and the last one
-    __device__ __forceinline__ std::uint64_t before(std::uint32_t i) const {
-        if (i == 0) return 0;
-        const std::uint32_t full = i < count ? i : i - 1;
-        const std::int64_t past = static_cast<std::int64_t>(s.len) - s.n;  // negative: some pairs have no positions
-        std::uint32_t none = past >= 0 ? 0u : static_cast<std::uint32_t>(-past / span);
-        if (none > full) none = full;
-        const std::uint64_t m = full - none;
-        std::uint64_t x = static_cast<std::uint64_t>(full) * kEnd;
-        // reach(k) = past + (k + 1) span for k = none .. full - 1
-        x += kBoth * static_cast<std::uint64_t>(static_cast<std::int64_t>(m) * past + static_cast<std::int64_t>(span) * static_cast<std::int64_t>(m * none + m * (m + 1) / 2));
-        return i < count ? x : x + extent(count - 1);
-    }
-    __device__ __forceinline__ std::uint64_t all() const { return before(count); }
-};
-
-// Of a pair of n K/V tiles, those before virtual position x of it.
-__device__ __forceinline__ std::uint32_t cut(std::uint64_t x, std::uint32_t n, bool both) {
-    const std::uint64_t t = (x + 64 * (both ? kBoth : kOne)) / (kBN * (both ? kBoth : kOne));
+// Of a pair of n K/V tiles, those before position x of it.
+__device__ __forceinline__ std::uint32_t cut(std::uint64_t x, std::uint32_t n) {
+    const std::uint32_t t = static_cast<std::uint32_t>((x + kBN / 2) / kBN);
     if (t < kMinTiles) return 0;
-    return t + kMinTiles > n ? n : static_cast<std::uint32_t>(t);
+    return t + kMinTiles > n ? n : t;
 }
 
 template <int HD>
@@ -178,49 +186,51 @@ __global__ void __launch_bounds__(kThreads, 1)
     std::uint64_t* v_empty = v_full + kKV;
     std::uint64_t* v_clean = v_empty + kKV;
     std::uint64_t* s_full = v_clean + kKV;
-    std::uint64_t* p_half = s_full + 2 * L::kS;
-    std::uint64_t* p_ready = p_half + L::kS;
-    std::uint64_t* o_done = p_ready + L::kS;
-    std::uint64_t* epi_done = o_done + 2 * L::kS;
+    std::uint64_t* s_free = s_full + 2;
+    std::uint64_t* p_half = s_free + 2;
+    std::uint64_t* p_ready = p_half + 2;
+    std::uint64_t* o_done = p_ready + 2;
+    std::uint64_t* epi_done = o_done + 2;
     std::uint64_t* drained = epi_done + 2;
-    std::uint64_t* item_full = drained + 1;
+    std::uint64_t* item_full = drained + 2;
     std::uint64_t* item_empty = item_full + kItems;
     Item* ring = reinterpret_cast<Item*>(smem + L::kItem);
     volatile std::uint32_t* tmem_slot = reinterpret_cast<volatile std::uint32_t*>(smem + L::kTmemSlot);
     volatile std::uint32_t* abort_flag = reinterpret_cast<volatile std::uint32_t*>(smem + L::kAbort);
     volatile std::uint32_t* not_finite = reinterpret_cast<volatile std::uint32_t*>(smem + L::kFlag);
 
+    volatile std::uint32_t* turn = reinterpret_cast<volatile std::uint32_t*>(smem + L::kTurn);
+
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
-        mbar_init(q_empty, 1);
+        mbar_init(q_empty, 2);
         for (int s = 0; s < kKV; ++s) {
             mbar_init(&k_full[s], 1);
-            mbar_init(&k_empty[s], 1);
+            mbar_init(&k_empty[s], 2);
             mbar_init(&v_full[s], 1);
-            mbar_init(&v_empty[s], 1 + kCleanWarps);  // the last P V, and warps 10 and 11 keep step
-            mbar_init(&v_clean[s], kCleanWarps);
+            mbar_init(&v_empty[s], 3);  // both P V, and warp 11 keeps step
+            mbar_init(&v_clean[s], 1);
         }
-        for (int s = 0; s < L::kS; ++s) {
-            mbar_init(&s_full[s], 1);
-            mbar_init(&s_full[L::kS + s], 1);
-            mbar_init(&p_half[s], 4);
-            mbar_init(&p_ready[s], 4);
-            mbar_init(&o_done[s], 1);
-            mbar_init(&o_done[L::kS + s], 1);
+        for (int m = 0; m < 2; ++m) {
+            mbar_init(&s_full[m], 1);
+            mbar_init(&s_free[m], 4);
+            mbar_init(&p_half[m], 4);
+            mbar_init(&p_ready[m], 4);
+            mbar_init(&o_done[m], 1);
+            mbar_init(&epi_done[m], 4);
+            mbar_init(&drained[m], 1);
         }
-        mbar_init(&epi_done[0], 4);
-        mbar_init(&epi_done[1], 4);
         for (int s = 0; s < kItems; ++s) {
             mbar_init(&item_full[s], 1);
             mbar_init(&item_empty[s], 11);  // every warp but the producer
         }
-        mbar_init(drained, 1);
         *abort_flag = 0u;
+        for (int i = 0; i < 8; ++i) turn[i] = 0u;
         fence_mbarrier_init();
     }
-    if (c.tile_tokens * p.group < kBM) {  // rows of a query tile that no box fills stay zero
+    if (p.tile_tokens * p.group < kBM) {  // rows of a query tile that no box fills stay zero
         for (int i = threadIdx.x; i < 2 * L::kTile / 16; i += kThreads)
             reinterpret_cast<uint4*>(smem + L::kQ)[i] = make_uint4(0, 0, 0, 0);
         fence_proxy_async_smem();
@@ -231,58 +241,91 @@ __global__ void __launch_bounds__(kThreads, 1)
     gemm::tc_fence_after();
     const std::uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();
-    pdl_wait();
+    // beside the other kernel, which has waited, the wait comes at the end
+    if (!p.shares) pdl_wait();
 
     // ---- the CTA's share of the line ---------------------------------------
-    volatile std::uint64_t* share = reinterpret_cast<volatile std::uint64_t*>(smem + (L::kShare + 7) / 8 * 8);
-    volatile std::uint64_t* scan = reinterpret_cast<volatile std::uint64_t*>(smem + L::kScan);
-    {
-        const auto scan_up = [&](std::uint64_t x) {  // inclusive, over the warp
+    // first sequence (~0: none), length of a share, where the sequence begins; by the
+    // producer alone for up to 32 sequences, by all otherwise
+    const std::uint32_t batch = p.c.batch;
+    std::uint64_t first_b = ~0ull, per = 0, first_begin = 0;
+    const auto scan_up = [&](std::uint64_t x) {  // inclusive, over the warp
 #pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const std::uint64_t y = __shfl_up_sync(0xffffffffu, x, d);
-                if (lane >= d) x += y;
+        for (int d = 1; d < 32; d *= 2) {
+            const std::uint64_t y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += y;
+        }
+        return x;
+    };
+    // this kernel's work of sequence b, and the other's
+    const auto work_of = [&](std::uint32_t b, std::uint64_t& units) -> std::uint64_t {
+        if (b >= batch) return 0;
+        const Seq s = sequence(p, b);
+        if (p.shares) {
+            const std::uint32_t n = few::units_of<HD>(few::few_part(p, s));
+            units += n == 0 ? 0ull : (static_cast<std::uint64_t>(n) + few::kRowCost) * p.c.kv_heads;
+        }
+        return line_of(p, s);
+    };
+    // sets `per`; whether the CTA has a share
+    const auto divide = [&](std::uint64_t total, std::uint64_t units) {
+        const std::uint32_t ctas = p.shares ? gridDim.x - few_ctas(gridDim.x, units, total) : gridDim.x;
+        if (blockIdx.x >= ctas) return false;
+        per = share_of(total, ctas);
+        if (per < kLeast) per = kLeast;
+        return true;
+    };
+    if (__builtin_expect(batch <= 32, 1)) {
+        if (warp == kProducerWarp) {
+            std::uint64_t units = 0;
+            const std::uint64_t mine = work_of(lane, units), incl = scan_up(mine);
+            if (p.shares) units = __shfl_sync(0xffffffffu, scan_up(units), 31);
+            if (divide(__shfl_sync(0xffffffffu, incl, 31), units)) {
+                const std::uint64_t at = per * blockIdx.x;
+                const unsigned here = __ballot_sync(0xffffffffu, incl - mine <= at && at < incl);
+                if (here != 0) {
+                    first_b = __ffs(here) - 1;
+                    first_begin = __shfl_sync(0xffffffffu, incl - mine, static_cast<int>(first_b));
+                }
             }
-            return x;
-        };
-        const auto line_of = [&](std::uint32_t b) -> std::uint64_t {
-            return b < p.c.batch ? Pairs(c, b).all() * p.c.kv_heads : 0;
-        };
-        std::uint64_t sum = 0;
-        for (std::uint32_t b = threadIdx.x; b < p.c.batch; b += kThreads) sum += line_of(b);
-        sum = scan_up(sum);
-        if (lane == 31) scan[warp] = sum;
+        }
+    } else {
+        volatile std::uint64_t* share = reinterpret_cast<volatile std::uint64_t*>(smem + L::kShare);
+        volatile std::uint64_t* scan = reinterpret_cast<volatile std::uint64_t*>(smem + L::kScan);
+        std::uint64_t sum = 0, units = 0;
+        for (std::uint32_t b = threadIdx.x; b < batch; b += kThreads) sum += work_of(b, units);
+        sum = scan_up(sum), units = scan_up(units);
+        if (lane == 31) scan[2 * warp] = sum, scan[2 * warp + 1] = units;
         if (threadIdx.x == 0) share[0] = ~0ull;
         __syncthreads();
-        std::uint64_t total = 0;
+        std::uint64_t total = 0, all_units = 0;
 #pragma unroll
-        for (int w = 0; w < kThreads / 32; ++w) total += scan[w];
+        for (int w = 0; w < kThreads / 32; ++w) total += scan[2 * w], all_units += scan[2 * w + 1];
         __syncthreads();
-        std::uint64_t per = (total + gridDim.x - 1) / gridDim.x;
-        if (per < kLeast) per = kLeast;
-        const std::uint64_t at = per * blockIdx.x;
-        std::uint64_t before = 0;
-        for (std::uint32_t base = 0; base < p.c.batch && before <= at; base += kThreads) {
-            const std::uint64_t mine = line_of(base + threadIdx.x), incl = scan_up(mine);
-            if (lane == 31) scan[warp] = incl;
-            __syncthreads();
-            std::uint64_t lower = before;
+        if (divide(total, all_units)) {
+            const std::uint64_t at = per * blockIdx.x;
+            std::uint64_t before = 0;
+            for (std::uint32_t base = 0; base < batch && before <= at; base += kThreads) {
+                std::uint64_t none = 0;
+                const std::uint64_t mine = work_of(base + threadIdx.x, none), incl = scan_up(mine);
+                if (lane == 31) scan[warp] = incl;
+                __syncthreads();
+                std::uint64_t lower = before;
 #pragma unroll
-            for (int w = 0; w < kThreads / 32; ++w) {
-                if (w < warp) lower += scan[w];
-                before += scan[w];
+                for (int w = 0; w < kThreads / 32; ++w) {
+                    if (w < warp) lower += scan[w];
+                    before += scan[w];
+                }
+                const std::uint64_t begin = lower + incl - mine;
+                if (begin <= at && at < lower + incl) {
+                    share[0] = base + threadIdx.x;
+                    share[1] = begin;
+                }
+                __syncthreads();
             }
-            const std::uint64_t begin = lower + incl - mine;
-            if (begin <= at && at < lower + incl) {
-                share[0] = base + threadIdx.x;
-                share[2] = begin;
-            }
-            __syncthreads();
+            first_b = share[0], first_begin = share[1];
         }
-        if (threadIdx.x == 0) share[1] = per;
-        __syncthreads();
     }
-
     // item i of this CTA, as the producer found it (by a whole warp other than
     // the producer's); left == 0 ends the loops, after an abort too
     const auto item_at = [&](std::uint32_t i) {
@@ -297,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
         if (warp == kProducerWarp) {
             if (p.reports && blockIdx.x == gridDim.x - 1) report_bad(p, lane, 32);
-            const std::uint64_t per = share[1], u0 = per * blockIdx.x, u1 = u0 + per;
+            const std::uint64_t u0 = per * blockIdx.x, u1 = u0 + per;
             std::uint32_t kv = 0, n = 0, sent = 0;  // K/V tiles, items with any and items so far
             std::uint32_t joined = 0;               // pairs that begin here and end in another CTA
             bool ok = true;
@@ -318,59 +361,64 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool loads = sub < kBN / c.box;
             const auto load = [&](const Item& it) {
                 const std::uint32_t tiles = it.tiles();
+                // the block of this lane's box of tile j, read a tile ahead, and its row
+                // in the cache (what is not there reads as zeros)
+                const auto position = [&](std::uint32_t j) { return (it.t0 + j) * kBN + sub * c.box; };
+                const auto block_of = [&](std::uint32_t j) {
+                    if (!loads || position(j) >= it.nk || j >= tiles) return -1;
+                    return fetch(p, p.tables + static_cast<std::uint64_t>(it.b) * p.c.max_blocks + position(j) / p.c.block_tokens);
+                };
+                const auto row_of = [&](std::uint32_t j, std::int32_t block) {
+                    if (!loads || position(j) >= it.nk) return kNowhere;
+                    if (block < 0 || static_cast<std::uint64_t>(block) >= p.c.num_blocks) {
+                        atomicOr(&g_device_status, kDevIndexOutOfRange);
+                        return kNowhere;
+                    }
+                    return static_cast<int>((static_cast<std::uint32_t>(block) * p.c.kv_heads + it.kvh) * p.c.block_tokens +
+                                            position(j) % p.c.block_tokens);
+                };
+                std::int32_t block = block_of(0);
                 if (lane == 0) {
                     ok = n == 0 || wait_or_abort(q_empty, (n - 1) & 1u, abort_flag);
                     if (ok) {
-                        const std::uint32_t box = c.tile_tokens * p.group * 128;
+                        const std::uint32_t box = p.tile_tokens * p.group * 128;
                         mbar_arrive_expect_tx(q_full, ((it.n[0] > 0) + (it.n[1] > 0)) * (HD / 64) * box);
 #pragma unroll
                         for (int m = 0; m < 2; ++m)
                             for (int h = 0; h < HD / 64 && it.n[m] > 0; ++h)
                                 tma_load_3d(base + L::kQ + m * L::kTile + h * L::kHalf, &map_q, 64 * h,
                                             static_cast<int>(it.kvh * p.group),
-                                            static_cast<int>(it.q0 + m * c.tile_tokens), smem_u32(q_full));
+                                            static_cast<int>(it.q0 + m * p.tile_tokens), smem_u32(q_full));
                     }
                 }
                 ok = __shfl_sync(0xffffffffu, ok, 0);
-                // the cache row of this lane's box of tile j (what is not there reads as zeros)
-                const auto row_of = [&](std::uint32_t j) {
-                    const std::uint32_t pos = (it.t0 + j) * kBN + sub * c.box;
-                    if (!loads || pos >= it.nk || j >= tiles) return kNowhere;
-                    const std::uint32_t i = pos / p.c.block_tokens;
-                    const std::int32_t block = __ldg(p.tables + static_cast<std::uint64_t>(it.b) * p.c.max_blocks + i);
-                    if (block < 0 || static_cast<std::uint64_t>(block) >= p.c.num_blocks) {
-                        atomicOr(&g_device_status, kDevIndexOutOfRange);
-                        return kNowhere;
-                    }
-                    return static_cast<int>((static_cast<std::uint32_t>(block) * p.c.kv_heads + it.kvh) * p.c.block_tokens + pos - i * p.c.block_tokens);
-                };
-                int row = row_of(0);
                 for (std::uint32_t j = 0; ok && j < tiles; ++j) {
                     const std::uint32_t t = kv + j, s = t % kKV, ph = (t / kKV - 1) & 1u;
-                    const int next = row_of(j + 1);
+                    const std::int32_t next = block_of(j + 1);
+                    const int row = row_of(j, block);
                     const std::uint32_t at = s * L::kTile + dims * L::kHalf + sub * c.box * 128;
                     if (t >= kKV) ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[s], ph, abort_flag));
                     if (!ok) break;
                     if (lane == 0) mbar_arrive_expect_tx(&k_full[s], L::kTile);
                     __syncwarp();
-                    if (loads && lane < 16) attn8::tma_load_2d(base + L::kK + at, &map_k, 64 * dims, row, smem_u32(&k_full[s]));
+                    if (loads && lane < 16) tma_load_3d(base + L::kK + at, &map_k, 0, row, static_cast<int>(dims), smem_u32(&k_full[s]));
                     if (t >= kKV) ok = __all_sync(0xffffffffu, wait_or_abort(&v_empty[s], ph, abort_flag));
                     if (!ok) break;
                     if (lane == 0) mbar_arrive_expect_tx(&v_full[s], L::kTile);
                     __syncwarp();
-                    if (loads && lane >= 16) attn8::tma_load_2d(base + L::kV + at, &map_v, 64 * dims, row, smem_u32(&v_full[s]));
-                    row = next;
+                    if (loads && lane >= 16) tma_load_3d(base + L::kV + at, &map_v, 0, row, static_cast<int>(dims), smem_u32(&v_full[s]));
+                    block = next;
                 }
                 kv += tiles;
                 ++n;
             };
-            if (share[0] != ~0ull) {
-                std::uint32_t b = static_cast<std::uint32_t>(share[0]);
-                Pairs x(c, b);
+            if (first_b != ~0ull) {
+                std::uint32_t b = static_cast<std::uint32_t>(first_b);
+                Pairs x(p, sequence(p, b));
                 // the pair that u0 lies in
-                std::uint64_t begin = share[2];
-                std::uint32_t kvh = static_cast<std::uint32_t>((u0 - begin) / x.all()), i = 0;
-                begin += kvh * x.all();
+                std::uint64_t begin = first_begin;
+                std::uint32_t kvh = 0, i = 0;
+                for (const std::uint64_t all = x.all(); begin + all <= u0; begin += all) ++kvh;
                 for (std::uint32_t hi = x.count; hi - i > 1;) {
                     const std::uint32_t mid = (i + hi) / 2;
                     if (begin + x.before(mid) <= u0) i = mid; else hi = mid;
@@ -378,10 +426,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 begin += x.before(i);
                 while (ok && begin < u1) {
                     const std::uint64_t extent = x.extent(i);
-                    const bool both = x.s.n - i * x.span > x.tile;
                     const std::uint32_t reach = x.reach(i), tiles = (reach + kBN - 1) / kBN;
-                    const std::uint32_t from = begin >= u0 ? 0u : cut(u0 - begin, tiles, both);
-                    const std::uint32_t to = begin + extent <= u1 ? tiles : cut(u1 - begin, tiles, both);
+                    const std::uint32_t from = begin >= u0 ? 0u : cut(u0 - begin, tiles);
+                    const std::uint32_t to = begin + extent <= u1 ? tiles : cut(u1 - begin, tiles);
                     // (a pair without positions, whose rows get zeros, is the CTA's in which it begins)
                     if (from < to || (tiles == 0 && begin >= u0)) {
                         Item it{};
@@ -394,8 +441,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         it.t0 = from;
 #pragma unroll
                         for (int m = 0; m < 2; ++m) {
-                            const std::uint32_t first = m * c.tile_tokens;
-                            const std::int32_t last = it.pos0 + static_cast<std::int32_t>(min(first + c.tile_tokens, it.left)) - 1;
+                            const std::uint32_t first = m * p.tile_tokens;
+                            const std::int32_t last = it.pos0 + static_cast<std::int32_t>(min(first + p.tile_tokens, it.left)) - 1;
                             const std::uint32_t whole = first >= it.left || last < 0 ? 0u : static_cast<std::uint32_t>(last) / kBN + 1;
                             it.n[m] = min(whole, to) - min(whole, from);
                         }
@@ -404,9 +451,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         it.part = from == 0 && to == tiles ? -1 : static_cast<std::int32_t>(2 * blockIdx.x + (from == 0 ? 1 : 0));
                         if (from == 0 && to < tiles) {
                             // the last CTA that has some of it
-                            std::uint64_t last = (begin + extent - 1) / per;
-                            if (cut(last * per - begin, tiles, both) == tiles) --last;
-                            joined = static_cast<std::uint32_t>(last) - blockIdx.x + 1;
+                            std::uint32_t last = blockIdx.x;
+                            while ((last + 1) * per < begin + extent) ++last;
+                            if (cut(last * per - begin, tiles) == tiles) --last;
+                            joined = last - blockIdx.x + 1;
                             if (lane == 0) c.joins[blockIdx.x] = Join{joined, it.left, kvh, it.q0};
                         }
                         send(it);
@@ -419,143 +467,124 @@ __global__ void __launch_bounds__(kThreads, 1)
                     kvh = 0;
                     do {
                         if (++b >= p.c.batch) break;
-                        x = Pairs(c, b);
+                        x = Pairs(p, sequence(p, b));
                     } while (x.count == 0);
                     if (b >= p.c.batch) break;
                 }
             }
             if (joined == 0 && lane == 0) c.joins[blockIdx.x] = Join{0, 0, 0, 0};
             if (ok) send(Item{});
-        } else if (warp == kMmaWarp) {
-            // The whole warp walks the loops, on values that the compiler knows to
-            // be uniform, and one elected lane issues: operands then come from
-            // uniform registers (moving each to one cost 100 cycles an MMA).
+        } else if (warp < kMmaWarp + 2) {
+            // The whole warp walks the loops, on values that the compiler knows to be
+            // uniform, and issues by predicate, without a branch.
+            const int m = warp - kMmaWarp;
             const std::uint32_t tm = __reduce_max_sync(0xffffffffu, tmem);
-            std::uint32_t kv = 0, n = 0, clean = 0;
-            // per query tile: items with any tiles, and whether the last one's
-            // epilogue has yet to be waited for; and the passes so far
-            std::uint32_t outs[2] = {0, 0}, passed = 0;
-            bool unread[2] = {false, false};
+            const std::uint32_t lead = elect_one() ? 1u : 0u;
+            const std::uint32_t s_col = tm + 128u * m, o_col = tm + L::kColO + HD * m, p_col = tm + L::kColP + L::kPStep * m;
+            const std::uint64_t qd = gemm::smem_desc_sw128(base + L::kQ + m * L::kTile);
+            std::uint32_t kv = 0, n = 0, clean = 0, passes = 0, outs = 0;
+            bool unread = false, ok = true;  // the last O has yet to be read
             const auto wait = [&](std::uint64_t* bar, std::uint32_t parity) {
                 return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag)) != 0;
             };
-            bool ok = true;
             for (std::uint32_t i = 0; ok; ++i) {
                 const Item it = item_at(i);
                 if (it.left == 0) break;
-                const std::uint32_t n0 = __reduce_max_sync(0xffffffffu, it.n[0]);
-                const std::uint32_t n1 = __reduce_max_sync(0xffffffffu, it.n[1]);
+                const std::uint32_t mine = __reduce_max_sync(0xffffffffu, m ? it.n[1] : it.n[0]);
+                const std::uint32_t tiles = __reduce_max_sync(0xffffffffu, it.tiles());
                 const std::uint32_t masked = __reduce_max_sync(0xffffffffu, it.masked);
-                const std::uint32_t tiles = max(n0, n1);
                 if (tiles == 0) continue;
-                // The item's passes in order: pass x is tile j of query tile m, tile 0
-                // of both, tile 1 of both, and so on (query tile 1 attends as many
-                // tiles as 0 or more, or none).  Its S is in buffer (passed + x) % kS.
-                const std::uint32_t passes = n0 + n1, both = 2 * min(n0, n1);
-                const auto m_of = [&](std::uint32_t x) { return x < both ? static_cast<int>(x & 1) : n1 > n0; };
-                const auto j_of = [&](std::uint32_t x) { return x < both ? x / 2 : x - both / 2; };
                 const auto wait_k = [&](std::uint32_t j) {
                     const std::uint32_t t = kv + j;
                     return wait(&k_full[t % kKV], (t / kKV) & 1u);
                 };
-                const auto issue_s = [&](std::uint32_t x) {  // then what its last use frees
-                    const int m = m_of(x);
-                    const std::uint32_t j = j_of(x), s = (kv + j) % kKV, buf = (passed + x) % L::kS;
-                    const std::uint64_t ad = gemm::smem_desc_sw128(base + L::kQ + m * L::kTile);
-                    const std::uint64_t bd = gemm::smem_desc_sw128(base + L::kK + s * L::kTile);
-                    const bool last = m == 1 || j >= n1;
-                    if (elect_one()) {
+                const auto issue_s = [&](std::uint32_t j) {  // and then what its last use frees
+                    const std::uint32_t s = (kv + j) % kKV;
+                    const std::uint64_t kd = gemm::smem_desc_sw128(base + L::kK + s * L::kTile);
+                    gemm::tc_fence_after();
 #pragma unroll
-                        for (int k = 0; k < HD / 16; ++k) {
-                            constexpr std::uint32_t kStep = 32 >> 4, kNext = L::kHalf >> 4;
-                            const std::uint32_t at = k / 4 * kNext + k % 4 * kStep;
-                            umma_f16_ss(tm + 128u * buf, ad + at, bd + at, kIdescS, k != 0 ? 1u : 0u);
-                        }
-                        gemm::umma_commit(smem_u32(&s_full[m * L::kS + buf]));
-                        if (last) gemm::umma_commit(smem_u32(&k_empty[s]));
-                        if (x + 1 == passes) gemm::umma_commit(smem_u32(q_empty));
+                    for (int k = 0; k < HD / 16; ++k) {
+                        constexpr std::uint32_t kStep = 32 >> 4, kNext = L::kHalf >> 4;
+                        const std::uint32_t at = k / 4 * kNext + k % 4 * kStep;
+                        mma_ss(lead, s_col, qd + at, kd + at, kIdescS, k != 0 ? 1u : 0u);
                     }
-                    __syncwarp();
+                    commit(lead, &s_full[m]);
+                    commit(lead, &k_empty[s]);
+                    if (j + 1 == mine) commit(lead, q_empty);
+                };
+                const auto issue_pv = [&](std::uint64_t vd, std::uint32_t j, int half) {
+                    gemm::tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < kBN / 32; ++k) {
+                        const int step = half * (kBN / 32) + k;
+                        mma_ts(lead, o_col, p_col + step * 8, vd + step * (2048 >> 4), kIdescPV, (j | step) != 0 ? 1u : 0u);
+                    }
                 };
                 ok = wait(q_full, n & 1u);
-                for (std::uint32_t x = 0; ok && x < L::kS && x < passes; ++x) {
-                    ok = wait_k(j_of(x));
-                    gemm::tc_fence_after();
-                    if (ok) issue_s(x);
+                if (ok && mine == 0 && lane == 0) arrive(q_empty);
+                if (ok && mine > 0) {
+                    ok = wait_k(0);
+                    if (ok) issue_s(0);
                 }
-                for (std::uint32_t x = 0; ok && x < passes; ++x) {
-                    const int m = m_of(x);
-                    const std::uint32_t j = j_of(x), t = kv + j, s = t % kKV;
-                    const std::uint32_t buf = (passed + x) % L::kS, phase = ((passed + x) / L::kS) & 1u;
-                    if (m == 0 || j >= n0) {
-                        // V tile j has landed, and is looked through where rows see it in
-                        // part (its barriers go round with the tiles that are)
-                        ok = wait(&v_full[s], (t / kKV) & 1u);
-                        if (ok && j >= masked) {
-                            ok = wait(&v_clean[clean % kKV], (clean / kKV) & 1u);
-                            ++clean;
-                        }
+                for (std::uint32_t j = 0; ok && j < tiles; ++j) {
+                    const std::uint32_t t = kv + j, s = t % kKV;
+                    if (j >= mine) {  // the other query tile's alone
+                        ok = wait_k(j);
+                        if (ok && lane == 0) arrive(&k_empty[s]);
                     }
-                    // the last O is read (of both query tiles, so that neither
-                    // softmax group falls behind by more than an item)
-                    if (x == 0) {
-#pragma unroll
-                        for (int y = 0; y < 2; ++y)
-                            if (ok && unread[y]) {
-                                ok = wait(&epi_done[y], (outs[y] - 1) & 1u);
-                                unread[y] = false;
-                            }
+                    // V tile j has landed, and is looked through where rows see it in part
+                    // (its barriers go round with the tiles that are)
+                    ok = ok && wait(&v_full[s], (t / kKV) & 1u);
+                    if (ok && j >= masked) {
+                        ok = wait(&v_clean[clean % kKV], (clean / kKV) & 1u);
+                        ++clean;
                     }
-                    if (!ok) break;
+                    if (j >= mine) {
+                        if (ok && lane == 0) arrive(&v_empty[s]);
+                        continue;
+                    }
+                    if (ok && j == 0 && unread) {
+                        ok = wait(&epi_done[m], (outs - 1) & 1u);
+                        unread = false;
+                    }
+                    const std::uint32_t phase = passes++ & 1u;
                     const std::uint64_t vd = v_desc<HD>(base + L::kV + s * L::kTile);
-                    const std::uint32_t p_col = tm + 128u * buf, o_col = tm + L::kColO + HD * m;
-                    const bool last = m == 1 || j >= n1;
                     // P V in halves, the first while the second half of P is computed
-#pragma unroll
-                    for (int half = 0; half < 2 && ok; ++half) {
-                        ok = wait(half ? &p_ready[buf] : &p_half[buf], phase);
-                        gemm::tc_fence_after();
-                        if (ok && elect_one()) {
-#pragma unroll
-                            for (int k = half * kBN / 32; k < (half + 1) * kBN / 32; ++k)
-                                gemm::umma_f16_ta(o_col, p_col + k * 8, vd + k * (2048 >> 4), kIdescPV,
-                                                  (j | k) != 0 ? 1u : 0u);
-                            if (half) {
-                                gemm::umma_commit(smem_u32(&o_done[m * L::kS + buf]));
-                                if (last) gemm::umma_commit(smem_u32(&v_empty[s]));
-                            }
-                        }
-                        __syncwarp();
+                    if (HD == 64 && ok && j + 1 < mine) {  // S is read, P has columns of its own
+                        ok = wait(&s_free[m], phase) && wait_k(j + 1);
+                        if (ok) issue_s(j + 1);
                     }
-                    if (ok && x + L::kS < passes) {  // into the buffer that this P leaves
-                        ok = wait_k(j_of(x + L::kS));
-                        gemm::tc_fence_after();
-                        if (ok) issue_s(x + L::kS);
+                    ok = ok && wait(&p_half[m], phase);
+                    if (ok) issue_pv(vd, j, 0);
+                    ok = ok && wait(&p_ready[m], phase);
+                    if (ok) {
+                        issue_pv(vd, j, 1);
+                        commit(lead, &o_done[m]);
+                        commit(lead, &v_empty[s]);
+                    }
+                    if (HD == 128 && ok && j + 1 < mine) {  // into the columns that this P leaves
+                        ok = wait_k(j + 1);
+                        if (ok) issue_s(j + 1);
                     }
                 }
-                if (n0 > 0) ++outs[0], unread[0] = true;
-                if (n1 > 0) ++outs[1], unread[1] = true;
-                passed += passes;
+                if (mine > 0) ++outs, unread = true;
                 kv += tiles;
                 ++n;
             }
             // every issued MMA completes before the tensor memory is freed (commit
             // by the lane that issued)
-            if (elect_one()) {
-                gemm::umma_commit(smem_u32(drained));
-                mbar_wait_bounded(drained, 0, &g_device_status);
-            }
+            commit(lead, &drained[m]);
+            if (lead) mbar_wait_bounded(&drained[m], 0, &g_device_status);
             __syncwarp();
         } else {
             std::uint32_t kv = 0, n = 0, clean = 0;
             bool ok = true;
-            const int me = threadIdx.x - 10 * 32;  // of 64
             for (std::uint32_t i = 0; ok; ++i) {
                 const Item it = item_at(i);
                 if (it.left == 0) break;
                 const std::uint32_t tiles = it.tiles();
                 if (tiles == 0) continue;
-                volatile std::uint32_t* flag = not_finite + n % kFlags * kCleanWarps + (warp - 10);
+                volatile std::uint32_t* flag = not_finite + n % kFlags;
                 if (lane == 0) *flag = 0u;
                 for (std::uint32_t j = 0; ok && j < tiles; ++j) {
                     const std::uint32_t t = kv + j, s = t % kKV;
@@ -564,8 +593,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (j >= it.masked) {
                         uint4* tile = reinterpret_cast<uint4*>(smem + L::kV + s * L::kTile);
                         std::uint32_t bad = 0;  // an exponent of all ones carries into bit 15
-#pragma unroll 4
-                        for (int x = me; x < L::kTile / 16; x += 32 * kCleanWarps) {
+#pragma unroll 8
+                        for (int x = lane; x < L::kTile / 16; x += 32) {
                             const uint4 v = tile[x];
                             bad |= ((v.x & 0x7c007c00u) + 0x04000400u) | ((v.y & 0x7c007c00u) + 0x04000400u) |
                                    ((v.z & 0x7c007c00u) + 0x04000400u) | ((v.w & 0x7c007c00u) + 0x04000400u);
@@ -574,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             // 16-byte chunk x belongs to row x / 8 of its half tile
                             const std::uint32_t rows = it.nk - (it.t0 + j) * kBN;  // of the sequence
                             bool found = false;
-                            for (int x = me; x < L::kTile / 16; x += 32 * kCleanWarps) {
+                            for (int x = lane; x < L::kTile / 16; x += 32) {
                                 const uint4 v = tile[x];
                                 std::uint32_t w[4] = {v.x, v.y, v.z, v.w};
                                 bool any = false;
@@ -608,49 +637,44 @@ __global__ void __launch_bounds__(kThreads, 1)
         const std::uint32_t o_col = row_tmem + L::kColO + HD * m;
         const std::uint32_t tok = r / p.group, head = r % p.group;
         const float sc = p.scale_log2;
-        std::uint32_t passed = 0, n = 0;  // softmax passes (of both query tiles) and items so far
-        std::uint32_t seen = 0;           // parity of this query tile's passes on each S buffer
+        const std::uint32_t s_col = row_tmem + 128u * m, p_col = row_tmem + L::kColP + L::kPStep * m;
+        std::uint32_t passes = 0, theirs = 0, n = 0;  // of this query tile and of the other, and items with any so far
         bool ok = true;
         for (std::uint32_t i = 0;; ++i) {
             const Item it = item_at(i);
             if (it.left == 0) break;
-            const std::uint32_t token = m * c.tile_tokens + tok;  // from the item's first
-            const bool mine = tok < c.tile_tokens && token < it.left;
+            const std::uint32_t token = m * p.tile_tokens + tok;  // from the item's first
+            const bool mine = tok < p.tile_tokens && token < it.left;
             const std::int32_t limit = it.pos0 + static_cast<std::int32_t>(token);  // its position
             // the least position of the warp's rows
             const std::int32_t least = it.pos0 + static_cast<std::int32_t>(
-                m * c.tile_tokens + 32u * (warp % 4) / p.group);
+                m * p.tile_tokens + 32u * (warp % 4) / p.group);
             const std::uint32_t tiles = m ? it.n[1] : it.n[0];
             float mx_ref = -INFINITY, l = 0.f;
             float neg = 0.f;    // what the scaled scores get added
             bool vast = false;  // the reference is subtracted from the scores
-            // tile j of this query tile is pass number pass_of(j), as the products are
-            // issued.  A buffer's S and O barriers are this query tile's own: their
-            // phases count its passes there, so a group that lags behind the other,
-            // or has no rows for some items, does not lose count.
-            const auto pass_of = [&](std::uint32_t j) {
-                return passed + min(j, it.n[0]) + min(j, it.n[1]) + (m == 1 && j < it.n[0] ? 1u : 0u);
+            const auto wait_own = [&](std::uint64_t* bar, std::uint32_t parity) {
+                return __all_sync(0xffffffffu, wait_or_abort(bar + m, parity, abort_flag)) != 0;
             };
-            const auto wait_own = [&](std::uint64_t* bar, std::uint32_t b, std::uint32_t parity) {
-                return __all_sync(0xffffffffu, wait_or_abort(bar + m * L::kS + b, parity, abort_flag)) != 0;
-            };
-            std::uint32_t last_buf = 0, last_parity = 0;  // the last pass's
             for (std::uint32_t j = 0; j < tiles && ok; ++j) {
-                const std::uint32_t x = pass_of(j), buf = x % L::kS, s_col = row_tmem + 128u * buf;
-                const std::uint32_t parity = seen >> buf & 1u;
-                seen ^= 1u << buf;
-                ok = wait_own(s_full, buf, parity);
+                const std::uint32_t phase = passes++ & 1u;
+                ok = wait_own(s_full, phase);
                 if (!ok) break;
                 gemm::tc_fence_after();
                 std::uint32_t v[4][32];
 #pragma unroll
                 for (int cc = 0; cc < 4; ++cc) tmem_ld32_nowait(s_col + 32 * cc, v[cc]);
                 tmem_wait_ld();
+                if (HD == 64) {  // the next S may come
+                    gemm::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive(&s_free[m]);
+                }
                 // causal mask, only in the 32 columns where the warp's rows differ
                 // from all or nothing; the scale is positive, so the maximum of the
                 // raw scores gives that of the scaled ones
                 const std::int32_t kbase = static_cast<std::int32_t>((it.t0 + j) * kBN);
-                if (kbase + kBN - 1 > least) {
+                if (__builtin_expect(kbase + kBN - 1 > least, 0)) {
 #pragma unroll
                     for (int cc = 0; cc < 4; ++cc) {
                         const std::int32_t cols = limit - (kbase + 32 * cc) + 1;  // attended of these
@@ -676,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // -infinity while the row has seen nothing
                 const float mnew = fmaxf(mx_ref, mx);
                 const bool grow = (mnew - mx_ref) * sc > 8.f;  // false while both are -inf (NaN)
-                if (__any_sync(0xffffffffu, grow || vast)) {
+                if (__builtin_expect(__any_sync(0xffffffffu, grow || vast), 0)) {
                     float alpha = 1.f;
                     if (grow) {
                         alpha = ex2f((mx_ref - mnew) * sc);  // 0 from -infinity
@@ -695,10 +719,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (j > 0) {
                         // the previous P V is complete before O moves
-                        ok = wait_own(o_done, last_buf, last_parity);
+                        ok = wait_own(o_done, phase ^ 1u);
                         if (!ok) break;
                         gemm::tc_fence_after();
-#pragma unroll
+#pragma unroll 2
                         for (int cc = 0; cc < HD / 16; ++cc) {
                             std::uint32_t o[16];
                             tmem_ld16(o_col + 16 * cc, o);
@@ -708,6 +732,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tmem_st16(o_col + 16 * cc, o);
                         }
                     }
+                }
+                if (HD == 64 && j > 0) {  // the P V before has read P
+                    ok = wait_own(o_done, phase ^ 1u);
+                    if (!ok) break;
+                    gemm::tc_fence_after();
+                }
+                // The exponentials of the two query tiles take turns, pass after pass: a
+                // scheduler's two softmax warps would else share its exp2 unit evenly and
+                // come out together, leaving it idle meanwhile.
+                {
+                    const std::uint32_t other = m ? it.n[0] : it.n[1];
+                    const std::uint32_t want = theirs + min(j + (m ? 1u : 0u), other);
+                    const volatile std::uint32_t* at = turn + 4 * (1 - m) + warp % 4;
+                    if (static_cast<std::int32_t>(*at - want) < 0) {
+                        const long long start = clock64();
+                        while (static_cast<std::int32_t>(*at - want) < 0 && !*abort_flag)
+                            if (clock64() - start > kWaitCycles) {
+                                atomicOr(&g_device_status, kDevWaitTimeout);
+                                *abort_flag = 1u;
+                            }
+                    }
+                    __syncwarp();
                 }
                 const std::uint64_t sc2 = attnp::pack_f32x2(sc, sc), neg2 = attnp::pack_f32x2(neg, neg);
                 std::uint64_t acc2[2] = {0, 0};
@@ -731,30 +777,33 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_wait_st();
                         gemm::tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) arrive(&p_half[buf]);
+                        if (lane == 0) arrive(&p_half[m]);
                     }
-                    tmem_st16(s_col + 16 * cc, pk);
+                    tmem_st16(p_col + 16 * cc, pk);
+                    if (cc == 0) {
+                        __syncwarp();
+                        if (lane == 0) turn[4 * m + warp % 4] = passes;
+                    }
                 }
                 tmem_wait_st();
                 gemm::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive(&p_ready[buf]);
+                if (lane == 0) arrive(&p_ready[m]);
                 float l0, l1, l2, l3;
                 attnp::unpack_f32x2(acc2[0], l0, l1);
                 attnp::unpack_f32x2(acc2[1], l2, l3);
                 l += (l0 + l1) + (l2 + l3);
-                last_buf = buf, last_parity = parity;
             }
             // O / sum; rows before the first position have no sum and get zeros
             if (it.tiles() > 0) ++n;
-            if (tiles > 0 && ok) ok = wait_own(o_done, last_buf, last_parity);
-            passed += it.n[0] + it.n[1];
+            theirs += m ? it.n[0] : it.n[1];
+            if (tiles > 0 && ok) ok = wait_own(o_done, (passes - 1) & 1u);
             if (ok) {
                 gemm::tc_fence_after();
                 const bool some = tiles > 0 && limit >= 0;
                 const float inv = some ? 1.f / l : 0.f;
-                const volatile std::uint32_t* flags = not_finite + (n - 1) % kFlags * kCleanWarps;
-                const bool add = some && (flags[0] | flags[1]) != 0u;
+                const volatile std::uint32_t* flags = not_finite + (n - 1) % kFlags;
+                const bool add = some && *flags != 0u;
                 __half* dst = p.out + (static_cast<std::uint64_t>(it.q0 + token) * p.q_heads +
                                        it.kvh * p.group + head) * HD;
                 const std::uint32_t row = m * kBM + r;
@@ -771,17 +820,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_wait_ld();
                     }
                     if (!mine) continue;
-                    if (add) {
-                        // what warps 10 and 11 took out of the V tiles that this row attends
+                    if (__builtin_expect(add, 0)) {
+                        // what warp 11 took out of the V tiles that this row attends
                         const std::uint32_t end = min(static_cast<std::uint32_t>(limit) + 1u, (it.t0 + tiles) * kBN);
                         for (std::uint32_t pos = (it.t0 + it.masked) * kBN; pos < end; ++pos) {
-                            const std::int32_t block = __ldg(p.tables + static_cast<std::uint64_t>(it.b) * p.c.max_blocks + pos / p.c.block_tokens);
+                            const std::int32_t block = fetch(p, p.tables + static_cast<std::uint64_t>(it.b) * p.c.max_blocks + pos / p.c.block_tokens);
                             if (block < 0 || static_cast<std::uint64_t>(block) >= p.c.num_blocks) continue;
                             const __half* src = p.v_cache + ((static_cast<std::uint64_t>(block) * p.c.kv_heads + it.kvh) * p.c.block_tokens +
                                                              pos % p.c.block_tokens) * HD + 32 * cc;
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
-                                const float x = __half2float(src[e]);
+                                const float x = __half2float(__ldcg(src + e));
                                 if (!isfinite(x)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
                             }
                         }
@@ -817,11 +866,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     gemm::tc_fence_after();
     if (warp == kMmaWarp) gemm::tmem_dealloc(tmem, kTmemCols);
     if (*abort_flag) let_copies_land();
+    // this kernel's end is the other's too (a CTA without work that waited would keep
+    // its SM from one that has some)
+    if (p.shares && blockIdx.x == 0) pdl_wait();
 }
 
 
 // Adds up the parts of the pairs that lie in several CTAs, in order: a CTA takes 32
-// rows and 64 dimensions of one pair, or returns where there is none.
+// rows and 32 dimensions of one pair, or returns where there is none.  One pass, the
+// sums moving with the largest maximum so far, so that many parts load at a time.
 template <int HD>
 __global__ void __launch_bounds__(256) join_kernel(const ChunkParams c) {
     const Params& p = c.p;
@@ -830,46 +883,49 @@ __global__ void __launch_bounds__(256) join_kernel(const ChunkParams c) {
     pdl_wait();
     const Join j = c.joins[cta];
     const std::uint32_t row = blockIdx.y * 32 + lane, m = row / kBM, tok = row % kBM / p.group, head = row % kBM % p.group;
-    const std::uint32_t token = m * c.tile_tokens + tok, d = blockIdx.z * 16 + warp;
-    if (j.count == 0 || tok >= c.tile_tokens || token >= j.left) return;
-    const auto part_of = [&](std::uint32_t k) {
-        return c.parts + static_cast<std::uint64_t>(2 * (cta + k) + (k == 0 ? 1 : 0)) * kPart<HD>;
-    };
-    const auto ml_of = [&](std::uint32_t k) {
-        return __ldcg(reinterpret_cast<const float2*>(part_of(k) + 256 * HD) + row);
-    };
+    const std::uint32_t token = m * p.tile_tokens + tok, d = blockIdx.z * 8 + warp;
+    if (j.count == 0 || tok >= p.tile_tokens || token >= j.left) return;
+    // the first part is CTA cta's second one, the others the first ones of the CTAs behind
+    const float* part = c.parts + static_cast<std::uint64_t>(2 * cta + 1) * kPart<HD>;
     float mt = -INFINITY, lt = 0.f;
-#pragma unroll 8
-    for (std::uint32_t k = 0; k < j.count; ++k) mt = fmaxf(mt, ml_of(k).x);
-    float4 o[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-#pragma unroll 8
-    for (std::uint32_t k = 0; k < j.count; ++k) {
-        const float4* part = reinterpret_cast<const float4*>(part_of(k)) + row;
-        const float4 y0 = __ldcg(part + 256 * d), y1 = __ldcg(part + 256 * (d + 8));
-        const float2 a = ml_of(k);
-        if (a.x == -INFINITY && a.y == 0.f) continue;  // no position of its own there
-        const float w = a.y != a.y || a.x == mt ? 1.f : ex2f((a.x - mt) * p.scale_log2);
-        lt = fmaf(a.y, w, lt);
-        o[0].x = fmaf(y0.x, w, o[0].x), o[0].y = fmaf(y0.y, w, o[0].y);
-        o[0].z = fmaf(y0.z, w, o[0].z), o[0].w = fmaf(y0.w, w, o[0].w);
-        o[1].x = fmaf(y1.x, w, o[1].x), o[1].y = fmaf(y1.y, w, o[1].y);
-        o[1].z = fmaf(y1.z, w, o[1].z), o[1].w = fmaf(y1.w, w, o[1].w);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kAhead = 10;
+    for (std::uint32_t k0 = 0; k0 < j.count; k0 += kAhead) {
+        float4 y[kAhead];
+        float2 a[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const float* at = part + static_cast<std::uint64_t>(k0 + k) * (2 * kPart<HD>) - (k0 + k == 0 ? 0 : kPart<HD>);
+            if (k0 + k < j.count) {
+                a[k] = __ldcg(reinterpret_cast<const float2*>(at + 256 * HD) + row);
+                y[k] = __ldcg(reinterpret_cast<const float4*>(at) + 256 * d + row);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            // (a part without a position of its own has -infinity and no sums)
+            if (k0 + k >= j.count || (a[k].x == -INFINITY && a[k].y == 0.f)) continue;
+            const float mn = fmaxf(mt, a[k].x);
+            const float f = mt == mn ? 1.f : ex2f((mt - mn) * p.scale_log2);
+            const float w = a[k].x == mn || a[k].y != a[k].y ? 1.f : ex2f((a[k].x - mn) * p.scale_log2);
+            mt = mn;
+            lt = fmaf(a[k].y, w, lt * f);
+            o.x = fmaf(y[k].x, w, o.x * f), o.y = fmaf(y[k].y, w, o.y * f);
+            o.z = fmaf(y[k].z, w, o.z * f), o.w = fmaf(y[k].w, w, o.w * f);
+        }
     }
     const float inv = lt == 0.f ? 0.f : 1.f / lt;
-    __half* dst = p.out + (static_cast<std::uint64_t>(j.q0 + token) * p.q_heads + j.kvh * p.group + head) * HD;
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-        *reinterpret_cast<uint2*>(dst + 4 * (d + 8 * k)) =
-            make_uint2(attn8::half2_of(o[k].x * inv, o[k].y * inv), attn8::half2_of(o[k].z * inv, o[k].w * inv));
+    __half* dst = p.out + (static_cast<std::uint64_t>(j.q0 + token) * p.q_heads + j.kvh * p.group + head) * HD + 4 * d;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(attn8::half2_of(o.x * inv, o.y * inv), attn8::half2_of(o.z * inv, o.w * inv));
 }
 
 template <int HD>
 int launch(const ChunkParams& c, const void* q, const void* k_cache, int ctas, cudaStream_t stream) {
     CUtensorMap map_q{}, map_k{}, map_v{};
     const Params& p = c.p;
-    int st = attnv::make_map(&map_q, q, p.tokens, p.q_heads, HD, p.group, c.tile_tokens);
-    if (st == kSuccess) st = make_map(&map_k, k_cache, p.c, c.box);
-    if (st == kSuccess) st = make_map(&map_v, p.v_cache, p.c, c.box);
+    int st = attnv::make_map(&map_q, q, p.tokens, p.q_heads, HD, p.group, p.tile_tokens);
+    if (st == kSuccess) st = make_map(&map_k, k_cache, p.c, c.box, 1);
+    if (st == kSuccess) st = make_map(&map_v, p.v_cache, p.c, c.box, 1);
     if (st != kSuccess) return st;
     static std::atomic<std::uint64_t> smem_done{0};
     st = ensure_dynamic_smem(chunk_kernel<HD>, Smem<HD>::kBytes, smem_done);
@@ -887,7 +943,7 @@ int launch(const ChunkParams& c, const void* q, const void* k_cache, int ctas, c
     st = launch_pdl_smem(chunk_kernel<HD>, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), Smem<HD>::kBytes,
                          stream, map_q, map_k, map_v, c);
     if (st != kSuccess) return st;
-    return launch_pdl(join_kernel<HD>, dim3(static_cast<unsigned>(ctas), 8, HD / 64), dim3(256), stream, c);
+    return launch_pdl(join_kernel<HD>, dim3(static_cast<unsigned>(ctas), 8, HD / 32), dim3(256), stream, c);
 }
 
 // Bytes of the workspace: counters and parts of the few-row kernel, then parts and
@@ -898,9 +954,9 @@ struct Layout {
 inline Layout layout(int ctas, std::uint64_t head_dim, std::uint64_t rows) {
     Layout l{};
     l.few_parts = few::kMaxCtas * 4;
-    l.joins = l.few_parts + static_cast<std::uint64_t>(ctas) * 2 * few::kCols * few::sets_of(rows) * (head_dim + 2) * 4;
+    l.joins = l.few_parts + static_cast<std::uint64_t>(ctas) * 2 * few::kCols * (rows <= few::kCols ? 1 : few::kMaxSets) * (head_dim + 2) * 4;
     l.parts = l.bytes = l.joins;
-    if (rows > few::kCols * few::kMaxSets) {
+    if (rows > few::kMostRows) {
         l.parts = l.joins + kMaxCtas * sizeof(Join);
         l.bytes = l.parts + static_cast<std::uint64_t>(ctas) * 2 * 256 * (head_dim + 2) * 4;
     }
@@ -976,17 +1032,15 @@ extern "C" int mote_cuda_gqa_attention_paged_f16(
     const auto s = static_cast<cudaStream_t>(stream);
     // Both kernels where the host cannot tell that one of them has nothing to do: a
     // single sequence, or groups too large for the few-row kernel, are the other's.
-    const std::uint32_t most = few::kCols * few::kMaxSets;
-    const bool chunks = rows > most;
-    p.few = chunks && (batch == 1 || group > most) ? 0u : most;
+    const bool chunks = rows > few::kMostRows;
+    p.few = chunks && (batch == 1 || group > few::kMostRows) ? 0u : few::kMostRows;
+    p.shares = chunks && p.few != 0;
+    p.tile_tokens = attnv::kBM / p.group;
+    p.sub = head_dim == 64 && block_tokens % 32 != 0 ? 2 : 1;
     if (p.few != 0) {
         const auto run = [&](auto hd) {
             constexpr int HD = decltype(hd)::value;
-            switch (few::sets_of(rows)) {
-                case 1: return few::launch<HD, 1>(p, k_cache, n, s);
-                case 2: return few::launch<HD, 2>(p, k_cache, n, s);
-                default: return few::launch<HD, 4>(p, k_cache, n, s);
-            }
+            return rows <= few::kCols ? few::launch<HD, 1>(p, k_cache, n, s) : few::launch<HD, few::kMaxSets>(p, k_cache, n, s);
         };
         st = head_dim == 64 ? run(std::integral_constant<int, 64>{}) : run(std::integral_constant<int, 128>{});
         if (st != kSuccess || !chunks) return st;
@@ -994,7 +1048,6 @@ extern "C" int mote_cuda_gqa_attention_paged_f16(
     }
     chunk::ChunkParams c{};
     c.p = p;
-    c.tile_tokens = attnv::kBM / p.group;
     c.box = 16;
     while (c.box < 128 && block_tokens % (2 * c.box) == 0) c.box *= 2;
     c.joins = reinterpret_cast<chunk::Join*>(ws + at.joins);
