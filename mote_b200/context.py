@@ -320,13 +320,25 @@ class CudaContext:
 
     def paged_workspace_bytes(self, q_heads: int, kv_heads: int, head_dim: int,
                               max_new: int) -> int:
-        """mote_cuda_gqa_attention_paged_f16_workspace_bytes on this context's
-        device."""
+        """mote_cuda_gqa_attention_paged_f16_workspace_bytes of a call that has
+        work, memoised by what it depends on: head_dim, this context's device
+        and whether a sequence may have more than 8 and than 16 query rows of a
+        KV head."""
+        rows = max_new * (q_heads // kv_heads) if kv_heads else 0
+        key = (head_dim, (rows > 8) + (rows > 16))
+        try:
+            return self._paged_need[key]
+        except AttributeError:
+            self._paged_need = {}
+        except KeyError:
+            pass
         out = ctypes.c_uint64(0)
         self.inner.select()
         errors.check(lib().mote_cuda_gqa_attention_paged_f16_workspace_bytes(
             q_heads, kv_heads, head_dim, max_new, ctypes.byref(out)),
             "query paged attention workspace")
+        if out.value:  # 0: shapes that the call refuses
+            self._paged_need[key] = out.value
         return out.value
 
     def paged_workspace(self, nbytes: int) -> tuple[int, int]:
@@ -335,8 +347,11 @@ class CudaContext:
         held = self.__dict__.setdefault("_paged_workspaces", [])
         if not held or held[-1].size_bytes < nbytes:
             self.sync()
-            size = max(int(nbytes), 1 << 20)
-            held.append(CudaStorage(self.inner, size, np.zeros(size, np.uint8)))
+            ws = CudaStorage(self.inner, max(int(nbytes), 1 << 20))
+            errors.check(lib().mote_cuda_memset_async(ws.pointer, 0, ws.size_bytes, self.stream),
+                         "clear paged attention workspace")
+            self.sync()
+            held.append(ws)
         return held[-1].pointer, held[-1].size_bytes
 
     def read_bytes(self, tensor: Tensor) -> bytes:

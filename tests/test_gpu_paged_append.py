@@ -105,6 +105,23 @@ def test_rows_behind_the_last_sequence_are_left(ctx):
     same(run(ctx, t), expected(t))
 
 
+def test_rows_before_the_first_sequence_are_left(ctx):
+    t = inputs([3, 18], [0, 40], 4, 2, 64, 32, 16, seed=13)
+    want = expected(t)
+    q0, t["q_out"] = t["q_out"], np.concatenate([t["q_out"][:4], t["q_out"]])
+    for n in ("qkv", "cos", "sin"):
+        t[n] = np.concatenate([t[n][:4], t[n]])
+    t["starts"] = t["starts"] + 4
+    q, k, v = run(ctx, t)
+    same((q[:4], q[4:], k, v), (q0[:4], *want))
+
+
+@pytest.mark.parametrize("batch", [33, 700])
+def test_many_sequences(ctx, batch):
+    t = inputs([i % 4 for i in range(batch)], [(7 * i) % 50 for i in range(batch)], 4, 2, 64, 32, 16, seed=batch)
+    same(run(ctx, t), expected(t))
+
+
 def test_empty_sequences_everywhere(ctx):
     t = inputs([0, 0, 4, 0, 0, 1, 0], [0, 9, 0, 3, 0, 20, 1], 4, 2, 64, 32, 16, seed=9)
     same(run(ctx, t), expected(t))

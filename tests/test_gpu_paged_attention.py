@@ -260,6 +260,85 @@ def test_blocks_out_of_range_read_as_zeros(ctx, number, new):
     check_attention(got, want, mag)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("batch,kinds", [(45, (1, 50)), (300, (1, 2, 9)), (700, (1, 0, 17)), (1000, (1,))])
+def test_many_sequences(ctx, hd, batch, kinds):
+    """More sequences than a warp's lanes, than a CTA's threads; of both kernels."""
+    new = [kinds[i % len(kinds)] for i in range(batch)]
+    verify(ctx, inputs(new, [(37 * i) % 130 for i in range(batch)], 4, 2, hd, 16, seed=batch))
+
+
+@pytest.mark.parametrize("new", [[1, 1], [40, 1], [70, 90]])
+def test_rows_before_the_first_sequence_keep_their_values(ctx, new):
+    t = inputs(new, [30, 9], 8, 2, 64, 16, seed=2, unused=0)
+    want, mag = expected(t)
+    t["q"] = np.concatenate([np.repeat(t["q"][:1], 5, 0), t["q"]])
+    t["starts"] = t["starts"] + 5
+    got = run(ctx, t, max(new))
+    assert (got[:5] == 7.0).all()
+    check_attention(got[5:], want, mag)
+
+
+@pytest.mark.parametrize("new", [[1], [3], [90]])
+def test_a_query_of_nan_or_infinity_is_its_own(ctx, new):
+    t = inputs(new, [200], 8, 2, 64, 16, seed=3, unused=0)
+    want, mag = expected(t)
+    t["q"][0, 1], t["q"][0, 6, 3] = np.nan, np.inf
+    got = run(ctx, t).copy()
+    assert np.isnan(got[0, 1]).all() and np.isnan(got[0, 6]).any()
+    for name in (got, want, mag):
+        name[0, [1, 6]] = 0
+    check_attention(got, want, mag)
+
+
+def test_offsets_past_32_bits(ctx):
+    """Caches of more than 2^32 values: rows in the last blocks."""
+    kvh, block, hd = 8, 256, 128
+    blocks = (1 << 32) // (kvh * block * hd) + 5
+    cache = [ctx.empty(plain((blocks, kvh, block, hd), DType.F16)) for _ in range(2)]
+    rng = np.random.default_rng(4)
+    for new, qh in (([300, 270], 16), ([1, 1], 16), ([40, 1], 16)):
+        tokens, total = sum(new), 300
+        t = {"qkv": rng.normal(0, 1, (600, qh + 2 * kvh, hd)).astype(np.float16),
+             "cos": np.ones((600, 64), np.float32), "sin": np.zeros((600, 64), np.float32),
+             "q_out": np.zeros((600, qh, hd), np.float16)}
+        table = np.array([[blocks - 1, blocks - 4], [blocks - 2, blocks - 3]], np.int32)
+        lens = np.array([total, total], np.int32)
+        held = {n: put(ctx, a) for n, a in t.items()}
+        tb, ln = put(ctx, table), put(ctx, lens)
+        ops.rope_kv_cache_append_paged_f16(ctx, held["qkv"], held["cos"], held["sin"], held["q_out"],
+                                           *cache, tb, put(ctx, np.array([0, 300, 600], np.int32)), ln)
+        starts = ref.starts_of(new)
+        q = rng.normal(0, 1, (tokens, qh, hd)).astype(np.float16)
+        out = put(ctx, np.zeros(q.shape, np.float16))
+        ops.gqa_attention_paged_f16(ctx, put(ctx, q), *cache, tb, put(ctx, starts), ln, out, max(new))
+        got = get(ctx, out)
+        for b in range(2):
+            k, v = (t["qkv"][300 * b:300 * b + 300, qh + i * kvh:qh + (i + 1) * kvh] for i in range(2))
+            rows = slice(starts[b], starts[b + 1])
+            want, mag = _q8_cache.attention(q[rows], k, v, total - new[b] + 1 + np.arange(new[b]),
+                                            1 / math.sqrt(hd))
+            check_attention(got[rows], want, mag)
+    assert ctx.device_status() == 0
+
+
+def test_calls_of_two_contexts_at_once(ctx):
+    """Two contexts' streams run the operators side by side."""
+    cases = []
+    for c in (ctx, CudaContext(0)):
+        for new, past in (([61, 1], [3000, 900]), ([1] * 7, [4000, 1, 90, 700, 0, 33, 2000])):
+            t = inputs(new, past, 8, 2, 128, 32, seed=len(new), unused=0)
+            cases.append((c, t, hold(c, t), max(new)))
+            launch(c, cases[-1][2], max(new))
+    for _ in range(20):
+        for c, _, held, most in cases:
+            launch(c, held, most)
+    for c, t, held, _ in cases:
+        want, mag = expected(t)
+        check_attention(get(c, held["out"]), want, mag)
+        assert c.device_status() == 0
+
+
 def test_graphs_that_share_the_workspace_take_turns(ctx):
     """Captured calls of several shapes and eager ones use one workspace, one
     after another; lengths are advanced between replays."""

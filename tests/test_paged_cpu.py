@@ -169,3 +169,52 @@ def test_axes_wrapper():
         run(_Context(), pos, cos, sin, (16, 49, -1))
     with pytest.raises(errors.AliasedStorage):
         run(_Context(), pos, cos, cos, (16, 24, 24))
+
+
+def test_workspace_size_is_kept_by_what_it_depends_on(monkeypatch):
+    """head_dim and the class of query rows, not the calls' sizes; a call that is
+    refused leaves nothing behind."""
+    import ctypes
+
+    from mote_b200 import context
+
+    asked = []
+
+    class _Lib:
+        @staticmethod
+        def mote_cuda_gqa_attention_paged_f16_workspace_bytes(qh, kvh, hd, most, out):
+            rows = most * (qh // kvh) if kvh else 0
+            asked.append((hd, rows))
+            ctypes.cast(out, ctypes.POINTER(ctypes.c_uint64))[0] = \
+                (1000 * hd + (rows > 8) + (rows > 16)) if kvh and hd in (64, 128) else 0
+            return 0
+
+    class _Inner:
+        def select(self):
+            pass
+
+    monkeypatch.setattr(context, "lib", lambda: _Lib)
+    c = context.CudaContext.__new__(context.CudaContext)
+    c.inner = _Inner()
+    assert c.paged_workspace_bytes(8, 0, 64, 1) == 0
+    assert c.paged_workspace_bytes(8, 2, 96, 1) == 0
+    for most in range(1, 300):
+        assert c.paged_workspace_bytes(8, 2, 64, most) == 64000 + (most > 2) + (most > 4)
+        assert c.paged_workspace_bytes(32, 2, 128, most) == 128000 + 1 + (most > 1)
+    assert len(c._paged_need) == 5 and len(asked) == 7
+
+
+def test_workspace_size_follows_its_classes(lib):
+    """The library's own sizes change at 8 and at 16 query rows and nowhere else
+    (without a device every call fails alike)."""
+    import ctypes
+
+    def size(qh, kvh, hd, most):
+        out = ctypes.c_uint64(0)
+        status = lib.mote_cuda_gqa_attention_paged_f16_workspace_bytes(qh, kvh, hd, most, ctypes.byref(out))
+        return status, out.value
+
+    for hd in (64, 128):
+        for a, b in (((8, 2, 1), (8, 2, 2)), ((8, 2, 3), (16, 1, 1)), ((8, 2, 5), (128, 1, 900))):
+            assert size(a[0], a[1], hd, a[2]) == size(b[0], b[1], hd, b[2])
+    assert size(0, 2, 64, 1) == (0, 0) and size(8, 0, 64, 1) == (0, 0) and size(8, 2, 96, 1) == (0, 0)
