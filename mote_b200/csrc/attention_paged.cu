@@ -691,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();  // the unit has landed; the stage before it is read by all lanes
             if (waiting) issue();  // (a stage whose copies are late gets no more)
             const std::int32_t from = static_cast<std::int32_t>(v * kUnit);
-            const bool masked = from + kUnit > static_cast<std::int32_t>(all);
+            const bool masked = v * kUnit + kUnit > all;  // (up to 2^31)
             std::int32_t here[SETS][2];
 #pragma unroll
             for (int c = 0; c < SETS; ++c)
@@ -717,6 +717,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (row.begin < u1) load_q(row);
         bad = __any_sync(0xffffffffu, bad);
         if (lane == 0) bad_flags[warp] = bad;
+        // what a column's sum of weights divides by; nothing attended: zeros
+        const auto inverse = [&](float sum, std::uint32_t col) {
+            return seq.len + col / p.group < seq.n ? 0.f : 1.f / sum;
+        };
         const auto out_of = [&](std::uint32_t col) {
             const std::uint32_t i = col / p.group, h = col - i * p.group;
             return p.out + ((static_cast<std::uint64_t>(seq.q0) + i) * p.q_heads + kvh * p.group + h) * HD;
@@ -772,7 +776,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 if (whole) {
-                    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+                    const float inv = inverse(lt, col);
                     *reinterpret_cast<std::uint32_t*>(out_of(col) + d) = attn8::half2_of(o.x * inv, o.y * inv);
                 } else {
                     *reinterpret_cast<float2*>(part + col * HD + d) = o;
@@ -822,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
 #pragma unroll
                     for (int d = 16; d > 0; d /= 2) lt += __shfl_xor_sync(0xffffffffu, lt, d);
-                    if (lane == 0) invs[col] = lt == 0.f ? 0.f : 1.f / lt;
+                    if (lane == 0) invs[col] = inverse(lt, col);
                 }
                 __syncthreads();
                 const auto sum_of = [&](std::uint32_t cell, std::uint32_t first, std::uint32_t step) {

@@ -115,6 +115,7 @@ struct Item {
 // whose number the entry has (0: none).
 struct Join {
     std::uint32_t count, left, kvh, q0;
+    std::int32_t pos0;
 };
 
 template <int HD>
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             while ((last + 1) * per < begin + extent) ++last;
                             if (cut(last * per - begin, tiles) == tiles) --last;
                             joined = last - blockIdx.x + 1;
-                            if (lane == 0) c.joins[blockIdx.x] = Join{joined, it.left, kvh, it.q0};
+                            if (lane == 0) c.joins[blockIdx.x] = Join{joined, it.left, kvh, it.q0, it.pos0};
                         }
                         send(it);
                         if (ok && it.tiles() > 0) load(it);
@@ -472,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (b >= p.c.batch) break;
                 }
             }
-            if (joined == 0 && lane == 0) c.joins[blockIdx.x] = Join{0, 0, 0, 0};
+            if (joined == 0 && lane == 0) c.joins[blockIdx.x] = Join{};
             if (ok) send(Item{});
         } else if (warp < kMmaWarp + 2) {
             // The whole warp walks the loops, on values that the compiler knows to be
@@ -914,7 +915,7 @@ __global__ void __launch_bounds__(256) join_kernel(const ChunkParams c) {
             o.z = fmaf(y[k].z, w, o.z * f), o.w = fmaf(y[k].w, w, o.w * f);
         }
     }
-    const float inv = lt == 0.f ? 0.f : 1.f / lt;
+    const float inv = j.pos0 + static_cast<std::int32_t>(token) < 0 ? 0.f : 1.f / lt;  // nothing attended: zeros
     __half* dst = p.out + (static_cast<std::uint64_t>(j.q0 + token) * p.q_heads + j.kvh * p.group + head) * HD + 4 * d;
     *reinterpret_cast<uint2*>(dst) = make_uint2(attn8::half2_of(o.x * inv, o.y * inv), attn8::half2_of(o.z * inv, o.w * inv));
 }
@@ -957,7 +958,7 @@ inline Layout layout(int ctas, std::uint64_t head_dim, std::uint64_t rows) {
     l.joins = l.few_parts + static_cast<std::uint64_t>(ctas) * 2 * few::kCols * (rows <= few::kCols ? 1 : few::kMaxSets) * (head_dim + 2) * 4;
     l.parts = l.bytes = l.joins;
     if (rows > few::kMostRows) {
-        l.parts = l.joins + kMaxCtas * sizeof(Join);
+        l.parts = l.joins + kMaxCtas * sizeof(Join);  // a multiple of 16
         l.bytes = l.parts + static_cast<std::uint64_t>(ctas) * 2 * 256 * (head_dim + 2) * 4;
     }
     return l;

@@ -291,6 +291,40 @@ def test_a_query_of_nan_or_infinity_is_its_own(ctx, new):
     check_attention(got, want, mag)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,past", [([1], [40]), ([3], [5000]), ([90], [20]), ([40], [9000]), ([50, 1], [4000, 80])])
+def test_scores_of_minus_infinity_alone_are_no_mask(ctx, hd, new, past):
+    """Positions are attended whose scores are all -infinity: 0 / 0, and not the zeros
+    of a query that attends nothing.  A finite score among them takes it all."""
+    t = inputs(new, past, 4, 1, hd, 16, 41, unused=0.0)
+    t["q"][:] = 1.0
+    t["k_cache"][..., 0] = -np.inf
+    assert np.isnan(run(ctx, t)).all()
+    for b, n in enumerate(t["lens"]):  # position 2 of each sequence
+        t["k_cache"][t["table"][b, 0], :, 2] = 0.5
+    got = run(ctx, t)
+    for b, n in enumerate(t["lens"]):
+        rows = got[t["starts"][b]:t["starts"][b + 1]]
+        assert (rows == t["v_cache"][t["table"][b, 0], 0, 2]).all()
+
+
+def test_positions_up_to_two_to_the_31st(ctx):
+    """A length whose last unit of positions ends at 2^31, all pages one block.  Scores
+    of -20 everywhere: positions behind the last one, had they weight e^0, would be
+    four times as heavy as all of the sequence.  Weights are equal, so the result is
+    the mean of V, here 1."""
+    length = 0x7ffffff0
+    t = {"q": put(ctx, np.full((1, 1, 64), 1.0, np.float16)),
+         "k_cache": put(ctx, np.full((1, 1, 16, 64), -2.5, np.float16)),
+         "v_cache": put(ctx, np.full((1, 1, 16, 64), 1.0, np.float16)),
+         "table": put(ctx, np.zeros((1, length // 16), np.int32)),
+         "starts": put(ctx, np.array([0, 1], np.int32)),
+         "lens": put(ctx, np.array([length], np.int32)),
+         "out": put(ctx, np.zeros((1, 1, 64), np.float16))}
+    launch(ctx, t, 1)  # -2.5 * 64 / 8 = -20
+    assert (get(ctx, t["out"]) == 1.0).all()
+
+
 def test_offsets_past_32_bits(ctx):
     """Caches of more than 2^32 values: rows in the last blocks."""
     kvh, block, hd = 8, 256, 128
