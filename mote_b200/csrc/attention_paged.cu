@@ -8,10 +8,13 @@
 // Two kernels, each for its own sequences of a batch (the lengths are on the
 // device): this file's for sequences with up to 16 query rows (tokens times grouped
 // heads of a KV head), whose cost is the stream of K and V;
-// attention_paged_chunk.cu's for more, on the tcgen05 tensor cores.  Where a batch may hold both, the kernels run at the same time, on SMs
-// that they divide by the work that each has (few_ctas).
+// attention_paged_chunk.cu's for more, on the tcgen05 tensor cores.  Where a batch may
+// hold both, the kernels run at the same time, on SMs that they divide by the work that
+// each has (few_ctas).
 //
-// Few rows: HBM-bound, K and V of the attended positions are read once.
+// Few rows: HBM-bound, K and V of the attended positions are read once.  48 sequences of
+// up to 8192 (773 MB, 32 query / 8 KV heads of 128): 122-126 us, 0.94-0.97 of the copy bandwidth;
+// one of 32768 (134 MB): 29.4, of which about 10 are the start and the join.
 // * The work is cut in units of 8 KB of K and V (16 positions at head_dim 128, 32
 //   at 64) of one (sequence, KV head) "row".  One CTA per SM takes an equal share
 //   of consecutive units, found from the lengths on the device, so ragged batches
@@ -21,7 +24,7 @@
 //   of 16 positions x 128 bytes, 128-byte swizzle: ldmatrix meets all banks).
 // * mma.sync m16n8k16 with the cache as the A operand: S^T = K Q^T with 16
 //   positions as rows and 8 (token, head) pairs as columns, then O^T += V^T P^T with
-//   16 dimensions as rows, so that 8 columns cost no idle rows; up to four sets of
+//   16 dimensions as rows, so that 8 columns cost no idle rows; up to two sets of
 //   8 columns share the operand.  P^T gets from the accumulator layout to the
 //   operand's with movmatrix.
 // * The running maximum moves only when a lane's sum of P passes 2^8, so a step
@@ -97,10 +100,10 @@ constexpr std::uint32_t kEnd = 256;
 // A sequence's pairs on that line, for one KV head.
 struct Pairs {
     Seq s;
-    std::uint32_t span;   // tokens of a pair
+    std::uint32_t tile, span;  // tokens of a query tile and of a pair
     std::uint32_t count;  // pairs
 
-    __device__ __forceinline__ Pairs(const Params& p, const Seq& of) : s(of), span(2 * p.tile_tokens) {
+    __device__ __forceinline__ Pairs(const Params& p, const Seq& of) : s(of), tile(p.tile_tokens), span(2 * p.tile_tokens) {
         if (static_cast<std::uint64_t>(s.n) * p.group <= p.few) s.n = 0;
         count = (s.n + span - 1) / span;
     }
@@ -122,22 +125,31 @@ struct Pairs {
         return i < count || count == 0 ? x : x + extent(count - 1);
     }
     __device__ __forceinline__ std::uint64_t all() const { return before(count); }
+    // how long they take, in positions of a pair of two tiles: one tile takes three
+    // quarters of it
+    __device__ __forceinline__ std::uint64_t cost() const {
+        return all() - (count > 0 && s.n - (count - 1) * span <= tile ? extent(count - 1) / 4 : 0u);
+    }
 };
 
 // The chunk kernel's work of a sequence.
-__device__ __forceinline__ std::uint64_t line_of(const Params& p, const Seq& s) {
-    return Pairs(p, s).all() * p.c.kv_heads;
-}
+__device__ __forceinline__ std::uint64_t cost_of(const Params& p, const Seq& s) { return Pairs(p, s).cost() * p.c.kv_heads; }
 // SMs of `n` that the few-row kernel has where both run, from its work (units, row
-// ends counted) and the other's (positions): a unit takes an SM about as long as
-// kUnitCost positions of a pair.  In f32, of which both kernels make the same.
-constexpr float kUnitCost = 11.f;
-__device__ __forceinline__ std::uint32_t few_ctas(std::uint32_t n, std::uint64_t units, std::uint64_t line) {
-    if (line == 0) return n;
+// ends counted) and the other's (cost): a unit takes an SM about as long as kUnitCost
+// positions of a pair, 160 ns to 20 at head_dim 128 and 16 at 64 (32 tokens over up to
+// 4000 beside a chunk of 512 at head_dim 64: 70 us, 88 with half of it and 89 with twice;
+// 23 over 3000 at 128: 93, 101 with one more).  On more than 7/8 of the SMs it would wait
+// for HBM (38 over 8000 beside two chunks of 100: 239, 287 on 128 SMs and 464 on 137).
+// In f32, of which both kernels make the same.
+template <int HD>
+constexpr float kUnitCost = HD == 128 ? 8.f : 10.f;
+template <int HD>
+__device__ __forceinline__ std::uint32_t few_ctas(std::uint32_t n, std::uint64_t units, std::uint64_t cost) {
+    if (cost == 0) return n;
     if (units == 0) return 0;
-    const float mine = __fmul_rn(__ull2float_rn(units), kUnitCost), all = __fadd_rn(mine, __ull2float_rn(line));
+    const float mine = __fmul_rn(__ull2float_rn(units), kUnitCost<HD>), all = __fadd_rn(mine, __ull2float_rn(cost));
     const std::uint32_t x = __float2uint_rn(__fmul_rn(__fdiv_rn(mine, all), static_cast<float>(n)));
-    return min(max(x, 1u), n - 1);
+    return min(max(x, 1u), n - max(n / 8, 1u));
 }
 // A share of `total` over `ctas`, rounded up (by up to 2^-22 of it).
 __device__ __forceinline__ std::uint64_t share_of(std::uint64_t total, std::uint32_t ctas) {
@@ -155,10 +167,13 @@ constexpr int kStage = 4 * kBox; // K and V of a unit
 constexpr int kStages = 3;
 constexpr int kMaxCtas = 192;
 constexpr int kMinUnits = 2 * kWarps;  // rows of up to this many units are not split
-// Sequences up to which every warp finds the CTA's share alone, one to a lane.
+// Sequences up to which every warp finds the CTA's share alone, one to a lane: 16 x 4096
+// at head_dim 64 26.2 us, 29.6 with the CTA's warps together (one row of 32768 29.8, 30.7).
 constexpr std::uint32_t kFew = 32;
-// What a row's end costs a CTA, in units.
-constexpr int kRowCost = 14;
+// What a row's end costs a CTA, in units: among shares (with 14: 16 x 4000 with 3 drafted
+// tokens 52.2 us, 48.1 now; with none, a row of 32768 31.6, 29.4 now), and between the two kernels (with 20: 23 single tokens over 3000 beside
+// a chunk of 512 97.9 us, 93.4 now).
+constexpr int kRowCost = 20, kSplitRowCost = 14;
 
 template <int HD>
 struct Smem {
@@ -414,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // CTA, of the smallest size (in small steps) that needs no more CTAs than
     // there are, unless shares are smaller by more than a row's end.
     std::uint32_t longest = 0, filled = 0;  // units, rows with any
-    std::uint64_t total = 0, line = 0;      // units, and the other kernel's work
+    std::uint64_t total = 0, line = 0;      // units, and the other kernel's cost
     std::uint32_t per = 0;  // units of a CTA
     std::uint32_t ctas = gridDim.x;
     bool pieces = false;
@@ -453,13 +468,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (static_cast<std::uint32_t>(lane) < batch) {
             const Seq s = sequence(p, lane);
             n = units(few_part(p, s));
-            if (p.shares) line = line_of(p, s);
+            if (p.shares) line = cost_of(p, s);
         }
         if (p.shares) line = __shfl_sync(0xffffffffu, scan_up(line), 31);
         longest = __reduce_max_sync(0xffffffffu, n);
         total = static_cast<std::uint64_t>(__reduce_add_sync(0xffffffffu, n)) * rows;
         filled = __popc(__ballot_sync(0xffffffffu, n > 0)) * rows;
-        if (p.shares) ctas = few_ctas(ctas, total + static_cast<std::uint64_t>(filled) * kRowCost, line);
+        if (p.shares) ctas = few_ctas<HD>(ctas, total + static_cast<std::uint64_t>(filled) * kSplitRowCost, line);
         if (total == 0 || blockIdx.x >= ctas) return;
         per = share();
         if (filled <= ctas) {
@@ -488,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (std::uint32_t b = threadIdx.x; b < batch; b += kThreads) {
             const Seq s = sequence(p, b);
             const std::uint32_t n = units(few_part(p, s));
-            if (p.shares) line += line_of(p, s);
+            if (p.shares) line += cost_of(p, s);
             total += n;
             filled += n > 0;
             longest = max(longest, n);
@@ -515,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         total *= rows;
         filled *= rows;
         __syncthreads();
-        if (p.shares) ctas = few_ctas(ctas, total + static_cast<std::uint64_t>(filled) * kRowCost, line);
+        if (p.shares) ctas = few_ctas<HD>(ctas, total + static_cast<std::uint64_t>(filled) * kSplitRowCost, line);
         if (total == 0 || blockIdx.x >= ctas) return;
         per = share();
         if (filled <= ctas) {
@@ -683,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 limit[c][h] = static_cast<std::int32_t>(seq.len - seq.n + tok + 1);
             }
         }
-        // positions that every column attends, and the first that is looked through
+        // positions that every column attends: what follows is looked through
         const std::uint32_t all = static_cast<std::uint32_t>(max(static_cast<std::int32_t>(seq.len - seq.n + 1), 0));
         bool bad = false;
         for (std::uint32_t v = v0 + warp; v < v1; v += kWarps) {
@@ -912,10 +927,10 @@ inline int sm_count(int& n) {
 
 namespace few {
 
-// Query rows of a KV head that the kernel takes: with four sets of columns 16
-// sequences of 4000 with 5 and 8 tokens of 4 grouped heads took 98 and 104 us at
-// head_dim 128 (registers spill), the chunk kernel 71 and 72; at head_dim 64 (32 of
-// 4000, 6 tokens) 73 against 80.
+// Query rows of a KV head that the kernel takes.  With four sets of columns 16 sequences
+// of 4000 with 5 and 8 tokens of 4 grouped heads took 98 and 104 us at head_dim 128
+// (registers spill), the chunk kernel takes 72 and 73; at head_dim 64 (32 of 4000, 6
+// tokens) 73 against 96, for which alone more code is not kept.
 constexpr std::uint32_t kMostRows = kCols * kMaxSets;
 
 template <int HD, int SETS>

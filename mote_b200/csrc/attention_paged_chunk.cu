@@ -12,7 +12,7 @@
 // * warps 9 and 10 issue the products, each for its query tile m: S_m = Q_m K^T and
 //   O_m += P_m V (P from tensor memory).  One warp for both had to take them in turn,
 //   and an MMA costs its warp 30 to 60 cycles to issue: chunk of 2048 over 16384 at
-//   head_dim 128 652 us, 590 with two;
+//   head_dim 128 688 us, 633 with two (and turns, below);
 // * warps 0-3 and 4-7 run the softmax of the two query tiles, one thread per row: the
 //   maximum moves (and O_m is rescaled) only when a score passes it by more than 8 in
 //   log2 units.  P is rounded to f16 (11 bits down to 2^-21 of the row's largest);
@@ -22,6 +22,11 @@
 //   positions, and the rows of a page behind the last position): 0 times an infinity
 //   or NaN would be NaN.  The rows that do attend such values add them at the end
 //   (rare, from global memory).
+// What bounds it: at head_dim 128 the chain S -> maximum -> exponentials -> P V of two
+// query tiles, under the power cap in long runs (chunk of 2048 over 16384: 583 GFLOP in 633
+// us, 0.57 of the measured tensor rate; 580 on a cooler GPU); at 64 the same chain and the
+// exp2 unit (six chunks of 300 to 1024 over up to 2500: 104 us, exp2 44 % of the cycles,
+// tensor pipe 22 %).
 // Every wait is bounded; an expired wait aborts the CTA, which waits for its issued
 // MMAs (bounded) and frees its tensor memory.  No load uses cluster multicast.
 //
@@ -65,9 +70,11 @@ using attnv::v_desc;
 using gemm::wait_or_abort;
 
 constexpr int kMaxCtas = 192;
-// The least share, in positions, and the least piece of a pair, in K/V tiles.
-constexpr std::uint64_t kLeast = 1024;
-constexpr std::uint32_t kMinTiles = 3;
+// The least share, in positions, and the least piece of a pair, in K/V tiles (1024 and 3:
+// 8 sequences of 8000 with one token of 32 query heads on one KV head 30.5 us, 22.9 now;
+// 16 of 4000 with 5 tokens 73.5 and 71.5).
+constexpr std::uint64_t kLeast = 512;
+constexpr std::uint32_t kMinTiles = 1;
 
 // One MMA, issued by the lane whose `lead` is set; all lanes of the (converged) warp
 // run through it, without a branch.
@@ -139,8 +146,8 @@ struct Smem {
     static constexpr int kFlag = kAbort + 4;          // [kFlags]
     static constexpr int kItem = kFlag + 4 * kFlags;  // [kItems]
     static constexpr int kShare = (kItem + kItems * static_cast<int>(sizeof(Item)) + 7) / 8 * 8;  // first sequence, its begin
-    static constexpr int kScan = kShare + 2 * 8;      // [warp][2] sums
-    static constexpr int kTurn = kScan + kThreads / 32 * 16;  // [query tile][warp] passes whose exponentials are done
+    static constexpr int kScan = kShare + 2 * 8;      // [warp][3] sums
+    static constexpr int kTurn = kScan + kThreads / 32 * 24;  // [query tile][warp] passes whose exponentials are done
     static constexpr int kUsed = kTurn + 8 * 4 + 1008;  // + alignment slack
     // one CTA per SM: its 512 TMEM columns never wait for another's
     static constexpr int kBytes = kUsed > 120 * 1024 ? kUsed : 120 * 1024;
@@ -247,7 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // ---- the CTA's share of the line ---------------------------------------
     // first sequence (~0: none), length of a share, where the sequence begins; by the
-    // producer alone for up to 32 sequences, by all otherwise
+    // producer alone for up to 32 sequences, by all otherwise (8 tokens over 30000 40.2 us,
+    // 41.0 by all)
     const std::uint32_t batch = p.c.batch;
     std::uint64_t first_b = ~0ull, per = 0, first_begin = 0;
     const auto scan_up = [&](std::uint64_t x) {  // inclusive, over the warp
@@ -258,19 +266,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         return x;
     };
-    // this kernel's work of sequence b, and the other's
-    const auto work_of = [&](std::uint32_t b, std::uint64_t& units) -> std::uint64_t {
+    // this kernel's work of sequence b, its cost and the other's work
+    const auto work_of = [&](std::uint32_t b, std::uint64_t& cost, std::uint64_t& units) -> std::uint64_t {
         if (b >= batch) return 0;
         const Seq s = sequence(p, b);
         if (p.shares) {
+            cost += cost_of(p, s);
             const std::uint32_t n = few::units_of<HD>(few::few_part(p, s));
-            units += n == 0 ? 0ull : (static_cast<std::uint64_t>(n) + few::kRowCost) * p.c.kv_heads;
+            units += n == 0 ? 0ull : (static_cast<std::uint64_t>(n) + few::kSplitRowCost) * p.c.kv_heads;
         }
-        return line_of(p, s);
+        return Pairs(p, s).all() * p.c.kv_heads;
     };
     // sets `per`; whether the CTA has a share
-    const auto divide = [&](std::uint64_t total, std::uint64_t units) {
-        const std::uint32_t ctas = p.shares ? gridDim.x - few_ctas(gridDim.x, units, total) : gridDim.x;
+    const auto divide = [&](std::uint64_t total, std::uint64_t cost, std::uint64_t units) {
+        const std::uint32_t ctas = p.shares ? gridDim.x - few_ctas<HD>(gridDim.x, units, cost) : gridDim.x;
         if (blockIdx.x >= ctas) return false;
         per = share_of(total, ctas);
         if (per < kLeast) per = kLeast;
@@ -278,10 +287,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     if (__builtin_expect(batch <= 32, 1)) {
         if (warp == kProducerWarp) {
-            std::uint64_t units = 0;
-            const std::uint64_t mine = work_of(lane, units), incl = scan_up(mine);
-            if (p.shares) units = __shfl_sync(0xffffffffu, scan_up(units), 31);
-            if (divide(__shfl_sync(0xffffffffu, incl, 31), units)) {
+            std::uint64_t cost = 0, units = 0;
+            const std::uint64_t mine = work_of(lane, cost, units), incl = scan_up(mine);
+            if (p.shares) {
+                cost = __shfl_sync(0xffffffffu, scan_up(cost), 31);
+                units = __shfl_sync(0xffffffffu, scan_up(units), 31);
+            }
+            if (divide(__shfl_sync(0xffffffffu, incl, 31), cost, units)) {
                 const std::uint64_t at = per * blockIdx.x;
                 const unsigned here = __ballot_sync(0xffffffffu, incl - mine <= at && at < incl);
                 if (here != 0) {
@@ -293,22 +305,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else {
         volatile std::uint64_t* share = reinterpret_cast<volatile std::uint64_t*>(smem + L::kShare);
         volatile std::uint64_t* scan = reinterpret_cast<volatile std::uint64_t*>(smem + L::kScan);
-        std::uint64_t sum = 0, units = 0;
-        for (std::uint32_t b = threadIdx.x; b < batch; b += kThreads) sum += work_of(b, units);
-        sum = scan_up(sum), units = scan_up(units);
-        if (lane == 31) scan[2 * warp] = sum, scan[2 * warp + 1] = units;
+        std::uint64_t sum = 0, cost = 0, units = 0;
+        for (std::uint32_t b = threadIdx.x; b < batch; b += kThreads) sum += work_of(b, cost, units);
+        sum = scan_up(sum), cost = scan_up(cost), units = scan_up(units);
+        if (lane == 31) scan[3 * warp] = sum, scan[3 * warp + 1] = cost, scan[3 * warp + 2] = units;
         if (threadIdx.x == 0) share[0] = ~0ull;
         __syncthreads();
-        std::uint64_t total = 0, all_units = 0;
+        std::uint64_t total = 0, all_cost = 0, all_units = 0;
 #pragma unroll
-        for (int w = 0; w < kThreads / 32; ++w) total += scan[2 * w], all_units += scan[2 * w + 1];
+        for (int w = 0; w < kThreads / 32; ++w) total += scan[3 * w], all_cost += scan[3 * w + 1], all_units += scan[3 * w + 2];
         __syncthreads();
-        if (divide(total, all_units)) {
+        if (divide(total, all_cost, all_units)) {
             const std::uint64_t at = per * blockIdx.x;
             std::uint64_t before = 0;
             for (std::uint32_t base = 0; base < batch && before <= at; base += kThreads) {
-                std::uint64_t none = 0;
-                const std::uint64_t mine = work_of(base + threadIdx.x, none), incl = scan_up(mine);
+                std::uint64_t cost = 0, units = 0;
+                const std::uint64_t mine = work_of(base + threadIdx.x, cost, units), incl = scan_up(mine);
                 if (lane == 31) scan[warp] = incl;
                 __syncthreads();
                 std::uint64_t lower = before;
