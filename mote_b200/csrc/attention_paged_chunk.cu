@@ -884,7 +884,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (p.shares && blockIdx.x == 0) pdl_wait();
 }
 
-
 // Adds up the parts of the pairs that lie in several CTAs, in order: a CTA takes 32
 // rows and 32 dimensions of one pair, or returns where there is none.  One pass, the
 // sums moving with the largest maximum so far, so that many parts load at a time.
