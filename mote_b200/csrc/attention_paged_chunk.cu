@@ -63,7 +63,6 @@ using attnv::kShift;
 using attnv::kSoftmaxRegs;
 using attnv::kThreads;
 using attnv::kTmemCols;
-using attnv::kVast;
 using attnv::tmem_ld16;
 using attnv::tmem_st16;
 using attnv::v_desc;
@@ -75,6 +74,11 @@ constexpr int kMaxCtas = 192;
 // 16 of 4000 with 5 tokens 73.5 and 71.5).
 constexpr std::uint64_t kLeast = 512;
 constexpr std::uint32_t kMinTiles = 1;
+// score * scale - reference is one fma with the rounded reference, off by up to 2^-24 of
+// it; beyond this (log2 units) the reference is subtracted from the scores instead.  Equal
+// scores meet under different references, where a row's moves and where its parts are
+// joined: near 35000 their weights were up to 2^-8 apart (log2), at 1024 it is 2^-13.
+constexpr float kVast = 1024.f;
 
 // One MMA, issued by the lane whose `lead` is set; all lanes of the (converged) warp
 // run through it, without a branch.
