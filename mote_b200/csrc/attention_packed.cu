@@ -75,9 +75,11 @@ constexpr int kItems = 4;          // items that the producer may be ahead
 // 2^-14 and 2^-24, where a large V of little weight lost its bits).
 constexpr float kShift = 7.f;
 // score * scale - reference * scale is one fma, whose rounded second product
-// leaves up to 2^-25 of it; references beyond this (log2 units) are subtracted
-// from the scores instead, so that the largest of any size weighs 1.
-constexpr float kVast = 65536.f;
+// leaves up to 2^-24 of it; references beyond this (log2 units) are subtracted
+// from the scores instead.  Equal scores meet under different references where a
+// row's moves: near 35000 their weights were up to 2^-8 apart (log2), at 1024 it is
+// 2^-13.
+constexpr float kVast = 1024.f;
 // Sequences up to which items are ranked by size: 8 to a lane of the producer
 // warp, in registers.  Ranked against in the order of the sequences: 12 prompts
 // of 60 to 1000 57 against 62 us, 64 of 50 to 100 over 2000 cached 108 against
