@@ -579,10 +579,10 @@ int mote_cuda_rope_kv_cache_append_paged_f16(
  * stands at position seq_lens[b] - n + i:
  *   out[i, h] = softmax_{p <= len - n + i}(scale * q[i, h] . K[p, h / g]) . V[p, h / g]
  * One token of a running sequence, a few drafted ones and chunks of prompts may
- * be mixed.  max_new: the most tokens that any sequence has.  A query before the
- * first position gets zeros; rows of no sequence keep their values; what the
- * cache holds past a query's position does not reach it (infinities and NaN
- * either).  A sequence whose offsets or length are out of range, or that has
+ * be mixed.  max_new: the most tokens that any sequence has (kernels are chosen
+ * by the smaller of it and tokens).  A query before the first position gets
+ * zeros; rows of no sequence keep their values; what the cache holds past a
+ * query's position does not reach it (infinities and NaN either).  A sequence whose offsets or length are out of range, or that has
  * more than max_new tokens, is skipped; a block outside [0, num_blocks) reads
  * as zeros; both set bit 1 of the device status.  q_heads a multiple of
  * kv_heads and at most 128 times it, q_heads <= 65535, scale finite and > 0,

@@ -1024,8 +1024,8 @@ extern "C" int mote_cuda_gqa_attention_paged_f16(
     int st = sm_count(n);
     if (st != kSuccess) return st;
     if (n > few::kMaxCtas) n = few::kMaxCtas;
-    const std::uint64_t group = q_heads / kv_heads, rows = max_new * group;
-    const chunk::Layout at = chunk::layout(n, head_dim, rows);
+    const std::uint64_t group = q_heads / kv_heads;
+    const chunk::Layout at = chunk::layout(n, head_dim, max_new * group);
     if (workspace == nullptr || workspace_bytes < at.bytes || !kvq8::aligned16({workspace}))
         return kInvalidValue;
     std::uint8_t* const ws = static_cast<std::uint8_t*>(workspace);
@@ -1047,7 +1047,10 @@ extern "C" int mote_cuda_gqa_attention_paged_f16(
     p.reports = true;
     const auto s = static_cast<cudaStream_t>(stream);
     // Both kernels where the host cannot tell that one of them has nothing to do: a
-    // single sequence, or groups too large for the few-row kernel, are the other's.
+    // single sequence, or groups too large for the few-row kernel, are the other's.  No
+    // sequence has more tokens than there are (one call alone, one token over 32768 with
+    // max_new 64: 33 us, 47 when max_new alone decided; over 117 10.2 and 18.4).
+    const std::uint64_t rows = (max_new < tokens ? max_new : tokens) * group;
     const bool chunks = rows > few::kMostRows;
     p.few = chunks && (batch == 1 || group > few::kMostRows) ? 0u : few::kMostRows;
     p.shares = chunks && p.few != 0;

@@ -1061,14 +1061,15 @@ def gqa_attention_paged_f16(context: CudaContext, q: Tensor, k_cache: Tensor, v_
     [tokens, q_heads, head_dim] f16, the last of its ``seq_lens[b]`` cached
     positions (their K and V already appended).  One token of a running
     sequence, a few drafted ones and chunks of prompts may be mixed;
-    ``max_new`` is the most that any sequence has.  A query before the first
-    position gets zeros; rows of no sequence keep their values.  A sequence
-    whose offsets or length are out of range, or with more than ``max_new``
-    tokens, is skipped, and a block out of range reads as zeros; both set the
-    device status.  ``scale`` defaults to ``1 / sqrt(head_dim)``.  The parts
-    of long rows meet in a workspace of the context, so calls of one context
-    (replays of its captured graphs among them) must not overlap; the first
-    call that needs a larger workspace comes before any graph capture."""
+    ``max_new`` is the most that any sequence has (kernels are chosen by the
+    smaller of it and ``tokens``).  A query before the first position gets
+    zeros; rows of no sequence keep their values.  A sequence whose offsets or
+    length are out of range, or with more than ``max_new`` tokens, is skipped,
+    and a block out of range reads as zeros; both set the device status.
+    ``scale`` defaults to ``1 / sqrt(head_dim)``.  The parts of long rows meet
+    in a workspace of the context, so calls of one context (replays of its
+    captured graphs among them) must not overlap; the first call that needs a
+    larger workspace comes before any graph capture."""
     blocks, kvh, bt, hd = cache = _dims(k_cache, "k_cache", 4)
     batch, width = tables = _dims(block_tables, "block_tables", 2)
     tokens, qh, _ = _dims(q, "q", 3)
