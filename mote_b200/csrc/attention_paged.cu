@@ -430,19 +430,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     // there are, unless shares are smaller by more than a row's end.
     std::uint32_t longest = 0, filled = 0;  // units, rows with any
     std::uint64_t total = 0, line = 0;      // units, and the other kernel's cost
-    std::uint32_t per = 0;  // units of a CTA
+    std::uint64_t per = 0;  // units of a CTA (past 2^32 where pages are shared without measure)
     std::uint32_t ctas = gridDim.x;
     bool pieces = false;
     const auto least = [&] { return min(longest, static_cast<std::uint32_t>(kMinUnits)); };
     const auto share = [&] {
-        return max(static_cast<std::uint32_t>(share_of(total + static_cast<std::uint64_t>(filled) * kRowCost, ctas)), least());
+        return max(share_of(total + static_cast<std::uint64_t>(filled) * kRowCost, ctas), static_cast<std::uint64_t>(least()));
     };
     const auto size = [&](std::uint32_t i, std::uint32_t steps) {  // pieces from the least on
         const std::uint32_t low = max(static_cast<std::uint32_t>(share_of(total, ctas)), least());
         return low + (low * i + steps - 1) / steps;
     };
     const auto extent = [&](std::uint32_t n) -> std::uint32_t {  // a row in virtual units
-        return pieces ? (n + per - 1) / per * per : n == 0 ? 0 : n + kRowCost;
+        const std::uint32_t piece = static_cast<std::uint32_t>(per);  // (of a row: at most 2^28)
+        return pieces ? (n + piece - 1) / piece * piece : n == 0 ? 0 : n + kRowCost;
     };
     // sequences without positions
     for (std::uint32_t b = blockIdx.x; b < batch; b += gridDim.x) {
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             pieces = fits != 0 && best <= per + kRowCost;
             if (pieces) per = best;
         }
-        u0 = static_cast<std::uint64_t>(per) * blockIdx.x;
+        u0 = per * blockIdx.x;
         const std::uint64_t ext = extent(n), incl = scan_up(ext);
         const std::uint64_t begin = (incl - ext) * rows;
         const unsigned here = __ballot_sync(0xffffffffu, n > 0 && begin <= u0 && u0 < incl * rows);
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (pieces) per = size(w, kWarps);
             __syncthreads();
         }
-        u0 = static_cast<std::uint64_t>(per) * blockIdx.x;
+        u0 = per * blockIdx.x;
         std::uint64_t before = 0;  // extents of the sequences before the chunk
         if (threadIdx.x == 0) found[1] = 0;
 
