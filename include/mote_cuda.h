@@ -586,9 +586,9 @@ int mote_cuda_rope_kv_cache_append_paged_f16(
  * whose offsets or length are out of range, or that has more than max_new
  * tokens, is skipped; a block outside [0, num_blocks) reads as zeros; both set
  * bit 1 of the device status.  q_heads a multiple of kv_heads and at most 128
- * times it, q_heads <= 65535, scale finite and > 0, num_blocks * kv_heads *
- * block_tokens <= 0x7fffff00; out must not overlap q or the caches; tokens == 0
- * returns 0.
+ * times it, q_heads <= 65535, scale > 0 and scale * log2(e) finite in f32,
+ * num_blocks * kv_heads * block_tokens <= 0x7fffff00; out must not overlap q or
+ * the caches; tokens == 0 returns 0.
  *
  * The workspace (16-byte aligned, at least ..._workspace_bytes for the current
  * device: 0 for shapes that are refused; missing or smaller -> 1) holds 768 bytes

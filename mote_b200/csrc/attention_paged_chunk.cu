@@ -1014,8 +1014,9 @@ extern "C" int mote_cuda_gqa_attention_paged_f16(
         return kInvalidValue;
     if (!kvq8::shape_ok(batch, kv_heads, head_dim, num_blocks, block_tokens, max_blocks) ||
         kv_heads == 0 || q_heads % kv_heads != 0 || q_heads > 65535 || q_heads / kv_heads > 128 ||
-        tokens > 0x7fffffffull || max_new > 0x7fffffffull || !std::isfinite(scale) ||
-        !(scale > 0.f) || !kvq8::aligned16({q, k_cache, v_cache, out}) ||
+        tokens > 0x7fffffffull || max_new > 0x7fffffffull || !(scale > 0.f) ||
+        !std::isfinite(scale * 1.4426950408889634f) ||  // (the kernels' factor)
+        !kvq8::aligned16({q, k_cache, v_cache, out}) ||
         !kvq8::aligned4({block_tables, q_starts, seq_lens}) ||
         num_blocks * kv_heads * block_tokens > kNowhere)  // below 2^55
         return kInvalidValue;
