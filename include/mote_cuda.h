@@ -591,11 +591,11 @@ int mote_cuda_rope_kv_cache_append_paged_f16(
  * the caches; tokens == 0 returns 0.
  *
  * The workspace (16-byte aligned, at least ..._workspace_bytes for the current
- * device: 0 for shapes that are refused; missing or smaller -> 1) holds 768 bytes
- * of counters, zeroed once before first use and left zero by every call, and
- * partial results.  One workspace, of the largest size needed, serves calls of any
- * shape that follow one another, captured graphs included; calls that may overlap
- * need one each. */
+ * device: 0 without heads or for a head_dim or max_new that is refused; missing
+ * or smaller -> 1) holds 768 bytes of counters, zeroed once before first use and
+ * left zero by every call, and partial results.  One workspace, of the largest
+ * size needed, serves calls of any shape that follow one another, captured graphs
+ * included; calls that may overlap need one each. */
 int mote_cuda_gqa_attention_paged_f16_workspace_bytes(uint64_t q_heads, uint64_t kv_heads,
                                                       uint64_t head_dim, uint64_t max_new,
                                                       uint64_t* bytes);

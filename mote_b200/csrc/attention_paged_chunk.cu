@@ -25,8 +25,8 @@
 // What bounds it: at head_dim 128 the chain S -> maximum -> exponentials -> P V of two
 // query tiles, under the power cap in long runs (chunk of 2048 over 16384: 583 GFLOP in 633
 // us, 0.57 of the measured tensor rate; 580 on a cooler GPU); at 64 the same chain and the
-// exp2 unit (six chunks of 300 to 1024 over up to 2500: 104 us, exp2 44 % of the cycles,
-// tensor pipe 22 %).
+// exp2 unit (six chunks of 300 to 1024 over up to 2500: 104 us, exp2 49 % of the cycles,
+// tensor pipe 24 %).
 // Every wait is bounded; an expired wait aborts the CTA, which waits for its issued
 // MMAs (bounded) and frees its tensor memory.  No load uses cluster multicast.
 //
@@ -482,6 +482,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     i = 0;
                     if (++kvh < p.c.kv_heads) continue;
                     kvh = 0;
+                    // (one sequence after another, 0.33 us each, while the tensor cores wait:
+                    // a chunk of 512 behind 400 single tokens 40 us, before them 148)
                     do {
                         if (++b >= p.c.batch) break;
                         x = Pairs(p, sequence(p, b));

@@ -87,7 +87,9 @@ __device__ __forceinline__ Place place_of(const Params& p, std::uint32_t t) {
 }
 
 // Pairs or head parts that are no whole 16-byte vectors, or tables that are not
-// aligned to them: one CTA for each token, element by element.
+// aligned to them: one CTA for each token, element by element.  The same rows with 60 or
+// 62 pairs of 64: 316 us in halves, 276 interleaved; 32 single rows 19-21 us on the device,
+// 3.2 in vectors.
 __global__ void __launch_bounds__(kThreads) append_scalar_kernel(const Params p) {
     pdl_launch_dependents();
     pdl_wait();
@@ -128,7 +130,8 @@ __device__ __forceinline__ float2 halves(std::uint32_t w) {
 }
 
 // HBM-bound: rows in 16-byte vectors, read and written once (14563 rows of 16 prompts, 32
-// query / 8 KV heads of 128, 366 MB: 63 us, 0.89 of the copy bandwidth).  `per_token` threads
+// query / 8 KV heads of 128, 366 MB: 63.6 us, 0.88 of the copy bandwidth; 67 and 75 with
+// half and a quarter of a head rotated in halves; 59 in interleaved pairs).  `per_token` threads
 // (32, 64 or 128) take a token.  Each keeps one place within a head (a vector and
 // its partner half a rotary width further, or one vector of interleaved pairs) with
 // the place's cosines and sines in registers, and goes through the heads; its first

@@ -283,7 +283,11 @@ __device__ unsigned g_device_status = 0;
 // calls pdl_wait() before it reads or writes memory the predecessor may
 // touch (the wait returns once the predecessor grid has completed and its
 // writes are visible), and pdl_launch_dependents() to let its own successor
-// be scheduled early.
+// be scheduled early.  One kernel does not: in a mixed call of the paged attention
+// chunk_kernel runs beside few_kernel, which is launched just before it and triggers
+// only behind its own wait, so what came before both is complete.  It reads that past
+// L1, writes other rows and another part of the workspace, and its CTA 0 waits at the
+// end, so that its completion is few_kernel's too.  No launch may come between the two.
 template <typename... KArgs, typename... Args>
 inline int launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t stream,
                       Args... args) {

@@ -12,9 +12,11 @@
 // crates/mote-backend-hip/src/rope.rs:66-82).
 //
 // An angle of a far position needs more than 32 bits before it is reduced to a
-// turn.  Frequencies are 64-bit fractions of a turn (off by 2^-53 of the frequency at
-// most), so position * frequency modulo 2^64 is the angle without its whole turns,
-// exactly, in three integer instructions; what is left of it to the nearest quarter
+// turn.  Frequencies are 64-bit fractions of a turn, so position * frequency modulo 2^64
+// is the angle without its whole turns, exactly, in three integer instructions.  A
+// frequency f is off by 2^-64 of a turn and, from exp2 and its argument in 64 bits, by up
+// to (4 + 3 ln(1 / f)) 2^-53 of itself: the angle by about position * 2^-51 at most, since
+// the low frequencies have the large share.  What is left of it to the nearest quarter
 // turn goes to f32 for the sine and cosine.  Results are within 2^-23 of the angle's
 // own up to positions of 2^26 or so.  65536 positions of 64 pairs: 8.2 us, 0.64 of the
 // copy bandwidth (about 28 instructions a pair take half of that; 11.7 us with products
