@@ -34,3 +34,19 @@ def test_ties_on_both_sides_of_a_new_maximum(ctx, hd):
     q, k, v = (x.astype(np.float16) for x in (q, k, v))
     check(attend(ctx, q, k, v, [0, n], [0, n], scale=1.0), q, k, v, [0, n], [0, n], scale=1.0)
     assert ctx.device_status() == 0
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scores_around_the_bound(ctx, hd):
+    """Rows side by side whose scores are s + c with c from -2047 to 2047: below and above
+    2^10 in log2 units, of both signs, within a warp's rows."""
+    n, qh = 600, 4
+    q, k, v = np.zeros((n, qh, hd)), np.zeros((n, 1, hd)), np.zeros((n, 1, hd))
+    q[..., 1], q[..., 2] = 1, np.random.default_rng(hd).integers(-2047, 2048, (n, qh))
+    k[..., 1], k[..., 2] = -64, 1
+    for p, s in ((10, -5.5), (140, 0.0), (270, 0.5), (400, 0.0), (500, 0.5)):
+        k[p, 0, 1] = s
+    v[140], v[400], v[270], v[500] = 1, -1, 0.25, -0.25
+    q, k, v = (x.astype(np.float16) for x in (q, k, v))
+    check(attend(ctx, q, k, v, [0, n], [0, n], scale=1.0), q, k, v, [0, n], [0, n], scale=1.0)
+    assert ctx.device_status() == 0

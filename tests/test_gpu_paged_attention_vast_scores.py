@@ -60,3 +60,15 @@ def test_ties_on_both_sides_of_a_new_maximum(ctx, hd, new):
     """Two equal scores, between them the largest, for which the running maximum moves:
     7.93 in log2 units above the first score, then 8.66."""
     verify(ctx, exact(new, 600, hd, {10: -5.5, 140: 0.0, 270: 0.5, 400: 0.0}, {140: 1.0, 400: -1.0}))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("new,past", [(1, 9000), (4, 9000), (61, 9000), (200, 600)])
+def test_scores_around_the_bound(ctx, hd, new, past):
+    """Rows side by side whose scores are s + c with c from -2047 to 2047: below and above
+    2^10 in log2 units, of both signs, within a warp's rows."""
+    scores = {10: -5.5, 140: 0.0, 270: 0.5, 400: 0.0, past - 100: 0.5}
+    t = exact(new, past, hd, scores, {140: 1.0, 270: 0.25, 400: -1.0, past - 100: -0.25})
+    t["q"][..., 0] = 0
+    t["q"][..., 2] = np.random.default_rng(new).integers(-2047, 2048, (new, 4))
+    verify(ctx, t)
